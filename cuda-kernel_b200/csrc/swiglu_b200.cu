@@ -15,6 +15,7 @@
 #include <numeric>
 #include <string>
 
+#include "host.h"
 #include "kernels.cuh"
 #include "layer.cuh"
 #include "registry.h"
@@ -25,7 +26,9 @@ namespace {
 
 thread_local std::string g_last_error;
 
-int fail(int status, const char* detail = nullptr) {
+}  // namespace
+
+int fail(int status, const char* detail) {
     g_last_error = swb_status_string(status);
     if (detail && *detail) {
         g_last_error += ": ";
@@ -39,6 +42,8 @@ int check_launch() {
     if (e != cudaSuccess) return fail(SWB_E_CUDA, cudaGetErrorString(e));
     return SWB_OK;
 }
+
+namespace {
 
 constexpr swb_config_t kConfigs[] = {
 #define SWB_META(ID, FAM, W, R, PK, U, CH, ST) {ID, FAM, W, R, PK, U, CH, ST},
@@ -67,12 +72,10 @@ const swb_config_t* find_config(int64_t id) {
 SWB_CONFIGS(SWB_CHECK)
 #undef SWB_CHECK
 
-// Shared-memory capacities of sm_100: 228 KB per SM, 227 KB opt-in per CTA,
-// 1 KB reserved per resident CTA.
-constexpr size_t kSmemPerSm = 233472;
-constexpr size_t kSmemPerCtaMax = 232448;
 // x is staged in shared memory by the LDG family while its fp32 copy fits this.
 constexpr size_t kXStageLimit = 96 * 1024;
+
+}  // namespace
 
 int sm_count() {
     static std::atomic<int> cache[64];
@@ -87,6 +90,8 @@ int sm_count() {
     if (dev < 64) cache[dev].store(n, std::memory_order_relaxed);
     return n;
 }
+
+namespace {
 
 // Raises a kernel's dynamic shared-memory limit once per device.
 template <typename Kernel>
@@ -588,10 +593,14 @@ int dispatch_layer(int64_t id, const LayerParams& L, const TpParams& tp, cudaStr
     return rc;
 }
 
+}  // namespace
+
 bool overlaps(const void* a, size_t abytes, const void* b, size_t bbytes) {
     const uintptr_t ap = reinterpret_cast<uintptr_t>(a), bp = reinterpret_cast<uintptr_t>(b);
     return ap < bp + bbytes && bp < ap + abytes;
 }
+
+namespace {
 
 Params make_params() {
     Params p;
@@ -659,6 +668,8 @@ const char* swb_status_string(int status) {
         case SWB_E_DEVICE: return "device-side error";
         case SWB_E_UNSUPPORTED: return "unsupported device";
         case SWB_E_WORKSPACE: return "intermediate size exceeds the built-in workspace";
+        case SWB_E_TYPE: return "unknown element type";
+        case SWB_E_ALIGNMENT: return "buffer not aligned";
         default: return "unknown status";
     }
 }
@@ -864,7 +875,9 @@ int swb_device_error(int clear, int* out) {
         e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof zero);
         if (e != cudaSuccess) return fail(SWB_E_CUDA, cudaGetErrorString(e));
     }
-    if (out) *out = v;
+    int more = 0;  // the other translation units' words
+    if (int rc = moe_device_error(clear, &more)) return rc;
+    if (out) *out = v | more;
     return SWB_OK;
 }
 

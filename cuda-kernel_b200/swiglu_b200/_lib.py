@@ -37,6 +37,19 @@ SWB_E_CUDA = 12
 SWB_E_DEVICE = 13
 SWB_E_UNSUPPORTED = 14
 SWB_E_WORKSPACE = 15
+SWB_E_TYPE = 16
+SWB_E_ALIGNMENT = 17
+SWB_F16 = 0
+SWB_BF16 = 1
+SWB_F32 = 2
+SWB_MX4_MAX_DIM = 1 << 20
+SWB_MX4_MAX_TOKENS = 1 << 24
+SWB_MOE_MAX_TOKENS = 64
+SWB_MOE_MAX_EXPERTS = 256
+SWB_MOE_MAX_TOPK = 16
+SWB_MOE_MAX_DIM = 100000
+SWB_MOE_MX4 = 1
+SWB_MOE_RENORMALIZE = 2
 SWB_NOALLOC_MAX_INTER = 65536
 SWB_TP_MAX_RANKS = 8
 SWB_LAYER_WORKSPACE_BYTES = 8192
@@ -77,6 +90,8 @@ _cublas = None
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
+_u = ctypes.c_uint
+_z = ctypes.c_size_t
 
 
 def _declare(L: ctypes.CDLL) -> ctypes.CDLL:
@@ -112,6 +127,11 @@ def _declare(L: ctypes.CDLL) -> ctypes.CDLL:
         "swb_swiglu_tp_out": ([_vp] * 7 + [_i64] * 4 + [ctypes.c_uint, _vp], _i),
         "swb_gate_epilogue": ([_vp, _vp, _vp, _vp, _vp, _i, _vp], _i),
         "swb_residual_epilogue": ([_vp, _vp, _vp, _i, _vp], _i),
+        "swb_mx4_quantize": ([_i, _vp, _i64, _vp, _vp, _i64, _i64, _vp], _i),
+        "swb_mx4_dequantize": ([_i, _vp, _vp, _vp, _i64, _i64, _i64, _vp], _i),
+        "swb_mx4_project": ([_i, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _u, _vp], _i),
+        "swb_moe_workspace_bytes": ([_i, _i, _i, _i], _z),
+        "swb_moe": ([_i, _u, _vp, _i64] + [_vp] * 10 + [_i] * 5 + [_vp, _z, _vp], _i),
         "swb_device_error": ([_i, ctypes.POINTER(_i)], _i),
     }
     for name, (args, res) in sig.items():

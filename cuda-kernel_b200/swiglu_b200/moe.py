@@ -1,0 +1,91 @@
+"""The SwiGLU layer as a mixture of experts, for up to 64 tokens, in one kernel (swb_moe).
+
+    logits = router x,  experts = the topk largest,  w = softmax
+    y_t = sum_j w_tj down_e (SiLU(gate_e x_t) * (up_e x_t))
+
+Ties go to the lowest index and a NaN logit counts as the largest. ``renormalize``: the
+softmax runs over the selected logits, so that a token's weights sum to one; else over all
+logits. Like ``swiglu_out`` the call adds no bias and no residual, writes buffers the caller
+owns, launches on the current CUDA stream and allocates nothing.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .binding import _check
+from .mx4 import _TYPES, _call, _check_packed
+
+MAX_TOKENS = _lib.SWB_MOE_MAX_TOKENS
+
+
+def moe_workspace(tokens: int, experts: int, topk: int, inter: int, device=None) -> torch.Tensor:
+    """A zeroed workspace for calls of up to these sizes, one per stream of calls (calls that may
+    overlap on the GPU, captured ones included, need one each)."""
+    n = _lib.lib().swb_moe_workspace_bytes(tokens, experts, topk, inter)
+    _check(n > 0, "invalid shape")
+    return torch.zeros(n, dtype=torch.uint8, device=device or "cuda")
+
+
+def moe_out(x: torch.Tensor, router: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor,
+            y: torch.Tensor, workspace: torch.Tensor, topk: int, *, renormalize: bool = True,
+            gate_scales: torch.Tensor | None = None, up_scales: torch.Tensor | None = None,
+            down_scales: torch.Tensor | None = None, ids: torch.Tensor | None = None,
+            weights: torch.Tensor | None = None) -> None:
+    """The layer into ``y`` [tokens, hidden].
+
+    x: [tokens, hidden] fp16 or bf16, rows contiguous; router: [experts, hidden] of x's type;
+    gate, up: [experts, inter, hidden] and down: [experts, hidden, inter] of x's type, or all
+    three four-bit codes with their scales (``mx4_quantize``; inter is then read from gate).
+    ids [tokens, topk] int32 and weights [tokens, topk] fp32 receive the selection.
+    """
+    _check(x.is_cuda and x.dtype in (torch.float16, torch.bfloat16) and x.dim() == 2,
+           "x must be a CUDA FP16 or BF16 matrix")
+    device, dtype = x.device, x.dtype
+    tokens, hidden = x.shape
+    pitch = x.stride(0) if tokens > 1 else hidden
+    _check((hidden <= 1 or x.stride(1) == 1) and pitch >= hidden, "x must have contiguous rows")
+    _check(router.dim() == 2 and router.size(1) == hidden, "router must be [experts, hidden]")
+    _check(gate.dim() == 3, "gate must be [experts, inter, hidden]")
+    experts, inter = router.size(0), gate.size(1)
+    four_bit = gate_scales is not None
+    _check(four_bit == (up_scales is not None) == (down_scales is not None),
+           "scales belong to all three matrices or to none")
+    if four_bit:
+        for codes, scales, shape in ((gate, gate_scales, (experts, inter, hidden)),
+                                     (up, up_scales, (experts, inter, hidden)),
+                                     (down, down_scales, (experts, hidden, inter))):
+            _check_packed(codes, scales, shape, device)
+        typed = (router, y)
+    else:
+        _check(gate.shape == (experts, inter, hidden) and up.shape == gate.shape
+               and down.shape == (experts, hidden, inter), "incompatible weights")
+        typed = (router, y, gate, up, down)
+    for t in typed:
+        _check(t.dtype == dtype and t.device == device and t.is_contiguous(),
+               "router, weights and y must be contiguous, of x's type and on its device")
+    for t in (x, *typed):
+        _check(not t.requires_grad, "inference only: disable gradients")
+    _check(y.shape == x.shape, "y must have x's shape")
+    _check(workspace.device == device and workspace.dtype == torch.uint8 and workspace.is_contiguous(),
+           "workspace must come from moe_workspace on x's device")
+    for t, kind, name in ((ids, torch.int32, "ids"), (weights, torch.float32, "weights")):
+        if t is not None:
+            _check(t.dtype == kind and t.device == device and t.is_contiguous()
+                   and tuple(t.shape) == (tokens, topk), f"{name} must be contiguous [tokens, topk]")
+    flags = (_lib.SWB_MOE_MX4 if four_bit else 0) | (_lib.SWB_MOE_RENORMALIZE if renormalize else 0)
+    _call(device, _lib.lib().swb_moe, _TYPES[dtype], flags, x.data_ptr(), pitch, router.data_ptr(), gate.data_ptr(),
+          up.data_ptr(), down.data_ptr(), gate_scales.data_ptr() if four_bit else None,
+          up_scales.data_ptr() if four_bit else None, down_scales.data_ptr() if four_bit else None, y.data_ptr(),
+          None if ids is None else ids.data_ptr(), None if weights is None else weights.data_ptr(), tokens, hidden,
+          inter, experts, topk, workspace.data_ptr(), workspace.numel())
+
+
+def moe(x: torch.Tensor, router: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, topk: int,
+        **kwargs) -> torch.Tensor:
+    """Allocating wrapper of ``moe_out`` (output and workspace; the options are ``moe_out``'s)."""
+    _check(x.dim() == 2 and router.dim() == 2 and gate.dim() == 3, "invalid dimensions")
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    workspace = moe_workspace(x.size(0), router.size(0), topk, gate.size(1), x.device)
+    moe_out(x, router, gate, up, down, y, workspace, topk, **kwargs)
+    return y

@@ -45,7 +45,10 @@ extern "C" {
 #define SWB_E_DEVICE 13        /* a kernel gave up a bounded wait (device error word set) */
 #define SWB_E_UNSUPPORTED 14   /* no usable sm_100 device / feature */
 #define SWB_E_WORKSPACE 15     /* size beyond the built-in workspace of swb_ffn_noalloc; a missing
-                                  or misaligned swb_ffn_fused workspace */
+                                  or misaligned swb_ffn_fused workspace; a swb_moe workspace that is
+                                  missing or too small */
+#define SWB_E_TYPE 16          /* element type not among those the call takes */
+#define SWB_E_ALIGNMENT 17     /* a buffer without the alignment its call names */
 
 /* project() flags (template flags of decode::launch, include/kernels.cuh:115) */
 #define SWB_RESIDUAL 1u /* add residual[row] after bias (RESIDUAL) */
@@ -275,6 +278,70 @@ SWB_API int swb_gate_epilogue(const float* a, const float* b, const void* bg, co
 /* residual_epilogue: y[i] += bias[i] + x[i]; also closes a tensor-parallel layer
  * after the all-reduce of the partial y. */
 SWB_API int swb_residual_epilogue(float* y, const void* bias, const void* x, int n, void* stream);
+
+/* ---- four-bit matrices (MXFP4) and products with them (no counterpart in the reference) ----
+ *
+ * A matrix [rows, cols] is held as codes [rows, ceil(cols/32) * 16] bytes and scales
+ * [rows, ceil(cols/32)] bytes, both contiguous: each block of 32 values along a row is
+ * 16 bytes of e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives; value 2i in the
+ * low half of byte i) times 2^(scale - 127); scale 255 makes the block NaN. A ragged last
+ * block is filled up with zero codes. */
+#define SWB_F16 0
+#define SWB_BF16 1
+#define SWB_F32 2
+#define SWB_MX4_MAX_DIM (1 << 20)    /* rows and cols of a product */
+#define SWB_MX4_MAX_TOKENS (1 << 24)
+
+/* Rounds x [rows, cols] (type SWB_F16, SWB_BF16 or SWB_F32; x_pitch elements from row to
+ * row) to codes and scales. A block's scale is 2^(floor(log2 max|x|) - 2), not below
+ * 2^-127; values go to the nearest code, ties to the even one, larger ones to 6; a block
+ * that holds a NaN or an infinity becomes NaN. rows == 0 or cols == 0: nothing to do. */
+SWB_API int swb_mx4_quantize(int type, const void* x, int64_t x_pitch, void* codes, void* scales, int64_t rows,
+                             int64_t cols, void* stream);
+
+/* Reads codes and scales back as values of `type`, exact but for its range (fp16: beyond
+ * 65504 to infinity, below 2^-24 to the nearest subnormal). */
+SWB_API int swb_mx4_dequantize(int type, const void* codes, const void* scales, void* out, int64_t out_pitch,
+                               int64_t rows, int64_t cols, void* stream);
+
+/* swb_project for any number of tokens on a four-bit matrix:
+ * out[t][r] = W[r].x[t] (+ bias[r]) (+ residual[t][r]). codes (16-byte aligned), scales:
+ * W [rows, cols]; x [tokens, cols] of `type` (SWB_F16 or SWB_BF16), x_pitch elements from
+ * token to token; bias [rows] or NULL and residual [tokens, rows] (read with SWB_RESIDUAL)
+ * of `type`; out [tokens, rows] fp32, or `type` with SWB_HALF_OUT (then residual may be
+ * out itself). Sums in fp32 over the exact values of W. tokens == 0: nothing to do. */
+SWB_API int swb_mx4_project(int type, const void* codes, const void* scales, const void* x, int64_t x_pitch,
+                            const void* bias, const void* residual, void* out, int64_t tokens, int64_t rows,
+                            int64_t cols, unsigned flags, void* stream);
+
+/* ---- mixture-of-experts layer for a few tokens (no counterpart in the reference) ----
+ *
+ * logits = router x, the topk largest select a token's experts (ties: the lowest index;
+ * NaN counts as largest), w = softmax over all logits at those places, or over the
+ * selected ones with SWB_MOE_RENORMALIZE;
+ * y[t] = sum_j w[t][j] down_e (SiLU(gate_e x[t]) * (up_e x[t])), e = ids[t][j], without bias
+ * or residual (as swb_swiglu_out). type: SWB_F16 or SWB_BF16 of x [tokens, hidden]
+ * (x_pitch elements from token to token), router [experts, hidden], y [tokens, hidden] and
+ * of gate, up [experts, inter, hidden] and down [experts, hidden, inter]; with SWB_MOE_MX4
+ * these three are four-bit codes (16-byte aligned) and *_scales their scales, else
+ * *_scales are ignored. The router's sums are held in 64 bits, the others in fp32; the
+ * product of the activations is rounded to `type` once. ids [tokens, topk] int32 and
+ * weights [tokens, topk] fp32 receive the selection; either may be NULL.
+ * One cooperative kernel. workspace: swb_moe_workspace_bytes of 256-byte aligned device
+ * memory, zeroed once when allocated, then reused by every call on one stream (calls that
+ * may overlap on the GPU need a workspace each). After a device error (swb_device_error)
+ * zero it again. swb_moe_workspace_bytes is 0 for sizes beyond the limits. */
+#define SWB_MOE_MAX_TOKENS 64
+#define SWB_MOE_MAX_EXPERTS 256
+#define SWB_MOE_MAX_TOPK 16
+#define SWB_MOE_MAX_DIM 100000 /* hidden and inter */
+#define SWB_MOE_MX4 1u
+#define SWB_MOE_RENORMALIZE 2u
+SWB_API size_t swb_moe_workspace_bytes(int tokens, int experts, int topk, int inter);
+SWB_API int swb_moe(int type, unsigned flags, const void* x, int64_t x_pitch, const void* router, const void* gate,
+                    const void* up, const void* down, const void* gate_scales, const void* up_scales,
+                    const void* down_scales, void* y, int* ids, float* weights, int tokens, int hidden, int inter,
+                    int experts, int topk, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Device error word of the current device: OR of SWB_DEVERR_* raised by kernels
  * whose bounded waits expired. Synchronises the device. clear != 0 resets it. */

@@ -1,0 +1,224 @@
+"""Four-bit matrices on the GPU against plain 64-bit forms.
+
+Rounding and reading back are exact (whole codes, power-of-two scales), so they are compared
+bit for bit; reading back as fp16 rounds what fp16 cannot hold, and is compared with numpy's
+rounding of the exact value.
+
+Products: a value is a sum of exact products. Inside a block the tensor core adds 32 of them
+in two instructions, each of which may lose 17 2^-24 relative to the magnitudes it adds
+(16 products and the running sum aligned to the largest, truncated); a block's sum is then added
+in fp32, one rounding (2^-24) a block, and the eight warps' parts, bias and residual add at
+most ten more. So |out - exact| <= (34 + K/32 + 10) 2^-24 sum|w x| (+ |bias| + |residual| terms in
+that sum) + half a step of the output type (eps/2 relative, or half of the smallest subnormal).
+"""
+import numpy as np
+import pytest
+import torch
+
+import mx4_reference as R
+import swiglu_b200 as S
+
+pytestmark = pytest.mark.gpu
+TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+def sample(shape, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype).cuda()
+
+
+def np64(t):
+    return t.double().cpu().numpy()
+
+
+def packed(shape, seed, scale=1.0):
+    """A four-bit matrix as the plain form rounds it: (codes, scales) on the GPU, values."""
+    x = np.random.RandomState(seed).randn(*shape) * scale
+    c, s = R.quantize(x.reshape(-1, shape[-1]))
+    c, s = c.reshape(*shape[:-1], -1), s.reshape(*shape[:-1], -1)
+    return torch.from_numpy(c).cuda(), torch.from_numpy(s).cuda(), R.values(c, s, shape[-1])
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 32), (3, 31), (5, 33), (2, 8), (7, 40), (4, 257), (9, 1030), (65, 96)])
+def test_quantize_and_back(kind, rows, cols):
+    x = sample((rows, cols), TYPES[kind], rows * 1000 + cols, 3.0)
+    codes, scales = S.mx4_quantize(x)
+    c, s = R.quantize(np64(x))
+    assert np.array_equal(codes.cpu().numpy(), c) and np.array_equal(scales.cpu().numpy(), s)
+    back = S.mx4_dequantize(codes, scales, cols, TYPES[kind])
+    want = torch.from_numpy(R.values(c, s, cols)).to(TYPES[kind])
+    assert torch.equal(back.cpu(), want)
+    whole = S.mx4_dequantize(codes, scales, dtype=torch.float32)  # pads read as zeros
+    assert whole.shape[1] == -(-cols // 32) * 32 and not whole[:, cols:].any()
+
+
+def test_quantize_ties_and_extremes():
+    e = [0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0, 7.99, 6.01, 4.0, -0.25, -0.24, -5.0, 0.0, -0.0]
+    rows = [np.array(e + [0.0] * 16) * 2.0 ** k for k in (-140, -131, -127, -126, -100, 0, 3, 100, 124)]
+    rows.append(np.zeros(32))
+    rows.append(np.full(32, -0.0))
+    rows.append(np.full(32, 2.0 ** -149))
+    rows.append(np.full(32, np.finfo(np.float32).max))
+    x = torch.from_numpy(np.stack(rows).astype(np.float32))
+    bad = x[:1].repeat(3, 1).clone()
+    bad[0, 3], bad[1, 31], bad[2, 0] = float("nan"), float("inf"), float("-inf")
+    x = torch.cat([x, bad]).cuda()
+    for view in (x, torch.nn.functional.pad(x, (1, 0))[:, 1:]):  # aligned, and rows off by one value
+        codes, scales = S.mx4_quantize(view)
+        c, s = R.quantize(np64(x))
+        assert np.array_equal(scales.cpu().numpy(), s) and np.array_equal(codes.cpu().numpy(), c)
+        back = S.mx4_dequantize(codes, scales, 32, torch.float32).cpu()
+        want = torch.from_numpy(R.values(c, s, 32)).float()
+        assert torch.equal(torch.isnan(back), torch.isnan(want))
+        assert torch.equal(back[:-3], want[:-3]) and torch.isnan(back[-3:]).all()
+
+
+def test_every_code_and_scale_reads_back():
+    codes = torch.arange(256, dtype=torch.uint8).repeat(256, 1).view(256, 16, 16).reshape(256, 256)
+    scales = torch.arange(256, dtype=torch.uint8).view(256, 1).repeat(1, 16)
+    exact = R.values(codes.numpy(), scales.numpy(), 512)
+    for kind in TYPES.values():
+        with np.errstate(over="ignore"):
+            want = torch.from_numpy(exact.astype(np.float32)).to(kind)  # one rounding: fp32 holds all but the largest
+        for cols in (512, 511):
+            got = S.mx4_dequantize(codes.cuda(), scales.cuda(), cols, kind).cpu()
+            w = want[:, :cols]
+            assert torch.equal(torch.isnan(got), torch.isnan(w))
+            assert torch.equal(got[~torch.isnan(w)], w[~torch.isnan(w)])
+
+
+def test_quantize_spaced_rows_three_dims_and_bounds():
+    base = sample((6, 200), torch.bfloat16, 1)
+    x = base[:, 8:72]
+    codes, scales = S.mx4_quantize(x)
+    c, s = R.quantize(np64(x))
+    assert np.array_equal(codes.cpu().numpy(), c) and np.array_equal(scales.cpu().numpy(), s)
+    out = torch.full((6, 200), 7.0, dtype=torch.bfloat16, device="cuda")
+    S.mx4_dequantize_out(codes, scales, out[:, 8:72])
+    assert torch.equal(out[:, 8:72].cpu().double(), torch.from_numpy(R.values(c, s, 64)))
+    assert (out[:, :8] == 7).all() and (out[:, 72:] == 7).all()
+    x3 = sample((2, 3, 45), torch.float16, 2)
+    c3, s3 = S.mx4_quantize(x3)
+    assert c3.shape == (2, 3, 32) and s3.shape == (2, 3, 2)
+    c2, s2 = S.mx4_quantize(x3.view(6, 45))
+    assert torch.equal(c3.view(6, -1), c2) and torch.equal(s3.view(6, -1), s2)
+    empty = S.mx4_quantize(torch.empty((0, 45), dtype=torch.float16, device="cuda"))
+    assert empty[0].shape == (0, 32)
+
+
+def project_bound(x, w, extra, rel=0.0):
+    return (44 + x.shape[1] / 32) * 2.0 ** -24 * (np.abs(x) @ np.abs(w).T + extra)
+
+
+def half_step(v, dtype):
+    f = torch.finfo(dtype)
+    return np.maximum(np.abs(v) * f.eps / 2, f.tiny * f.eps / 2)
+
+
+def check_product(got, x, w, bias, residual, dtype):
+    want = x @ w.T
+    extra = np.zeros_like(want)
+    for t in (bias, residual):
+        if t is not None:
+            want = want + t
+            extra = extra + np.abs(t)
+    bound = project_bound(x, w, extra)
+    err = np.abs(np64(got) - want)
+    limit = bound + half_step(np.abs(want) + bound, dtype)
+    assert np.isfinite(np64(got)).all() and (err <= limit).all(), float((err / limit).max())
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("tokens,rows,cols", [
+    (1, 1, 1), (1, 32, 128), (1, 33, 31), (2, 16, 32), (3, 65, 130), (8, 48, 1024), (9, 100, 257), (16, 31, 160),
+    (17, 512, 96), (33, 40, 72), (64, 64, 544), (65, 17, 33), (130, 96, 1030), (1, 5632, 2048)])
+def test_project(kind, tokens, rows, cols):
+    dtype = TYPES[kind]
+    codes, scales, w = packed((rows, cols), rows + cols, cols ** -0.5)
+    x = sample((tokens, cols), dtype, tokens)
+    bias, residual = sample((rows,), dtype, 3, 0.1), sample((tokens, rows), dtype, 4)
+    check_product(S.mx4_project(x, codes, scales), np64(x), w, None, None, dtype)
+    check_product(S.mx4_project(x, codes, scales, bias, residual, torch.float32), np64(x), w, np64(bias), np64(residual),
+                  torch.float32)
+    out = residual.clone()
+    S.mx4_project_out(x, codes, scales, out, bias, out)  # in place
+    check_product(out, np64(x), w, np64(bias), np64(residual), dtype)
+
+
+def test_project_views_and_bounds():
+    """Tokens in spaced or misaligned rows, scales off a word, outputs between guards."""
+    codes, scales, w = packed((40, 160), 5, 0.1)
+    wide = sample((5, 400), torch.float16, 6)
+    room = torch.zeros(scales.numel() + 1, dtype=torch.uint8, device="cuda")
+    room[1:] = scales.flatten()
+    odd = room[1:].view_as(scales)
+    for x in (wide[:, 8:168], wide[:, 3:163]):
+        for s in (scales, odd):
+            buf = torch.full((7, 40), 9.0, dtype=torch.float32, device="cuda")
+            S.mx4_project_out(x, codes, s, buf[1:6])
+            check_product(buf[1:6], np64(x), w, None, None, torch.float32)
+            assert (buf[0] == 9).all() and (buf[6] == 9).all()
+
+
+def test_project_special_values():
+    """Scales of 0 and 255, the largest scales, and infinities and NaN among the tokens."""
+    cols = 128
+    codes = torch.randint(0, 256, (48, cols // 2), dtype=torch.uint8, generator=torch.Generator().manual_seed(1))
+    scales = torch.full((48, 4), 127, dtype=torch.uint8)
+    scales[0] = 0
+    scales[1, 2] = 255
+    scales[2] = 200
+    scales[3, 1] = 0
+    w = R.values(codes.numpy(), scales.numpy(), cols)
+    for dtype in (torch.float16, torch.bfloat16):
+        x = sample((4, cols), dtype, 2)
+        got = np64(S.mx4_project(x, codes.cuda(), scales.cuda(), dtype=torch.float32))
+        want = np64(x) @ w.T
+        assert np.isnan(got[:, 1]).all()
+        keep = [i for i in range(48) if i != 1]
+        bound = project_bound(np64(x), w[keep], 0)
+        # the smallest scale's products are subnormal in fp32: half of its smallest step each
+        assert (np.abs(got[:, keep] - want[:, keep]) <= bound + half_step(want[:, keep], torch.float32) + cols * 2.0 ** -149).all()
+        x[2, 5], x[3, 7] = float("inf"), float("nan")
+        got = S.mx4_project(x, codes.cuda(), scales.cuda(), dtype=torch.float32)
+        rest = S.mx4_project(x[:2].contiguous(), codes.cuda(), scales.cuda(), dtype=torch.float32)
+        assert torch.equal(got[:2].nan_to_num(), rest.nan_to_num()) and torch.isnan(got[3]).all()
+        assert not torch.isfinite(got[2]).any()
+
+
+def test_project_refusals():
+    codes, scales, _ = packed((8, 64), 1)
+    x = sample((2, 64), torch.float16, 1)
+    for bad in (lambda: S.mx4_project(x.float(), codes, scales), lambda: S.mx4_project(x[:, :32], codes, scales),
+                lambda: S.mx4_project(x, codes[:4], scales), lambda: S.mx4_project(x, codes.cpu(), scales.cpu()),
+                lambda: S.mx4_project(x, codes, scales, bias=x[0, :7]),
+                lambda: S.mx4_project(x, codes, scales, dtype=torch.bfloat16),
+                lambda: S.mx4_project(x.t().contiguous().t(), codes, scales),
+                lambda: S.mx4_project(x.requires_grad_(), codes, scales)):
+        with pytest.raises(RuntimeError):
+            bad()
+    assert S.mx4_project(x.detach()[:0], codes, scales).shape == (0, 8)
+
+
+def test_project_streams_graphs_and_repeats():
+    codes, scales, w = packed((96, 512), 8, 0.05)
+    x = sample((3, 512), torch.bfloat16, 9)
+    want = S.mx4_project(x, codes, scales)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = S.mx4_project(x, codes, scales)
+    side.synchronize()
+    assert torch.equal(want, again)
+    out = torch.empty_like(want)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        S.mx4_project_out(x, codes, scales, out)
+    x.copy_(sample((3, 512), torch.bfloat16, 10))
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, S.mx4_project(x, codes, scales))
