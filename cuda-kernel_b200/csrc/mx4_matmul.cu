@@ -1,0 +1,612 @@
+// Product of two MXFP4 matrices on the fifth-generation tensor cores
+// (declaration: include/swiglu_b200.h).
+//
+//   out[t][r] = sum_k X[t][k] W[r][k] (+ bias[r]) (+ residual[t][r])
+//
+// tcgen05.mma kind::mxf4 multiplies 64 four-bit values a step and applies the two
+// blocks' power-of-two scales itself, so codes go from global memory to the tensor
+// core untouched: TMA brings 256 values (128 bytes) of every row of both tiles into a
+// 128-byte swizzled stage; four warps bring the scale bytes of the same rows into
+// the 32 x 16-byte blocks that tcgen05.cp spreads over TMEM; one thread issues the
+// copies and products; four warps drain the accumulators.
+//
+// Long batches (tokens on the M side, MT x 128 of them by N = 192 rows of W): two
+// accumulators of 192 columns and the stages' scales fill TMEM. Without sharing a
+// tile between CTAs the bytes that L2 hands out bound this kernel (0.5 B per value at
+// 4x the rate of 16-bit products), hence the large tile.
+// Few tokens (W on the M side, N = 16 to 128 tokens): bound by the bytes of W. The
+// CTAs of a cluster split K, so that every SM streams, and add their parts through
+// each other's shared memory in a fixed order.
+#include <cuda.h>
+
+#include <algorithm>
+#include <cstring>
+
+#include "device.cuh"
+#include "host.h"
+#include "stream.cuh"
+
+namespace swb {
+
+int mx4_matmul_device_error(int clear, int* out) {
+    int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, g_device_error, sizeof v);
+    if (e == cudaSuccess && clear) {
+        const int zero = 0;
+        e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof zero);
+    }
+    if (e != cudaSuccess) return fail(SWB_E_CUDA, cudaGetErrorString(e));
+    *out = v;
+    return SWB_OK;
+}
+
+namespace {
+
+constexpr int kMmaM = 128;
+constexpr int kRowBytes = 128;     // of a row in a stage: 256 values, 8 scales
+constexpr int kWindow = 16;        // scale bytes of a row that a thread loads at once: two stages
+constexpr int kScaleBlock = 512;   // scales of 128 rows x 128 values as tcgen05.cp reads them
+constexpr int kEpilogueWarps = 4, kScaleWarps = 4;
+constexpr int kThreads = (kEpilogueWarps + kScaleWarps + 2) * 32;
+
+struct MatmulParams {
+    const unsigned char* sa;  // scales of the M side, [rows_a, blocks]
+    const unsigned char* sb;  // of the N side
+    const void* bias;
+    const void* residual;
+    void* out;
+    int64_t rows_a, rows_b;   // rows of the M and N side
+    int64_t tokens, rows;     // of the output
+    int tiles_a, tiles_b;     // M tiles, N tiles
+    int64_t tiles;
+    int blocks;               // scales of a row
+    int stages_k;             // stages that cover K
+    int splits;               // CTAs of a cluster that share a tile's K
+};
+
+// ------------------------------------------------------------ tcgen05 and TMA
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t columns) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns));
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// Arrives on `bar` once every tcgen05 operation this thread issued so far is done.
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void scale_copy(uint32_t tmem, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                         bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.u32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(uint32_t(accumulate)) : "memory");
+}
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+        "%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand descriptors: K-major rows of 128 swizzled bytes, groups of eight
+// rows 1024 bytes apart; scale blocks: unswizzled 16-byte rows, groups of eight 128 apart.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+    return uint64_t((addr & 0x3FFFF) >> 4) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+           (uint64_t(2) << 61);
+}
+__device__ __forceinline__ uint64_t scale_desc(uint32_t addr) {
+    return uint64_t((addr & 0x3FFFF) >> 4) | (uint64_t(1) << 16) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
+}
+// Instruction descriptor: e2m1 operands, E8M0 scales, K-major, M x N; `id`: which half of a
+// scale word (blocks 0 and 1, or 2 and 3 of 128 values) the step takes.
+__device__ __forceinline__ constexpr uint32_t instruction_desc(int n, int id) {
+    return (1u << 7) | (1u << 10) | (uint32_t(n >> 3) << 17) | (1u << 23) | (uint32_t(kMmaM >> 7) << 27) |
+           (uint32_t(id) << 4) | (uint32_t(id) << 29);
+}
+
+template <int N, int MT, bool TOKENS_M>
+struct MatmulShape {
+    static constexpr int kStages = TOKENS_M ? (MT == 2 ? 3 : 5) : (N <= 32 ? 5 : 4);
+    static constexpr int kPerSm = TOKENS_M || N > 64 ? 1 : 2;
+    static constexpr int kRowsA = MT * kMmaM;
+    static constexpr int kBytesA = kRowsA * kRowBytes, kBytesB = N * kRowBytes;
+    static constexpr int kBlocksB = (N + kMmaM - 1) / kMmaM;   // 128-row blocks of scales of the N side
+    static constexpr int kScales = 2 * (MT + kBlocksB) * kScaleBlock;
+    static constexpr int kStage = kBytesA + kBytesB + kScales;
+    static_assert(kStage % 1024 == 0, "stages keep the swizzle's alignment");
+    static constexpr int kAccs = TOKENS_M ? 2 : 1;             // accumulators of N columns
+    static constexpr int kScaleColumns = 2 * (MT + kBlocksB) * 4;
+    static constexpr int kUsed = kAccs * N + kStages * kScaleColumns;
+    static constexpr int kColumns = kUsed <= 32 ? 32 : kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
+    static_assert(kUsed <= 512, "TMEM columns");
+    static constexpr int kPartPitch = kMmaM + 1;               // floats of a token's column in the exchange
+    static constexpr int kExchange = TOKENS_M ? 0 : N * kPartPitch * 4;
+    static constexpr size_t kSmem = size_t(kStages) * kStage + 1024;  // the exchange reuses the stages
+    static_assert(kExchange <= kStages * kStage, "exchange fits the stages");
+    static_assert(kColumns * kPerSm <= 512, "CTAs of an SM share TMEM");
+    static_assert((kSmem + 2048) * kPerSm <= kSmemPerSm, "CTAs of an SM share its shared memory");
+};
+
+// One window of a row's scale bytes: bytes [b0, b0 + 16) of `blocks`, zero beyond.
+__device__ __forceinline__ uint4 load_scales(const unsigned char* row, int b0, int blocks) {
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    if ((blocks & 15) == 0 && (reinterpret_cast<uintptr_t>(row) & 15) == 0) {
+        if (b0 < blocks) return __ldg(reinterpret_cast<const uint4*>(row + b0));
+    } else if ((blocks & 3) == 0 && (reinterpret_cast<uintptr_t>(row) & 3) == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (b0 + 4 * i < blocks) w[i] = __ldg(reinterpret_cast<const uint32_t*>(row + b0) + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (b0 + i < blocks) w[i >> 2] |= uint32_t(__ldg(row + b0 + i)) << (8 * (i & 3));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T>
+__device__ __forceinline__ float load_value(const void* p, int64_t i) {
+    return Num<T>::to_float(static_cast<const T*>(p)[i]);
+}
+
+template <typename T, int N, int MT, bool TOKENS_M>
+__global__ void __launch_bounds__(kThreads, 1)
+    matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                  const MatmulParams P) {
+    using S = MatmulShape<N, MT, TOKENS_M>;
+    extern __shared__ unsigned char raw[];
+    __shared__ uint64_t full[S::kStages], scaled[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_failed;
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // this CTA's tiles [first, last) by `step`, and its share of K
+    const int rank = P.splits > 1 ? int(blockIdx.x % P.splits) : 0;
+    const int64_t step = gridDim.x / P.splits, first = blockIdx.x / P.splits;
+    const int k0 = int(int64_t(P.stages_k) * rank / P.splits), k1 = int(int64_t(P.stages_k) * (rank + 1) / P.splits);
+
+    if (threadIdx.x == 0) {
+        s_failed = 0;
+        for (int i = 0; i < S::kStages; ++i) {
+            mbar_init(smem_u32(full + i), 1);
+            mbar_init(smem_u32(scaled + i), kScaleWarps * 32);
+            mbar_init(smem_u32(empty + i), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(acc_full + i), 1);
+            mbar_init(smem_u32(acc_empty + i), kEpilogueWarps * 32);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 0) tmem_alloc(smem_u32(&s_tmem), S::kColumns);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = s_tmem;
+    const uint32_t scale_columns = tmem + S::kAccs * N;
+
+    if (warp == kEpilogueWarps + kScaleWarps) {
+        // ------------------------------------------------------- codes, by TMA
+        if (lane == 0) {
+            int s = 0, issued = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int64_t tile = first; tile < P.tiles && ok; tile += step) {
+                const int a = int(tile % P.tiles_a), b = int(tile / P.tiles_a);
+                for (int k = k0; k < k1; ++k) {
+                    if (issued >= S::kStages && !mbar_wait(smem_u32(empty + s), ph ^ 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t bar = smem_u32(full + s), at = base + s * S::kStage;
+                    mbar_arrive_expect_tx(bar, S::kBytesA + S::kBytesB);
+                    tma_load_2d(at, &map_a, k * kRowBytes, a * S::kRowsA, bar);
+                    tma_load_2d(at + S::kBytesA, &map_b, k * kRowBytes, b * N, bar);
+                    ++issued;
+                    if (++s == S::kStages) s = 0, ph ^= 1u;
+                }
+            }
+            // nothing stays in flight into shared memory when the CTA leaves early
+            if (!ok) {
+                for (int i = 0; i < S::kStages && i < issued; ++i) {
+                    const int idx = issued - 1 - i;
+                    mbar_wait(smem_u32(full + idx % S::kStages), uint32_t(idx / S::kStages) & 1u);
+                }
+                s_failed = 1;
+            }
+        }
+    } else if (warp == kEpilogueWarps + kScaleWarps + 1) {
+        // ------------------------------------------------------- products
+        if (lane == 0) {
+            int s = 0, acc = 0;
+            uint32_t ph = 0, aph = 0;
+            bool ok = true;
+            int64_t done = 0;
+            for (int64_t tile = first; tile < P.tiles && ok; tile += step, ++done) {
+                for (int k = k0; k < k1 && ok; ++k) {
+                    ok = mbar_wait(smem_u32(full + s), ph) && mbar_wait(smem_u32(scaled + s), ph);
+                    if (!ok) break;
+                    fence_after();
+                    const uint32_t at = base + s * S::kStage, sc = at + S::kBytesA + S::kBytesB;
+                    const uint32_t col = scale_columns + s * S::kScaleColumns;
+#pragma unroll
+                    for (int i = 0; i < 2 * (MT + S::kBlocksB); ++i)
+                        scale_copy(col + 4 * i, scale_desc(sc + i * kScaleBlock));
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        const int use = MT == 2 ? m : acc;
+                        // the accumulator's last tile has been read
+                        if (k == k0 && done >= (MT == 2 ? 1 : S::kAccs)) {
+                            ok = mbar_wait(smem_u32(acc_empty + use), aph ^ 1u);
+                            if (!ok) break;
+                            fence_after();
+                        }
+                        const uint64_t da = operand_desc(at + m * kMmaM * kRowBytes), db = operand_desc(at + S::kBytesA);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)  // 64 values a step; scales: blocks of 128 values, then rows
+                            mma_mxf4(tmem + use * N, da + 2 * i, db + 2 * i, instruction_desc(N, (i & 1) * 2),
+                                     col + ((i >> 1) * MT + m) * 4, col + (2 * MT + (i >> 1) * S::kBlocksB) * 4,
+                                     k > k0 || i > 0);
+                    }
+                    if (!ok) break;
+                    mma_commit(smem_u32(empty + s));
+                    if (k == k1 - 1) {
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) mma_commit(smem_u32(acc_full + (MT == 2 ? m : acc)));
+                    }
+                    if (++s == S::kStages) s = 0, ph ^= 1u;
+                }
+                if (MT == 2 || S::kAccs == 1) {
+                    aph ^= 1u;
+                } else if (++acc == S::kAccs) {
+                    acc = 0;
+                    aph ^= 1u;
+                }
+            }
+            if (!ok) s_failed = 1;
+        }
+    } else if (warp >= kEpilogueWarps) {
+        // ------------------------------------------------------- scales
+        constexpr int kRows = S::kRowsA + N, kPer = (kRows + 127) / 128;
+        const int t = threadIdx.x - kEpilogueWarps * 32;
+        int s = 0, issued = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int64_t tile = first; tile < P.tiles && ok; tile += step) {
+            const int64_t a0 = tile % P.tiles_a * S::kRowsA, b0 = tile / P.tiles_a * N;
+            const unsigned char* row[kPer];
+            uint32_t dst[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int r = t + 128 * i;
+                row[i] = nullptr;
+                const bool in_a = r < S::kRowsA;
+                const int q = in_a ? r : r - S::kRowsA, in = q & 127;
+                const int64_t global = in_a ? a0 + q : b0 + q;
+                if (r < kRows && global < (in_a ? P.rows_a : P.rows_b))
+                    row[i] = (in_a ? P.sa : P.sb) + global * P.blocks;
+                // blocks of the M side: [128 values][128 rows], then the N side's
+                dst[i] = (in_a ? q >> 7 : 2 * MT + (q >> 7)) * kScaleBlock + (in & 31) * 16 + (in >> 5) * 4;
+            }
+            uint4 next[kPer];
+            auto load = [&](int k) {  // the window that holds stage k's scales
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+                    next[i] = row[i] ? load_scales(row[i], k * 8 & ~(kWindow - 1), P.blocks) : make_uint4(0u, 0u, 0u, 0u);
+            };
+            load(k0);
+            uint4 now[kPer];
+            for (int k = k0; k < k1; ++k) {
+                if (k == k0 || (k & 1) == 0) {
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) now[i] = next[i];
+                    const int then = (k | 1) + 1;
+                    if (then < k1) load(then);
+                }
+                if (issued >= S::kStages && !mbar_wait(smem_u32(empty + s), ph ^ 1u)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t sc = base + s * S::kStage + S::kBytesA + S::kBytesB;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const int r = t + 128 * i;
+                    if (r < kRows) {
+                        const uint32_t next_block = (r < S::kRowsA ? MT : S::kBlocksB) * kScaleBlock;
+                        sts32(sc + dst[i], k & 1 ? now[i].z : now[i].x);
+                        sts32(sc + dst[i] + next_block, k & 1 ? now[i].w : now[i].y);
+                    }
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(smem_u32(scaled + s));
+                ++issued;
+                if (++s == S::kStages) s = 0, ph ^= 1u;
+            }
+        }
+        if (!ok) s_failed = 1;
+    } else {
+        // ------------------------------------------------------- epilogue
+        int acc = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        const uint32_t quadrant = uint32_t(warp * 32) << 16;
+        for (int64_t tile = first; tile < P.tiles && ok; tile += step) {
+            const int64_t a0 = tile % P.tiles_a * S::kRowsA, b0 = tile / P.tiles_a * N;
+#pragma unroll 1
+            for (int m = 0; m < MT; ++m) {
+                const int use = MT == 2 ? m : acc;
+                ok = mbar_wait(smem_u32(acc_full + use), ph);
+                if (!ok) break;
+                __syncwarp();
+                fence_after();
+                const int in_tile = m * kMmaM + warp * 32 + lane;
+                if constexpr (TOKENS_M) {
+                    const int64_t token = a0 + in_tile;
+                    const bool wide = P.rows % 8 == 0 && (reinterpret_cast<uintptr_t>(P.out) & 15) == 0 &&
+                                      (reinterpret_cast<uintptr_t>(P.residual) & 15) == 0;
+#pragma unroll 1
+                    for (int c = 0; c < N; c += 32) {
+                        uint32_t v[32];
+                        __syncwarp();
+                        tmem_load32(tmem + quadrant + use * N + c, v);
+                        tmem_load_wait();
+                        if (token >= P.tokens) continue;
+                        const int64_t row0 = b0 + c, at = token * P.rows + row0;
+                        T* out = static_cast<T*>(P.out) + at;
+#pragma unroll
+                        for (int j = 0; j < 32; j += 8) {
+                            if (row0 + j >= P.rows) break;
+                            float f[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[j + e]);
+                            if (wide) {
+                                if (P.bias) {
+#pragma unroll
+                                    for (int e = 0; e < 8; ++e) f[e] += load_value<T>(P.bias, row0 + j + e);
+                                }
+                                if (P.residual) {
+                                    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const T*>(P.residual) + at + j);
+#pragma unroll
+                                    for (int e = 0; e < 8; ++e) f[e] += Num<T>::to_float(reinterpret_cast<const T*>(&q)[e]);
+                                }
+                                uint4 q;
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(&q)[e] = Num<T>::from_float(f[e]);
+                                *reinterpret_cast<uint4*>(out + j) = q;
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    if (row0 + j + e >= P.rows) break;
+                                    if (P.bias) f[e] += load_value<T>(P.bias, row0 + j + e);
+                                    if (P.residual) f[e] += load_value<T>(P.residual, at + j + e);
+                                    out[j + e] = Num<T>::from_float(f[e]);
+                                }
+                            }
+                        }
+                    }
+                } else {
+                    // a column is a token, a lane a row of W: to shared memory, [token][row]
+                    float* part = reinterpret_cast<float*>(raw + (base - smem_u32(raw)));
+#pragma unroll 1
+                    for (int c = 0; c < N; c += 16) {
+                        uint32_t v[16];
+                        tmem_load16(tmem + quadrant + use * N + c, v);
+                        tmem_load_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) part[(c + j) * S::kPartPitch + in_tile] = __uint_as_float(v[j]);
+                    }
+                }
+                fence_before();
+                mbar_arrive(smem_u32(acc_empty + use));
+            }
+            if (MT == 2 || S::kAccs == 1) {
+                ph ^= 1u;
+            } else if (++acc == S::kAccs) {
+                acc = 0;
+                ph ^= 1u;
+            }
+        }
+        if (!ok) s_failed = 1;
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        fence_after();
+        tmem_free(tmem, S::kColumns);
+    }
+    if constexpr (!TOKENS_M) {
+        // The cluster's parts, added in rank order; each CTA takes its share of the tile's outputs.
+        // A CTA that failed writes nothing, and its peers keep what they could add.
+        asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+        const int64_t w0 = first % P.tiles_a * S::kRowsA, t0 = first / P.tiles_a * N;
+        const int count = int(min(int64_t(N), P.tokens - t0)) * kMmaM;
+        if (!s_failed) {
+            for (int i = rank * kThreads + threadIdx.x; i < count; i += P.splits * kThreads) {
+                const int t = i / kMmaM, r = i % kMmaM;
+                if (w0 + r >= P.rows) continue;
+                float v = 0.f;
+                for (int j = 0; j < P.splits; ++j) {
+                    uint32_t remote;
+                    float f;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(base + (t * S::kPartPitch + r) * 4), "r"(j));
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(remote) : "memory");
+                    v += f;
+                }
+                const int64_t row = w0 + r, at = (t0 + t) * P.rows + row;
+                if (P.bias) v += load_value<T>(P.bias, row);
+                if (P.residual) v += load_value<T>(P.residual, at);
+                static_cast<T*>(P.out)[at] = Num<T>::from_float(v);
+            }
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    }
+}
+
+// ------------------------------------------------------------ host
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            p = nullptr;
+        }
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+int make_map(CUtensorMap* map, const void* codes, int64_t rows, int64_t blocks, int box_rows) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return fail(SWB_E_UNSUPPORTED, "the driver has no tensor maps");
+    const cuuint64_t dims[2] = {cuuint64_t(blocks * kMxBlockBytes), cuuint64_t(rows)};
+    const cuuint64_t strides[1] = {cuuint64_t(blocks * kMxBlockBytes)};
+    const cuuint32_t box[2] = {cuuint32_t(kRowBytes), cuuint32_t(box_rows)}, one[2] = {1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, one,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? SWB_OK : fail(SWB_E_CUDA, "tensor map");
+}
+
+struct Side {
+    const void* codes;
+    const unsigned char* scales;
+    int64_t rows;
+};
+
+template <typename T, int N, int MT, bool TOKENS_M>
+int launch_matmul(const Side& x, const Side& w, MatmulParams P, cudaStream_t stream) {
+    using S = MatmulShape<N, MT, TOKENS_M>;
+    static std::atomic<uint64_t> smem_set{0};
+    const int sms = sm_count();
+    if (sms <= 0) return check_launch();
+    auto kernel = matmul_kernel<T, N, MT, TOKENS_M>;
+    if (int rc = allow_smem(kernel, smem_set, S::kSmem)) return rc;
+    const Side& a = TOKENS_M ? x : w;
+    const Side& b = TOKENS_M ? w : x;
+    CUtensorMap map_a, map_b;
+    if (int rc = make_map(&map_a, a.codes, a.rows, P.blocks, S::kRowsA)) return rc;
+    if (int rc = make_map(&map_b, b.codes, b.rows, P.blocks, N)) return rc;
+    P.sa = a.scales;
+    P.sb = b.scales;
+    P.rows_a = a.rows;
+    P.rows_b = b.rows;
+    P.tiles_a = int((a.rows + S::kRowsA - 1) / S::kRowsA);
+    P.tiles_b = int((b.rows + N - 1) / N);
+    P.tiles = int64_t(P.tiles_a) * P.tiles_b;
+    P.stages_k = (P.blocks + 7) / 8;
+    P.splits = 1;
+    int64_t grid = std::min<int64_t>(P.tiles, sms);
+    if (!TOKENS_M) {
+        // every SM streams: split K until the CTAs fill the GPU, down to two stages each
+        while (P.splits < 8 && P.tiles * P.splits * 2 <= int64_t(sms) * S::kPerSm && P.stages_k / (P.splits * 2) >= 2)
+            P.splits *= 2;
+        grid = P.tiles * P.splits;
+        if (grid > 0x7FFFFFFF) return fail(SWB_E_SHAPE);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(grid));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(P.splits);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, P);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return fail(SWB_E_CUDA, cudaGetErrorString(e));
+    }
+    return SWB_OK;
+}
+
+template <typename T>
+int dispatch_matmul(const Side& x, const Side& w, const MatmulParams& P, cudaStream_t stream) {
+    if (P.tokens <= 16) return launch_matmul<T, 16, 1, false>(x, w, P, stream);
+    if (P.tokens <= 32) return launch_matmul<T, 32, 1, false>(x, w, P, stream);
+    if (P.tokens <= 64) return launch_matmul<T, 64, 1, false>(x, w, P, stream);
+    if (P.tokens <= 128) return launch_matmul<T, 128, 1, false>(x, w, P, stream);
+    return launch_matmul<T, 192, 1, true>(x, w, P, stream);
+}
+
+}  // namespace
+}  // namespace swb
+
+using namespace swb;
+
+extern "C" int swb_mx4_matmul(int type, const void* x_codes, const void* x_scales, const void* w_codes,
+                              const void* w_scales, const void* bias, const void* residual, void* out, int64_t tokens,
+                              int64_t rows, int64_t cols, unsigned flags, void* stream) {
+    if (type != SWB_F16 && type != SWB_BF16) return fail(SWB_E_TYPE);
+    if (flags & ~SWB_RESIDUAL) return fail(SWB_E_INPUT, "unknown flags");
+    if (tokens < 0 || tokens > SWB_MX4_MAX_TOKENS || rows <= 0 || cols <= 0 || rows > SWB_MX4_MAX_DIM ||
+        cols > SWB_MX4_MAX_DIM)
+        return fail(SWB_E_SHAPE);
+    if (tokens == 0) return SWB_OK;
+    if (!x_codes || !x_scales || !w_codes || !w_scales) return fail(SWB_E_INPUT);
+    if (!out) return fail(SWB_E_HALF_OUTPUT);
+    if ((flags & SWB_RESIDUAL) && !residual) return fail(SWB_E_RESIDUAL);
+    if ((reinterpret_cast<uintptr_t>(x_codes) | reinterpret_cast<uintptr_t>(w_codes)) % 16)
+        return fail(SWB_E_ALIGNMENT, "codes must be 16-byte aligned");
+    const int64_t blocks = mx_blocks(cols);
+    const size_t out_bytes = size_t(tokens) * rows * 2;
+    if (overlaps(out, out_bytes, x_codes, size_t(tokens) * blocks * kMxBlockBytes) ||
+        overlaps(out, out_bytes, x_scales, size_t(tokens) * blocks) ||
+        overlaps(out, out_bytes, w_codes, size_t(rows) * blocks * kMxBlockBytes) ||
+        overlaps(out, out_bytes, w_scales, size_t(rows) * blocks) ||
+        (bias && overlaps(out, out_bytes, bias, size_t(rows) * 2)))
+        return fail(SWB_E_OVERLAP_INPUT);
+    // the residual may be the output itself: each value is read by the thread that writes it
+    if ((flags & SWB_RESIDUAL) && residual != out && overlaps(out, out_bytes, residual, out_bytes))
+        return fail(SWB_E_OVERLAP_INPUT);
+    MatmulParams P;
+    std::memset(&P, 0, sizeof P);
+    P.bias = bias;
+    P.residual = (flags & SWB_RESIDUAL) ? residual : nullptr;
+    P.out = out;
+    P.tokens = tokens;
+    P.rows = rows;
+    P.blocks = int(blocks);
+    const Side x{x_codes, static_cast<const unsigned char*>(x_scales), tokens};
+    const Side w{w_codes, static_cast<const unsigned char*>(w_scales), rows};
+    auto s = static_cast<cudaStream_t>(stream);
+    return type == SWB_F16 ? dispatch_matmul<__half>(x, w, P, s) : dispatch_matmul<__nv_bfloat16>(x, w, P, s);
+}

@@ -875,9 +875,10 @@ int swb_device_error(int clear, int* out) {
         e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof zero);
         if (e != cudaSuccess) return fail(SWB_E_CUDA, cudaGetErrorString(e));
     }
-    int more = 0;  // the other translation units' words
-    if (int rc = moe_device_error(clear, &more)) return rc;
-    if (out) *out = v | more;
+    int moe = 0, matmul = 0;  // the other translation units' words
+    if (int rc = moe_device_error(clear, &moe)) return rc;
+    if (int rc = mx4_matmul_device_error(clear, &matmul)) return rc;
+    if (out) *out = v | moe | matmul;
     return SWB_OK;
 }
 

@@ -17,12 +17,12 @@ from .binding import (CublasBaseline, config_ids, config_info, device_error, ffn
                       layer_config_ids, layer_workspace, project,
                       residual_epilogue, swiglu, swiglu_out, valid_config)
 from .moe import moe, moe_out, moe_workspace
-from .mx4 import (mx4_dequantize, mx4_dequantize_out, mx4_empty, mx4_project, mx4_project_out, mx4_quantize,
-                  mx4_quantize_out)
+from .mx4 import (mx4_dequantize, mx4_dequantize_out, mx4_empty, mx4_matmul, mx4_matmul_out, mx4_project,
+                  mx4_project_out, mx4_quantize, mx4_quantize_out)
 from ._lib import build, lib
 
 __all__ = ["swiglu_out", "swiglu", "config_ids", "config_info", "valid_config", "gate", "project", "ffn", "ffn_fused", "ffn_tp",
            "layer_config_ids", "layer_workspace",
            "residual_epilogue", "device_error", "CublasBaseline", "build", "lib",
            "mx4_quantize", "mx4_quantize_out", "mx4_dequantize", "mx4_dequantize_out", "mx4_empty",
-           "mx4_project", "mx4_project_out", "moe", "moe_out", "moe_workspace"]
+           "mx4_project", "mx4_project_out", "mx4_matmul", "mx4_matmul_out", "moe", "moe_out", "moe_workspace"]

@@ -130,6 +130,7 @@ def _declare(L: ctypes.CDLL) -> ctypes.CDLL:
         "swb_mx4_quantize": ([_i, _vp, _i64, _vp, _vp, _i64, _i64, _vp], _i),
         "swb_mx4_dequantize": ([_i, _vp, _vp, _vp, _i64, _i64, _i64, _vp], _i),
         "swb_mx4_project": ([_i, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _u, _vp], _i),
+        "swb_mx4_matmul": ([_i] + [_vp] * 7 + [_i64] * 3 + [_u, _vp], _i),
         "swb_moe_workspace_bytes": ([_i, _i, _i, _i], _z),
         "swb_moe": ([_i, _u, _vp, _i64] + [_vp] * 10 + [_i] * 5 + [_vp, _z, _vp], _i),
         "swb_device_error": ([_i, ctypes.POINTER(_i)], _i),

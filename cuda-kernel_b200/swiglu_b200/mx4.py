@@ -148,3 +148,34 @@ def mx4_project(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bias
     out = torch.empty((x.size(0), codes.size(0)), dtype=dtype or x.dtype, device=x.device)
     mx4_project_out(x, codes, scales, out, bias, residual)
     return out
+
+
+def mx4_matmul_out(x_codes: torch.Tensor, x_scales: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+                   out: torch.Tensor, bias: torch.Tensor | None = None,
+                   residual: torch.Tensor | None = None) -> None:
+    """out[t] = W x[t] (+ bias) (+ residual[t]), both sides in four bits (swb_mx4_matmul).
+
+    x: [tokens, cols] and W: [rows, cols] as codes and scales of the same number of blocks (codes
+    beyond a ragged cols are zero, as ``mx4_quantize`` leaves them); out: [tokens, rows] fp16 or
+    bf16, the type of bias [rows] and residual [tokens, rows]. ``residual`` may be ``out`` itself.
+    """
+    _check(out.is_cuda and out.dtype in (torch.float16, torch.bfloat16), "out must be a CUDA FP16 or BF16 matrix")
+    _check(x_codes.dim() == 2 and codes.dim() == 2 and x_scales.dim() == 2, "codes must be matrices")
+    tokens, rows, cols = x_codes.size(0), codes.size(0), x_scales.size(1) * BLOCK
+    _check_packed(x_codes, x_scales, (tokens, cols), out.device)
+    _check_packed(codes, scales, (rows, cols), out.device)
+    _product_arguments(out, out.dtype, tokens, rows, bias, residual)
+    _call(out.device, _lib.lib().swb_mx4_matmul, _TYPES[out.dtype], x_codes.data_ptr(), x_scales.data_ptr(),
+          codes.data_ptr(), scales.data_ptr(), None if bias is None else bias.data_ptr(),
+          None if residual is None else residual.data_ptr(), out.data_ptr(), tokens, rows, cols,
+          _lib.SWB_RESIDUAL if residual is not None else 0)
+
+
+def mx4_matmul(x_codes: torch.Tensor, x_scales: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+               bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+               dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """Allocating wrapper of ``mx4_matmul_out``."""
+    _check(x_codes.dim() == 2 and codes.dim() == 2, "codes must be matrices")
+    out = torch.empty((x_codes.size(0), codes.size(0)), dtype=dtype, device=x_codes.device)
+    mx4_matmul_out(x_codes, x_scales, codes, scales, out, bias, residual)
+    return out

@@ -314,6 +314,16 @@ SWB_API int swb_mx4_project(int type, const void* codes, const void* scales, con
                             const void* bias, const void* residual, void* out, int64_t tokens, int64_t rows,
                             int64_t cols, unsigned flags, void* stream);
 
+/* The product of two four-bit matrices: out[t][r] = W[r].X[t] (+ bias[r]) (+ residual[t][r]).
+ * x_codes, x_scales: X [tokens, cols]; w_codes, w_scales: W [rows, cols], both codes 16-byte
+ * aligned; a ragged last block's codes beyond cols must be zero, as swb_mx4_quantize leaves
+ * them. type: SWB_F16 or SWB_BF16 of out [tokens, rows], bias [rows] or NULL and residual
+ * [tokens, rows] (read with SWB_RESIDUAL; may be out itself). Sums in fp32 on the tensor
+ * cores (every product and scale exact). tokens == 0: nothing to do. */
+SWB_API int swb_mx4_matmul(int type, const void* x_codes, const void* x_scales, const void* w_codes,
+                           const void* w_scales, const void* bias, const void* residual, void* out, int64_t tokens,
+                           int64_t rows, int64_t cols, unsigned flags, void* stream);
+
 /* ---- mixture-of-experts layer for a few tokens (no counterpart in the reference) ----
  *
  * logits = router x, the topk largest select a token's experts (ties: the lowest index;

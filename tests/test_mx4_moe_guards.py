@@ -76,6 +76,30 @@ def test_project_guards():
     assert call(res=o + 2, flags=_lib.SWB_RESIDUAL | _lib.SWB_HALF_OUT) == _lib.SWB_E_OVERLAP_INPUT
 
 
+def test_matmul_guards():
+    f = L().swb_mx4_matmul
+    xc, xs, w, s, o, e = (F + k * (1 << 30) for k in range(6))
+    ok = dict(type=0, xc=xc, xs=xs, w=w, s=s, bias=None, res=None, out=o, tokens=2, rows=8, cols=64, flags=0)
+
+    def call(**kw):
+        a = {**ok, **kw}
+        return f(a["type"], a["xc"], a["xs"], a["w"], a["s"], a["bias"], a["res"], a["out"], a["tokens"], a["rows"],
+                 a["cols"], a["flags"], None)
+    assert call(type=2) == _lib.SWB_E_TYPE and call(flags=_lib.SWB_HALF_OUT) == _lib.SWB_E_INPUT
+    assert call(tokens=-1) == _lib.SWB_E_SHAPE and call(rows=0) == _lib.SWB_E_SHAPE and call(cols=0) == _lib.SWB_E_SHAPE
+    assert call(rows=_lib.SWB_MX4_MAX_DIM + 1) == _lib.SWB_E_SHAPE
+    assert call(tokens=0, out=None) == _lib.SWB_OK
+    for name in ("xc", "xs", "w", "s"):
+        assert call(**{name: None}) == _lib.SWB_E_INPUT, name
+    assert call(out=None) == _lib.SWB_E_HALF_OUTPUT
+    assert call(flags=_lib.SWB_RESIDUAL) == _lib.SWB_E_RESIDUAL
+    assert call(xc=xc + 8) == _lib.SWB_E_ALIGNMENT and call(w=w + 4) == _lib.SWB_E_ALIGNMENT
+    for name in ("xc", "xs", "w", "s"):
+        assert call(out=ok[name]) == _lib.SWB_E_OVERLAP_INPUT, name
+    assert call(bias=o + 4) == _lib.SWB_E_OVERLAP_INPUT
+    assert call(res=o + 2, flags=_lib.SWB_RESIDUAL) == _lib.SWB_E_OVERLAP_INPUT
+
+
 def test_moe_guards():
     f = L().swb_moe
     x, r, g, u, d, y, ws, gs, us, ds, ids, wt = (F + k * (1 << 30) for k in range(12))
