@@ -35,17 +35,17 @@ int launch_moe(const MoeParams& P, cudaStream_t stream) {
     if (sms <= 0) return check_launch();
     auto kernel = moe_kernel<T, MX, NT>;
     if (int rc = allow_smem(kernel, smem_set, S::kSmem)) return rc;
+    static_assert(S::kStages >= 3, "a ring");
     // every CTA resident at once: the cooperative launch makes the runtime check it
-    return launch_ex(kernel, unsigned(sms * S::kPerSm), kMoeThreads, S::kSmem, stream, true, P);
+    return launch_ex(kernel, unsigned(sms), kStreamThreads, S::kSmem, stream, true, P);
 }
 
 template <typename T, bool MX>
 int dispatch_moe(const MoeParams& P, cudaStream_t stream) {
-    // an expert can be given every token
+    // an expert can be given every token; beyond 32 in groups of 32
     if (P.tokens <= 8) return launch_moe<T, MX, 1>(P, stream);
     if (P.tokens <= 16) return launch_moe<T, MX, 2>(P, stream);
-    if (P.tokens <= 32) return launch_moe<T, MX, 4>(P, stream);
-    return launch_moe<T, MX, 8>(P, stream);
+    return launch_moe<T, MX, 4>(P, stream);
 }
 
 }  // namespace
@@ -82,8 +82,6 @@ int swb_moe(int type, unsigned flags, const void* x, int64_t x_pitch, const void
     if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(SWB_E_ALIGNMENT, "workspace must be 256-byte aligned");
     const uintptr_t bases[3] = {reinterpret_cast<uintptr_t>(gate), reinterpret_cast<uintptr_t>(up),
                                 reinterpret_cast<uintptr_t>(down)};
-    const uintptr_t scales[3] = {reinterpret_cast<uintptr_t>(gate_scales), reinterpret_cast<uintptr_t>(up_scales),
-                                 reinterpret_cast<uintptr_t>(down_scales)};
     if (mx && ((bases[0] | bases[1] | bases[2]) % 16)) return fail(SWB_E_ALIGNMENT, "codes must be 16-byte aligned");
     // what the call writes may not overlap what it reads, nor each other
     const size_t n = size_t(experts) * hidden * inter;
@@ -138,13 +136,6 @@ int swb_moe(int type, unsigned flags, const void* x, int64_t x_pitch, const void
     P.renormalize = (flags & SWB_MOE_RENORMALIZE) != 0;
     P.x_aligned = hidden % 8 == 0 && x_pitch % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
     P.router_aligned = hidden % 8 == 0 && reinterpret_cast<uintptr_t>(router) % 16 == 0;
-    if (mx) {
-        P.gate_aligned = mx_blocks(hidden) % 4 == 0 && ((scales[0] | scales[1]) & 3) == 0;
-        P.down_aligned = mx_blocks(inter) % 4 == 0 && (scales[2] & 3) == 0;
-    } else {
-        P.gate_aligned = hidden % 8 == 0 && ((bases[0] | bases[1]) & 15) == 0;
-        P.down_aligned = inter % 8 == 0 && (bases[2] & 15) == 0;
-    }
     auto s = static_cast<cudaStream_t>(stream);
     if (type == SWB_F16) return mx ? dispatch_moe<__half, true>(P, s) : dispatch_moe<__half, false>(P, s);
     return mx ? dispatch_moe<__nv_bfloat16, true>(P, s) : dispatch_moe<__nv_bfloat16, false>(P, s);

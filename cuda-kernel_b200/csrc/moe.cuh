@@ -12,23 +12,28 @@
 //   router  a CTA takes four experts by four tokens, its warps splitting H; products
 //           and sums in 64 bits, so that the selection does not depend on the order of
 //           a sum. The CTA that completes a group of four tokens selects their experts.
-//   gate    items (expert, 16 rows of Wg and Wu) spread over the CTAs; h, rounded to
-//           the layer's type (the operand of the next product), goes to the workspace
-//           with an expert's tokens side by side.
+//   gate    items (expert, 16 rows of Wg and Wu) spread over the CTAs; h goes to the
+//           workspace with an expert's tokens side by side, as two values of the layer's
+//           type (h rounded, and what the rounding left), so that y keeps h's fp32 bits.
 //   down    a CTA owns 16 rows of y at a time and takes every expert's product for
-//           them in expert order, so y needs no atomics and repeats bit for bit.
+//           them in expert order, so y needs no atomics and repeats bit for bit. Its
+//           weights are on their way while the grid waits for h.
+//
+// An expert with more than 32 tokens is taken in groups of 32, each group of a tile right
+// after the other, so that the second finds the weights in L2.
 #pragma once
 
 #include "stream.cuh"
 
 namespace swb {
 
-constexpr int kMoeWarps = 8;
-constexpr int kMoeThreads = kMoeWarps * 32;
 constexpr int kMoeMaxTokens = 64;
 constexpr int kMoeMaxExperts = 256;
 constexpr int kMoeMaxTopk = 16;
+constexpr int kMoeGroup = 32;  // tokens of an item
+constexpr int kMoeMaxGroups = kMoeMaxExperts + kMoeMaxTokens * kMoeMaxTopk / kMoeGroup;
 constexpr int kRouteExperts = 4, kRouteTokens = 4;  // of a router unit
+constexpr int kRouteThreads = kConsumers * 32;
 
 struct MoeParams {
     const void* x;
@@ -42,12 +47,11 @@ struct MoeParams {
     double* logits;  // [tokens, experts]
     int* picks;      // [tokens, topk]
     float* shares;   // [tokens, topk]
-    void* h;         // [tokens * topk, h_pitch]
+    void* h;         // [2][tokens * topk, h_pitch]: rounded, then what is left
     int64_t x_pitch;
     int tokens, hidden, inter, experts, topk, h_pitch;
     int renormalize;
-    int x_aligned, router_aligned;   // 16-byte pieces of the rows of x, of Wr
-    int gate_aligned, down_aligned;  // copies of Wg and Wu, of Wd (WeightView::aligned)
+    int x_aligned, router_aligned;  // 16-byte pieces of the rows of x, of Wr
 };
 
 // Offsets of the workspace's parts.
@@ -61,35 +65,32 @@ __host__ __device__ inline MoeWorkspace moe_workspace(int tokens, int experts, i
     m.picks = m.logits + size_t(tokens) * experts * 8;
     m.shares = m.picks + size_t(tokens) * topk * 4;
     m.h = (m.shares + size_t(tokens) * topk * 4 + 255) / 256 * 256;
-    m.total = m.h + size_t(tokens) * topk * moe_h_pitch(inter) * 2;
+    m.total = m.h + size_t(tokens) * topk * moe_h_pitch(inter) * 4;
     return m;
 }
 
-// What every CTA derives from the selection.
+// What every CTA derives from the selection. Rows of h stand in the order of their experts,
+// then tokens; a group is up to 32 of an expert's rows.
 struct MoeRoute {
-    int active;                                // experts with a token
-    float share[kMoeMaxTokens * kMoeMaxTopk];  // [token, place]: the expert's weight
-    short pick[kMoeMaxTokens * kMoeMaxTopk];   // [token, place]: the expert
-    short act[kMoeMaxTokens * kMoeMaxTopk];    // [token, place]: its index among the active
-    short row[kMoeMaxTokens * kMoeMaxTopk];    // [token, place]: its row of h
-    short count[kMoeMaxExperts];               // tokens of each expert
-    short expert[kMoeMaxExperts];              // active experts, ascending
-    short start[kMoeMaxExperts + 1];           // first row of h of each active expert, and the end
-    unsigned char token[kMoeMaxTokens * kMoeMaxTopk];  // token of each row of h
+    int groups;
+    float share[kMoeMaxTokens * kMoeMaxTopk];          // of each row of h: its expert's weight
+    short pick[kMoeMaxTokens * kMoeMaxTopk];           // [token, place]: the expert
+    short count[kMoeMaxExperts];                       // tokens of each expert
+    short expert[kMoeMaxGroups];                       // of each group
+    short start[kMoeMaxGroups + 1];                    // its first row of h, and the end
+    short first[kMoeMaxGroups];                        // the expert's first group
+    short of_expert[kMoeMaxGroups];                    // and how many it has
+    unsigned char token[kMoeMaxTokens * kMoeMaxTopk];  // of each row of h
 };
 
 template <typename T, bool MX, int NT>
 struct MoeShape {
-    static constexpr int kPerSm = NT <= 2 ? 2 : 1;  // CTAs of an SM
-    static constexpr int kGateStages = NT <= 2 ? 4 : 6;
-    using Gate = WarpStream<T, MX, 2, NT, kGateStages>;
-    using Down = WarpStream<T, MX, 1, NT, 2 * kGateStages>;
-    static constexpr size_t kRing = size_t(Gate::kRing) * kMoeWarps;
-    static constexpr int kPart = 2 * NT * 8 * kPartPitch;  // floats of a warp
-    static constexpr size_t kPartBytes = size_t(kMoeWarps) * kPart * 4;
-    static constexpr size_t kSmem = kRing + kPartBytes + (sizeof(MoeRoute) + 15) / 16 * 16;
-    static_assert(int(Down::kRing) <= int(Gate::kRing), "one ring serves both phases");
-    static_assert(kSmem + 1024 <= 233472 / kPerSm && kSmem <= 232448 - 1024, "shared memory");
+    using Pipe = Stream<T, MX, NT>;
+    static constexpr size_t kOther = (sizeof(MoeRoute) + 15) / 16 * 16 + kMoeMaxTokens * kTileRows * 4 + 1280;
+    static constexpr int kStages = Pipe::stages(kOther);
+    static constexpr size_t kRoute = (Pipe::bytes(kStages) + 15) / 16 * 16;   // offset of MoeRoute
+    static constexpr size_t kTotal = kRoute + (sizeof(MoeRoute) + 15) / 16 * 16;  // of y's sums
+    static constexpr size_t kSmem = kTotal + kMoeMaxTokens * kTileRows * 4;
 };
 
 __device__ __forceinline__ uint32_t moe_ld_acquire(const uint32_t* p) {
@@ -98,26 +99,29 @@ __device__ __forceinline__ uint32_t moe_ld_acquire(const uint32_t* p) {
     return v;
 }
 
-// Grid barrier over one word whose low 31 bits are zero between barriers: CTA 0 adds
-// what the others' ones leave to 2^31, so the top bit flips once everybody arrived.
-// Waits at most kWaitLimitNs; false (in every thread of the CTA) when it gave up.
+// One thread's part of a grid barrier over a word whose low 31 bits are zero between
+// barriers: CTA 0 adds what the others' ones leave to 2^31, so the top bit flips once
+// everybody arrived. Waits at most kWaitLimitNs; false when it gave up. What the CTA wrote
+// before (ordered by a barrier among its threads) is visible to every CTA afterwards.
+__device__ __forceinline__ bool moe_grid_arrive_wait(uint32_t* word) {
+    __threadfence();
+    const uint32_t add = blockIdx.x == 0 ? 0x80000000u - uint32_t(gridDim.x - 1) : 1u;
+    const uint32_t seen = atomicAdd(word, add) & 0x80000000u;
+    const uint64_t t0 = global_timer_ns();
+    while ((moe_ld_acquire(word) & 0x80000000u) == seen) {
+        if (global_timer_ns() - t0 > kWaitLimitNs) {
+            atomicOr(&g_device_error, 1);
+            return false;
+        }
+    }
+    __threadfence();
+    return true;
+}
+
+// The barrier for every thread of the CTA; false in all of them when it gave up.
 __device__ __forceinline__ bool moe_grid_barrier(uint32_t* word, int* ok) {
     __syncthreads();
-    if (threadIdx.x == 0) {
-        *ok = 1;
-        __threadfence();
-        const uint32_t add = blockIdx.x == 0 ? 0x80000000u - uint32_t(gridDim.x - 1) : 1u;
-        const uint32_t seen = atomicAdd(word, add) & 0x80000000u;
-        const uint64_t t0 = global_timer_ns();
-        while ((moe_ld_acquire(word) & 0x80000000u) == seen) {
-            if (global_timer_ns() - t0 > kWaitLimitNs) {
-                atomicOr(&g_device_error, 1);
-                *ok = 0;
-                break;
-            }
-        }
-        __threadfence();
-    }
+    if (threadIdx.x == 0) *ok = moe_grid_arrive_wait(word);
     __syncthreads();
     return *ok != 0;
 }
@@ -187,6 +191,7 @@ __device__ void moe_select(const MoeParams& P, int token, int lane) {
     }
 }
 
+// The first kRouteThreads threads of the CTA.
 template <typename T>
 __device__ void moe_router(const MoeParams& P, double* scratch, int* flag) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -202,7 +207,7 @@ __device__ void moe_router(const MoeParams& P, double* scratch, int* flag) {
 #pragma unroll
             for (int b = 0; b < kRouteTokens; ++b) sum[a][b] = 0.0;
         const int nt = min(kRouteTokens, P.tokens - t0);
-        for (int k = threadIdx.x * 8; k < P.hidden; k += kMoeThreads * 8) {
+        for (int k = threadIdx.x * 8; k < P.hidden; k += kRouteThreads * 8) {
             uint4 wv[kRouteExperts], xv[kRouteTokens];
 #pragma unroll
             for (int a = 0; a < kRouteExperts; ++a)
@@ -231,19 +236,19 @@ __device__ void moe_router(const MoeParams& P, double* scratch, int* flag) {
                 if (b >= nt) break;
 #pragma unroll
                 for (int d = 16; d > 0; d >>= 1) sum[a][b] += __shfl_xor_sync(0xFFFFFFFFu, sum[a][b], d);
-                if (lane == 0) scratch[(a * kRouteTokens + b) * kMoeWarps + warp] = sum[a][b];
+                if (lane == 0) scratch[(a * kRouteTokens + b) * kConsumers + warp] = sum[a][b];
             }
-        __syncthreads();
+        named_barrier_sync(1, kRouteThreads);
         if (threadIdx.x < kRouteExperts * kRouteTokens) {
             const int a = threadIdx.x / kRouteTokens, b = threadIdx.x % kRouteTokens;
             if (e0 + a < P.experts && b < nt) {
                 double s = 0.0;
-                for (int j = 0; j < kMoeWarps; ++j) s += scratch[(a * kRouteTokens + b) * kMoeWarps + j];
+                for (int j = 0; j < kConsumers; ++j) s += scratch[(a * kRouteTokens + b) * kConsumers + j];
                 P.logits[size_t(t0 + b) * P.experts + e0 + a] = s;
             }
             __threadfence();
         }
-        __syncthreads();
+        named_barrier_sync(1, kRouteThreads);
         if (threadIdx.x == 0) {
             *flag = atomicAdd(P.sync + 1 + group, 1u) == uint32_t(expert_units - 1);
             if (*flag) {
@@ -251,204 +256,201 @@ __device__ void moe_router(const MoeParams& P, double* scratch, int* flag) {
                 __threadfence();
             }
         }
-        __syncthreads();
+        named_barrier_sync(1, kRouteThreads);
         if (*flag && warp < nt) moe_select<T>(P, t0 + warp, lane);
-        __syncthreads();
+        named_barrier_sync(1, kRouteThreads);
     }
 }
 
-// Lists of each expert's tokens, in token order, the same in every CTA.
+// Groups of each expert's tokens, in token order, the same in every CTA.
 __device__ inline void moe_lists(const MoeParams& P, MoeRoute& R) {
     const int n = P.tokens * P.topk, t = threadIdx.x;
-    for (int i = t; i < n; i += kMoeThreads) {
-        R.pick[i] = short(__ldcg(P.picks + i));
-        R.share[i] = __ldcg(P.shares + i);
+    for (int i = t; i < n; i += kStreamThreads) R.pick[i] = short(__ldcg(P.picks + i));
+    __syncthreads();
+    if (t < kMoeMaxExperts) {
+        int mine = 0;
+        for (int i = 0; i < n; ++i) mine += R.pick[i] == t;
+        R.count[t] = short(mine);
     }
     __syncthreads();
-    int mine = 0;
-    if (t < P.experts)
-        for (int i = 0; i < n; ++i) mine += R.pick[i] == t;
-    R.count[t] = mine;
-    __syncthreads();
-    if (t < 32) {  // eight experts a lane: sums of tokens and of active experts before them
+    if (t < 32) {  // eight experts a lane: rows and groups before them
         constexpr int kPer = kMoeMaxExperts / 32;
-        int rows = 0, act = 0;
+        int rows = 0, groups = 0;
         for (int i = 0; i < kPer; ++i) {
-            rows += R.count[t * kPer + i];
-            act += R.count[t * kPer + i] > 0;
+            const int c = R.count[t * kPer + i];
+            rows += c;
+            groups += (c + kMoeGroup - 1) / kMoeGroup;
         }
-        int row = rows, a = act;
+        int row = rows, a = groups;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int r = __shfl_up_sync(0xFFFFFFFFu, row, d), b = __shfl_up_sync(0xFFFFFFFFu, a, d);
             if (t >= d) row += r, a += b;
         }
         if (t == 31) {
-            R.active = a;
-            R.start[a] = row;
+            R.groups = a;
+            R.start[a] = short(row);
         }
         row -= rows;
-        a -= act;
+        a -= groups;
         for (int i = 0; i < kPer; ++i) {
-            const int e = t * kPer + i;
-            if (R.count[e] > 0) {
-                R.expert[a] = short(e);
-                R.start[a++] = short(row);
+            const int e = t * kPer + i, c = R.count[e], k = (c + kMoeGroup - 1) / kMoeGroup;
+            for (int j = 0; j < k; ++j) {
+                R.expert[a + j] = short(e);
+                R.start[a + j] = short(row + j * kMoeGroup);
+                R.first[a + j] = short(a);
+                R.of_expert[a + j] = short(k);
             }
-            row += R.count[e];
+            a += k;
+            row += c;
         }
     }
     __syncthreads();
-    if (t < R.active) {
+    if (t < R.groups && R.first[t] == t) {
         const int e = R.expert[t];
         int row = R.start[t];
         for (int i = 0; i < n; ++i)
             if (R.pick[i] == e) {
                 R.token[row] = static_cast<unsigned char>(i / P.topk);
-                R.act[i] = short(t);
-                R.row[i] = short(row++);
+                R.share[row++] = __ldcg(P.shares + i);
             }
     }
     __syncthreads();
 }
 
-// A tensor of experts' matrices [experts, rows, cols] as the copies see one of them.
-template <bool MX>
-__device__ __forceinline__ WeightView moe_view(int cols, int aligned) {
-    WeightView v;
-    v.blocks = MX ? int(mx_blocks(cols)) : 0;
-    v.row_bytes = MX ? v.blocks * kMxBlockBytes : cols * 2;
-    v.pitch = v.row_bytes;
-    v.steps = (v.row_bytes + kStepBytes - 1) / kStepBytes;
-    v.aligned = aligned != 0;
-    return v;
-}
-
 template <typename T, bool MX, int NT>
-__global__ void __launch_bounds__(kMoeThreads, MoeShape<T, MX, NT>::kPerSm) moe_kernel(const MoeParams P) {
+__global__ void __launch_bounds__(kStreamThreads, 1) moe_kernel(const MoeParams P) {
     using S = MoeShape<T, MX, NT>;
-    using Gate = typename S::Gate;
-    using Down = typename S::Down;
+    using Pipe = typename S::Pipe;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ double scratch[kRouteExperts * kRouteTokens * kMoeWarps];
-    __shared__ int flag;
-    float* part = reinterpret_cast<float*>(smem + S::kRing);
-    MoeRoute& R = *reinterpret_cast<MoeRoute*>(smem + S::kRing + S::kPartBytes);
+    __shared__ double scratch[kRouteExperts * kRouteTokens * kConsumers];
+    __shared__ int flag, sums_ok;
+    MoeRoute& R = *reinterpret_cast<MoeRoute*>(smem + S::kRoute);
+    float* total = reinterpret_cast<float*>(smem + S::kTotal);  // [token][16 rows of y]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = gridDim.x, b = blockIdx.x;
-    const uint32_t ring = smem_u32(smem) + warp * Gate::kRing;
+    const auto l = Pipe::layout(smem_u32(smem), S::kStages);
+    if (threadIdx.x == kStreamThreads - 1) Pipe::init(l);
 
-    moe_router<T>(P, scratch, &flag);
+    if (warp < kConsumers) moe_router<T>(P, scratch, &flag);
     if (!moe_grid_barrier(P.sync, &flag)) return;
     moe_lists(P, R);
 
+    // gate: items [g0, g1) are (expert, tile, group); down: tiles [d0, d1) times every group
+    const int gate_tiles = (P.inter + kTileRows - 1) / kTileRows, down_tiles = (P.hidden + kTileRows - 1) / kTileRows;
+    const long long gate_items = (long long)R.groups * gate_tiles;
+    const int g0 = int(b * gate_items / G), g1 = int((b + 1) * gate_items / G);
+    const int d0 = int((long long)b * down_tiles / G), d1 = int((long long)(b + 1) * down_tiles / G);
+    auto gate_item = [&](int item, int& group, int& row) {
+        const int a = item / gate_tiles, f = R.first[a], k = R.of_expert[a], j = item - f * gate_tiles;
+        group = f + j % k;
+        row = j / k * kTileRows;
+    };
+    WeightView gv[2] = {weight_view<MX>(P.w[0], P.s[0], int64_t(P.experts) * P.inter, P.hidden),
+                        weight_view<MX>(P.w[1], P.s[1], int64_t(P.experts) * P.inter, P.hidden)};
+    gv[0].shifted = gv[1].shifted = gv[0].shifted || gv[1].shifted;
+    const WeightView dv[1] = {weight_view<MX>(P.w[2], P.s[2], int64_t(P.experts) * P.hidden, P.inter)};
+    auto gate_rows = [&](int group, int row) {
+        Tiles<2> t;
+        t.row[0] = t.row[1] = int64_t(R.expert[group]) * P.inter + row;
+        t.rows[0] = t.rows[1] = min(kTileRows, P.inter - row);
+        return t;
+    };
+    auto down_rows = [&](int group, int tile) {
+        Tiles<1> t;
+        t.row[0] = int64_t(R.expert[group]) * P.hidden + tile * kTileRows;
+        t.rows[0] = min(kTileRows, P.hidden - tile * kTileRows);
+        return t;
+    };
     T* h = static_cast<T*>(P.h);
-    {
-        const WeightView v = moe_view<MX>(P.hidden, P.gate_aligned);
-        const int tiles = (P.inter + kTileRows - 1) / kTileRows;
-        const int all = R.active * tiles;
-        const int first = int((long long)b * all / G), mine = int((long long)(b + 1) * all / G) - first;
-        const int rounds = round_count(mine, kMoeWarps);
-        const T* x = static_cast<const T*>(P.x);
-        auto get = [&](int i, Piece<T, 2, NT>& p) {
-            if (i >= rounds) return false;
-            const Round r = round_at(i, mine, kMoeWarps);
-            const int share = kMoeWarps / r.items, part_of = warp % share;
-            const int item = first + r.first + warp / share;
-            const int a = item / tiles, row = item % tiles * kTileRows;
-            const int e = R.expert[a], start = R.start[a];
-            p.count = R.start[a + 1] - start;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-                p.x[n] = x + R.token[start + min(n * 8 + (lane >> 2), p.count - 1)] * P.x_pitch;
-            const int64_t base = int64_t(e) * P.inter + row;
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                p.rows[m] = P.inter - row;
-                p.w[m] = P.w[m] + base * v.pitch;
-                p.s[m] = P.s[m] + base * v.blocks;
-            }
-            p.s0 = v.steps * part_of / share;
-            p.s1 = v.steps * (part_of + 1) / share;
-            return true;
-        };
-        auto done = [&](int i, const Piece<T, 2, NT>& p, const float (&acc)[2][NT][4]) {
-            const Round r = round_at(i, mine, kMoeWarps);
-            const int share = kMoeWarps / r.items;
-            __syncthreads();  // the last round's sums are read
-            store_partial<2, NT>(part + warp * S::kPart, acc, p.count, lane);
-            __syncthreads();
-            for (int c = threadIdx.x; c < r.items * kTileRows * NT * 8; c += kMoeThreads) {
-                const int row16 = c & 15, n = (c >> 4) % (NT * 8), idx = (c >> 4) / (NT * 8);
-                const int item = first + r.first + idx;
-                const int a = item / tiles, row = item % tiles * kTileRows + row16;
-                const int start = R.start[a];
-                if (n >= R.start[a + 1] - start) continue;
-                const float* q = part + idx * share * S::kPart + n * kPartPitch + row16;
-                float g = 0.f, u = 0.f;
-                for (int j = 0; j < share; ++j) {
-                    g += q[j * S::kPart];
-                    u += q[j * S::kPart + NT * 8 * kPartPitch];
-                }
-                // rows up to the pitch of h are zero, so that a whole piece of h may be read
-                h[int64_t(start + n) * P.h_pitch + row] = Num<T>::from_float(row < P.inter ? silu(g) * u : 0.f);
-            }
-        };
-        Gate::run(ring, v, P.hidden, P.x_aligned != 0, get, done);
-    }
-    if (!moe_grid_barrier(P.sync, &flag)) return;
+    const int64_t h_plane = int64_t(P.tokens) * P.topk * P.h_pitch;
+    typename Pipe::Place place;
 
-    {
-        const WeightView v = moe_view<MX>(P.inter, P.down_aligned);
-        const int tiles = (P.hidden + kTileRows - 1) / kTileRows;
-        const int first = int((long long)b * tiles / G), mine = int((long long)(b + 1) * tiles / G) - first;
-        const int per_tile = round_count(R.active, kMoeWarps), rounds = mine * per_tile;
-        T* y = static_cast<T*>(P.y);
-        float* total = reinterpret_cast<float*>(part) + kMoeWarps * (NT * 8 * kPartPitch);  // [tokens][16]
-        auto get = [&](int i, Piece<T, 1, NT>& p) {
-            if (i >= rounds) return false;
-            const Round r = round_at(i % per_tile, R.active, kMoeWarps);
-            const int share = kMoeWarps / r.items, part_of = warp % share;
-            const int a = r.first + warp / share, row = (first + i / per_tile) * kTileRows;
-            const int start = R.start[a];
-            p.count = R.start[a + 1] - start;
+    if (warp == kConsumers) {
+        const uint64_t policy = l2_evict_first_policy();
+        for (int i = g0; i < g1 && place.ok; ++i) {
+            int group, row;
+            gate_item(i, group, row);
+            Pipe::template produce<2>(l, place, gate_rows(group, row), gv, policy);
+        }
+        for (int d = d0; d < d1; ++d)
+            for (int a = 0; a < R.groups && place.ok; ++a)
+                Pipe::template produce<1>(l, place, down_rows(a, d), dv, policy);
+        Pipe::drain(l, place);
+    } else if (warp < kConsumers) {
+        const T* x[2 * NT];
+        for (int i = g0; i < g1 && place.ok; ++i) {
+            int group, row;
+            gate_item(i, group, row);
+            const int start = R.start[group], count = R.start[group + 1] - start;
+            const T* xg[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-                p.x[n] = h + int64_t(start + min(n * 8 + (lane >> 2), p.count - 1)) * P.h_pitch;
-            const int64_t base = int64_t(R.expert[a]) * P.hidden + row;
-            p.rows[0] = P.hidden - row;
-            p.w[0] = P.w[2] + base * v.pitch;
-            p.s[0] = P.s[2] + base * v.blocks;
-            p.s0 = v.steps * part_of / share;
-            p.s1 = v.steps * (part_of + 1) / share;
-            return true;
-        };
-        auto done = [&](int i, const Piece<T, 1, NT>& p, const float (&acc)[1][NT][4]) {
-            constexpr int kPart = NT * 8 * kPartPitch;
-            const int turn = i % per_tile;
-            const Round r = round_at(turn, R.active, kMoeWarps);
-            const int share = kMoeWarps / r.items;
-            __syncthreads();  // the last round's sums are read
-            store_partial<1, NT>(part + warp * kPart, acc, p.count, lane);
-            __syncthreads();
-            for (int c = threadIdx.x; c < P.tokens * kTileRows; c += kMoeThreads) {
-                const int row16 = c & 15, t = c >> 4;
-                float sum = turn == 0 ? 0.f : total[c];
-                for (int j = 0; j < P.topk; ++j) {
-                    const int at = t * P.topk + j, idx = R.act[at] - r.first;
-                    if (idx < 0 || idx >= r.items) continue;
-                    const int n = R.row[at] - R.start[R.act[at]];
-                    const float* q = part + idx * share * kPart + n * kPartPitch + row16;
-                    float d = 0.f;
-                    for (int w = 0; w < share; ++w) d += q[w * kPart];
-                    sum = fmaf(R.share[at], d, sum);
+                xg[n] = static_cast<const T*>(P.x) + R.token[start + min(n * 8 + (lane >> 2), count - 1)] * P.x_pitch;
+            Pipe::template consume<2, false>(l, place, gate_rows(group, row), gv, xg, count, P.hidden, P.x_aligned != 0);
+        }
+        named_barrier_sync(2, kStreamThreads - 32);  // h is complete, or flag says that it will not be
+        for (int d = d0; d < d1 && flag; ++d)
+            for (int a = 0; a < R.groups && place.ok; ++a) {
+                const int start = R.start[a], count = R.start[a + 1] - start;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    x[n] = h + int64_t(start + min(n * 8 + (lane >> 2), count - 1)) * P.h_pitch;
+                    x[NT + n] = x[n] + h_plane;
                 }
-                total[c] = sum;
-                const int row = (first + i / per_tile) * kTileRows + row16;
-                if (turn == per_tile - 1 && row < P.hidden) y[int64_t(t) * P.hidden + row] = Num<T>::from_float(sum);
+                Pipe::template consume<1, true>(l, place, down_rows(a, d), dv, x, count, P.h_pitch, true);
             }
-        };
-        Down::run(ring, v, P.h_pitch, true, get, done);
+    } else {
+        const int thread = threadIdx.x - (kConsumers + 1) * 32;
+        for (int i = g0; i < g1 && Pipe::acquire(l, place); ++i) {
+            int group, row;
+            gate_item(i, group, row);
+            const int start = R.start[group], count = R.start[group + 1] - start;
+            for (int c = thread; c < count * kTileRows; c += kEpilogueThreads) {
+                const int n = c >> 4, r = c & 15;
+                const float g = Pipe::template sum<2>(l, place, 0, n, r), u = Pipe::template sum<2>(l, place, 1, n, r);
+                // rows up to the pitch of h are zero, so that a whole piece of h may be read
+                const float v = row + r < P.inter ? silu(g) * u : 0.f;
+                const T hi = Num<T>::from_float(v);
+                const int64_t at = int64_t(start + n) * P.h_pitch + row + r;
+                h[at] = hi;
+                h[h_plane + at] = Num<T>::from_float(v - Num<T>::to_float(hi));
+            }
+            Pipe::release(l, place);
+        }
+        named_barrier_sync(3, kEpilogueThreads);
+        if (thread == 0) {
+            flag = place.ok && moe_grid_arrive_wait(P.sync);
+            __threadfence();
+        }
+        named_barrier_sync(2, kStreamThreads - 32);
+        T* y = static_cast<T*>(P.y);
+        for (int d = d0; d < d1 && flag; ++d) {
+            for (int c = thread; c < P.tokens * kTileRows; c += kEpilogueThreads) total[c] = 0.f;
+            for (int a = 0; a < R.groups; ++a) {
+                if (thread < 32) {
+                    Pipe::acquire(l, place);
+                    if (thread == 0) sums_ok = place.ok;
+                }
+                named_barrier_sync(3, kEpilogueThreads);  // the sums are there, the last group's additions done
+                place.ok = sums_ok != 0;
+                if (!place.ok) break;
+                const int start = R.start[a], count = R.start[a + 1] - start;
+                for (int c = thread; c < count * kTileRows; c += kEpilogueThreads) {
+                    const int n = c >> 4, r = c & 15;  // a token takes an expert once: no two threads meet
+                    float& sum = total[R.token[start + n] * kTileRows + r];
+                    sum = fmaf(R.share[start + n], Pipe::template sum<1>(l, place, 0, n, r), sum);
+                }
+                Pipe::release(l, place);
+            }
+            if (!place.ok) break;
+            named_barrier_sync(3, kEpilogueThreads);
+            for (int c = thread; c < P.tokens * kTileRows; c += kEpilogueThreads) {
+                const int row = d * kTileRows + (c & 15);
+                if (row < P.hidden) y[int64_t(c >> 4) * P.hidden + row] = Num<T>::from_float(total[c]);
+            }
+            named_barrier_sync(3, kEpilogueThreads);
+        }
     }
 }
 

@@ -253,111 +253,108 @@ struct ProjectParams {
     int half_out;
 };
 
-constexpr int kProjectWarps = 8;
+template <typename T, int NT>
+struct ProjectShape {
+    using Pipe = Stream<T, true, NT>;
+    static constexpr int kStages = Pipe::stages(0);
+    static constexpr size_t kSmem = Pipe::bytes(kStages);
+};
 
 template <typename T, int NT>
-constexpr int project_stages() { return NT <= 2 ? 4 : 6; }
-
-template <typename T, int NT>
-using ProjectStream = WarpStream<T, true, 2, NT, project_stages<T, NT>()>;
-
-template <typename T, int NT>
-constexpr size_t project_smem() {
-    return size_t(kProjectWarps) * (ProjectStream<T, NT>::kRing + 2 * NT * 8 * kPartPitch * 4);
-}
-
-template <typename T, int NT>
-__global__ void __launch_bounds__(kProjectWarps * 32, NT <= 2 ? 2 : 1) project_kernel(const ProjectParams P) {
-    using Stream = ProjectStream<T, NT>;
+__global__ void __launch_bounds__(kStreamThreads, 1) project_kernel(const ProjectParams P) {
+    using Shape = ProjectShape<T, NT>;
+    using Pipe = typename Shape::Pipe;
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float* part = reinterpret_cast<float*>(smem + kProjectWarps * Stream::kRing);
-    constexpr int kPart = 2 * NT * 8 * kPartPitch;
+    const auto l = Pipe::layout(smem_u32(smem), Shape::kStages);
+    if (threadIdx.x == 0) Pipe::init(l);
+    __syncthreads();
+
     const int64_t first = int64_t(blockIdx.x) * P.items / gridDim.x;
-    const int mine = int(int64_t(blockIdx.x + 1) * P.items / gridDim.x - first);
-    const T* x = static_cast<const T*>(P.x);
-
-    WeightView v;
-    v.blocks = int(mx_blocks(P.cols));
-    v.row_bytes = v.blocks * kMxBlockBytes;
-    v.pitch = v.row_bytes;
-    v.steps = (v.blocks + 3) / 4;
-    v.aligned = v.blocks % 4 == 0 && (reinterpret_cast<uintptr_t>(P.s) & 3) == 0;
-
-    const int rounds = round_count(mine, kProjectWarps);
-    auto get = [&](int i, Piece<T, 2, NT>& p) {
-        if (i >= rounds) return false;
-        const Round r = round_at(i, mine, kProjectWarps);
-        const int share = kProjectWarps / r.items, part_of = warp % share;
-        const int64_t item = first + r.first + warp / share;
-        const int tile = int(item % P.tiles);
-        const int64_t t0 = item / P.tiles * (NT * 8);
-        p.count = int(min(int64_t(NT * 8), P.tokens - t0));
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-            p.x[n] = x + (t0 + min(n * 8 + (lane >> 2), p.count - 1)) * P.x_pitch;
-#pragma unroll
+    const int64_t last = int64_t(blockIdx.x + 1) * P.items / gridDim.x;
+    const WeightView one = weight_view<true>(P.w, P.s, P.rows, P.cols);
+    const WeightView v[2] = {one, one};
+    typename Pipe::Place place;
+    auto tiles = [&](int64_t item) {
+        Tiles<2> t;
         for (int m = 0; m < 2; ++m) {
-            const int row = (tile * 2 + m) * kTileRows;
-            p.rows[m] = P.rows - row;
-            p.w[m] = P.w + (p.rows[m] > 0 ? int64_t(row) * v.pitch : 0);
-            p.s[m] = P.s + (p.rows[m] > 0 ? int64_t(row) * v.blocks : 0);
+            t.row[m] = item % P.tiles * 32 + m * kTileRows;
+            t.rows[m] = int(min(int64_t(kTileRows), max(int64_t(0), P.rows - t.row[m])));
         }
-        p.s0 = int(int64_t(v.steps) * part_of / share);
-        p.s1 = int(int64_t(v.steps) * (part_of + 1) / share);
-        return true;
+        return t;
     };
-    auto done = [&](int i, const Piece<T, 2, NT>&, const float (&acc)[2][NT][4]) {
-        const Round r = round_at(i, mine, kProjectWarps);
-        const int share = kProjectWarps / r.items;
-        __syncthreads();  // the last round's sums are read
-        store_partial<2, NT>(part + warp * kPart, acc, NT * 8, lane);
-        __syncthreads();
-        for (int e = threadIdx.x; e < r.items * 32 * NT * 8; e += kProjectWarps * 32) {
-            const int row32 = e & 31, t = (e >> 5) % (NT * 8), idx = (e >> 5) / (NT * 8);
-            const int64_t item = first + r.first + idx;
-            const int64_t token = item / P.tiles * (NT * 8) + t;
-            const int row = int(item % P.tiles) * 32 + row32;
-            if (token >= P.tokens || row >= P.rows) continue;
-            const float* q = part + idx * share * kPart + ((row32 >> 4) * NT * 8 + t) * kPartPitch + (row32 & 15);
-            float a = 0.f;
-            for (int j = 0; j < share; ++j) a += q[j * kPart];
-            if (P.bias) a += Num<T>::to_float(static_cast<const T*>(P.bias)[row]);
-            const int64_t at = token * P.rows + row;
-            if (P.residual) a += Num<T>::to_float(static_cast<const T*>(P.residual)[at]);
-            if (P.half_out)
-                static_cast<T*>(P.out)[at] = Num<T>::from_float(a);
-            else
-                static_cast<float*>(P.out)[at] = a;
+    if (warp == kConsumers) {
+        const uint64_t policy = P.items > P.tiles ? l2_normal_policy() : l2_evict_first_policy();
+        for (int64_t i = first; i < last && place.ok; ++i) Pipe::template produce<2>(l, place, tiles(i), v, policy);
+        Pipe::drain(l, place);
+    } else if (warp < kConsumers) {
+        const T* x[NT];
+        for (int64_t i = first; i < last && place.ok; ++i) {
+            const int64_t t0 = i / P.tiles * (NT * 8);
+            const int count = int(min(int64_t(NT * 8), P.tokens - t0));
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                x[n] = static_cast<const T*>(P.x) + (t0 + min(n * 8 + (lane >> 2), count - 1)) * P.x_pitch;
+            Pipe::template consume<2, false>(l, place, tiles(i), v, x, count, P.cols, P.x_aligned != 0);
         }
-    };
-    Stream::run(smem_u32(smem + warp * Stream::kRing), v, P.cols, P.x_aligned != 0, get, done);
+    } else {
+        const int thread = threadIdx.x - (kConsumers + 1) * 32;
+        for (int64_t i = first; i < last && Pipe::acquire(l, place); ++i) {
+            const int64_t t0 = i / P.tiles * (NT * 8);
+            const int count = int(min(int64_t(NT * 8), P.tokens - t0)), row0 = int(i % P.tiles) * 32;
+            for (int e = thread; e < count * 32; e += kEpilogueThreads) {
+                const int t = e >> 5, row = row0 + (e & 31);
+                if (row >= P.rows) continue;
+                float a = Pipe::template sum<2>(l, place, (e & 31) >> 4, t, e & 15);
+                if (P.bias) a += Num<T>::to_float(static_cast<const T*>(P.bias)[row]);
+                const int64_t at = (t0 + t) * P.rows + row;
+                if (P.residual) a += Num<T>::to_float(static_cast<const T*>(P.residual)[at]);
+                if (P.half_out)
+                    static_cast<T*>(P.out)[at] = Num<T>::from_float(a);
+                else
+                    static_cast<float*>(P.out)[at] = a;
+            }
+            Pipe::release(l, place);
+        }
+    }
 }
 
 template <typename T, int NT>
 int launch_project(ProjectParams P, cudaStream_t stream) {
+    using Shape = ProjectShape<T, NT>;
     static std::atomic<uint64_t> smem_set{0};
     const int sms = sm_count();
     if (sms <= 0) return check_launch();
     auto kernel = project_kernel<T, NT>;
-    constexpr size_t smem = project_smem<T, NT>();
-    static_assert(smem <= (NT <= 2 ? kSmemPerSm / 2 - 1024 : kSmemPerCtaMax), "ring and partial sums fit");
-    if (int rc = allow_smem(kernel, smem_set, smem)) return rc;
+    static_assert(Shape::kStages >= 3, "a ring");
+    if (int rc = allow_smem(kernel, smem_set, Shape::kSmem)) return rc;
     P.tiles = (P.rows + 31) / 32;
     P.items = int64_t(P.tiles) * ((P.tokens + NT * 8 - 1) / (NT * 8));
-    const unsigned grid = unsigned(std::min<int64_t>(P.items, int64_t(sms) * (NT <= 2 ? 2 : 1)));
-    return launch_ex(kernel, grid, kProjectWarps * 32, smem, stream, false, P);
+    const unsigned grid = unsigned(std::min<int64_t>(P.items, sms));
+    return launch_ex(kernel, grid, kStreamThreads, Shape::kSmem, stream, false, P);
 }
 
 template <typename T>
 int dispatch_project(const ProjectParams& P, cudaStream_t stream) {
     if (P.tokens <= 8) return launch_project<T, 1>(P, stream);
     if (P.tokens <= 16) return launch_project<T, 2>(P, stream);
-    if (P.tokens <= 32) return launch_project<T, 4>(P, stream);
-    return launch_project<T, 8>(P, stream);
+    return launch_project<T, 4>(P, stream);
 }
 
 }  // namespace
+
+int mx4_device_error(int clear, int* out) {
+    int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, g_device_error, sizeof v);
+    if (e == cudaSuccess && clear) {
+        const int zero = 0;
+        e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof zero);
+    }
+    if (e != cudaSuccess) return fail(SWB_E_CUDA, cudaGetErrorString(e));
+    *out = v;
+    return SWB_OK;
+}
+
 }  // namespace swb
 
 using namespace swb;

@@ -362,9 +362,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
             for (int m = 0; m < MT; ++m) {
                 const int use = MT == 2 ? m : acc;
-                ok = mbar_wait(smem_u32(acc_full + use), ph);
+                ok = mbar_wait_warp(smem_u32(acc_full + use), ph);
                 if (!ok) break;
-                __syncwarp();
                 fence_after();
                 const int in_tile = m * kMmaM + warp * 32 + lane;
                 if constexpr (TOKENS_M) {

@@ -1,21 +1,28 @@
 // Products of a streamed weight matrix with a few 16-bit tokens, as mma.sync tiles.
 //
-// A warp takes 16 rows of a matrix (or of NM matrices, or NM such tiles) and a range
-// of steps along the row; a step is 64 bytes of every row: 32 values of a 16-bit
-// matrix, 128 of an MXFP4 one. The weights are the m16n8k16 A operand, eight tokens
-// per N tile the B operand, sums in fp32. The order of k inside a step is free as
-// long as both operands agree, so each lane keeps the 16 bytes of its row that it
-// loaded itself (16-bit matrices) and reads B as one 16-byte piece of a token's row.
+// A CTA works through items: one or two tiles of 16 weight rows (NM: the gate's and the
+// up projection's rows of one expert, or two neighbouring tiles of a matrix) against up
+// to NT * 8 tokens over the whole row. Few-token products are bound by the bytes of the
+// weights, so the CTA is a pipeline that never drains between items:
 //
-// Batch-one and few-token products are bound by the bytes of the weights: every warp
-// keeps STAGES - 1 steps in flight through its own ring of asynchronous copies (no
-// barrier between warps), while the tokens, a few KB that every tile reads again,
-// come through L1 into registers one sub-step ahead.
+//   producer   one warp; each lane copies its row's next piece (1 or 2 KB, a bulk copy)
+//              into a ring of stages, running ahead across items as far as the ring goes
+//   consumers  kWarps warps share each stage by columns; weights are the m16n8k16 A operand,
+//              eight tokens the B operand, sums in fp32. The tokens, a few KB that every item
+//              reads again, come through L1 into registers. (With the weights on the same
+//              path their latency would be the weights': loads return in order.)
+//   epilogue   three warps add the consumers' partial sums, kept in shared memory, and finish
+//              the item while the consumers are at the next one.
 //
-// MXFP4: a step's codes are decoded in registers, each block of 32 values is summed
-// from zero and added to the totals times its scale (both scales are powers of two,
-// so the only roundings are the fp32 sums'). The copies swap pieces between lanes of
-// a quad through the ring, hence the warp barrier after each wait.
+// The order of k inside 32 values is free as long as both operands agree, so a lane's four
+// registers of A and of B are one 16-byte piece of its row.
+//
+// MXFP4: codes are decoded in registers, each block of 32 values is summed from zero and
+// added to the totals times its scale (both scales are powers of two, so the only
+// roundings are the fp32 sums').
+//
+// Rows that do not start on 16 bytes (16-bit matrices of ragged sizes, scales of ragged
+// rows) are copied from the 16 bytes before and read back shifted. Waits are bounded.
 #pragma once
 
 #include "device.cuh"
@@ -24,7 +31,7 @@
 namespace swb {
 
 constexpr int kTileRows = 16;
-constexpr int kStepBytes = 64;  // of each row
+constexpr int kUnitBytes = 64;  // of a row: what a consumer warp multiplies at once
 
 template <typename T>
 struct Num;
@@ -61,19 +68,6 @@ struct Num<__nv_bfloat16> {
     }
 };
 
-// Global -> shared, 16 bytes, of which the first `valid` are read and the rest zeroed.
-// Weights are read once: past L1.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int valid) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
@@ -84,23 +78,56 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
     return v;
 }
-__device__ __forceinline__ void sts128(uint32_t a, const uint4& v) {
-    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
 __device__ __forceinline__ void sts32(uint32_t a, uint32_t v) {
     asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
+__device__ __forceinline__ void sts8(uint32_t a, uint32_t v) {
+    asm volatile("st.shared.u8 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+// mbar_wait for a whole warp, with one answer for its lanes.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity));
+}
+// L2 policy for weights that another item reads again.
+__device__ __forceinline__ uint64_t l2_normal_policy() {
+    uint64_t pol;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(pol));
+    return pol;
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
 
-// A row-major weight matrix as the copies see it.
+// A tensor of row-major matrices of one shape as the copies see it: the codes or values,
+// and for MXFP4 the scales.
 struct WeightView {
-    int64_t pitch;   // bytes from row to row
-    int row_bytes;   // bytes of one row
-    int blocks;      // MXFP4: scale bytes of one row
-    int steps;       // kStepBytes pieces of one row, the last one filled up with zeros
-    bool aligned;    // 16-byte rows (16-bit matrices) / 4-byte rows of scales (MXFP4)
+    const unsigned char* begin[2];  // of the whole tensor: values or codes, scales
+    const unsigned char* end[2];
+    int pitch[2];                   // bytes of a row: values or codes, scales
+    int cols;
+    int units;                      // kUnitBytes pieces of a row, the last one ragged
+    bool shifted;                   // rows (16-bit) or rows of scales (MXFP4) not on 16 bytes
 };
 
-// A token's row as B pieces: `cols` values, `aligned` when every piece is 16 aligned bytes.
+template <bool MX>
+__host__ __device__ __forceinline__ WeightView weight_view(const unsigned char* w, const unsigned char* s, int64_t rows,
+                                                           int cols) {
+    WeightView v;
+    const int blocks = int(mx_blocks(cols));
+    v.pitch[0] = MX ? blocks * kMxBlockBytes : cols * 2;
+    v.pitch[1] = blocks;
+    v.begin[0] = w;
+    v.begin[1] = s;
+    v.end[0] = w + rows * v.pitch[0];
+    v.end[1] = s + (MX ? rows * blocks : 0);
+    v.cols = cols;
+    v.units = (v.pitch[0] + kUnitBytes - 1) / kUnitBytes;
+    const uintptr_t start = reinterpret_cast<uintptr_t>(MX ? s : w);
+    v.shifted = ((start | uintptr_t(v.pitch[MX ? 1 : 0])) & 15) != 0;
+    return v;
+}
+
+// Eight values of a token's row from k on, zero beyond `cols`; `aligned`: 16-byte pieces.
 template <typename T>
 __device__ __forceinline__ uint4 load_piece(const T* row, int k, int cols, bool aligned) {
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -117,224 +144,357 @@ __device__ __forceinline__ uint4 load_piece(const T* row, int k, int cols, bool 
     return v;
 }
 
-// One warp's piece of work: NM tiles of 16 rows (`rows` of them exist), steps [s0, s1),
-// `count` tokens whose rows each lane's `x` names.
-template <typename T, int NM, int NT>
-struct Piece {
-    const unsigned char* w[NM];  // first byte of the tile's first row
-    const unsigned char* s[NM];  // MXFP4: its first scale byte
+// One item's weights: NM tiles, each the first row's index in its tensor and how many
+// of its 16 rows exist.
+template <int NM>
+struct Tiles {
+    int64_t row[NM];
     int rows[NM];
-    int s0, s1;
-    int count;
-    const T* x[NT];
 };
 
-template <typename T, bool MX, int NM, int NT, int STAGES>
-struct WarpStream {
-    static constexpr int kTileBytes = kTileRows * kStepBytes;
-    static constexpr int kScaleBytes = MX ? kTileRows * 4 : 0;
-    static constexpr int kStage = NM * (kTileBytes + kScaleBytes);
-    static constexpr int kRing = kStage * STAGES;
-    static constexpr int kSub = MX ? 4 : 1;  // groups of 32 values in a step
-
-    // Where in the ring lane 4g + q's 16 bytes of half a tile go. MXFP4: a quad's lanes
-    // read each other's pieces a word at a time; the rotation keeps those reads free of
-    // bank conflicts.
-    static __device__ __forceinline__ uint32_t slot(int g, int q) {
-        return uint32_t(g * 4 + (MX ? ((q + (g >> 1)) & 3) : q)) * 16u;
-    }
-
-    static __device__ __forceinline__ void fetch(const Piece<T, NM, NT>& p, int step, uint32_t stage,
-                                                 const WeightView& v, int lane) {
-        const int g = lane >> 2, q = lane & 3;
-        const int off = step * kStepBytes + q * 16;
-        const int left = min(16, v.row_bytes - off);
-#pragma unroll
-        for (int m = 0; m < NM; ++m) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int row = g + 8 * half;
-                const int valid = row < p.rows[m] ? max(left, 0) : 0;
-                const unsigned char* src = valid > 0 ? p.w[m] + row * v.pitch + off : p.w[m];
-                const uint32_t dst = stage + m * kTileBytes + half * (kTileBytes / 2) + slot(g, q);
-                if (MX || v.aligned) {
-                    copy16(dst, src, valid);
-                } else {
-                    const unsigned short* r = reinterpret_cast<const unsigned short*>(src);
-                    uint32_t e[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) e[i] = 2 * i < valid ? r[i] : 0u;
-                    sts128(dst, make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16),
-                                           e[6] | (e[7] << 16)));
-                }
-            }
-            if (MX && lane < kTileRows) {
-                const int b0 = step * 4;
-                const bool have = lane < p.rows[m];
-                const unsigned char* src = have ? p.s[m] + int64_t(lane) * v.blocks + b0 : p.s[m];
-                const uint32_t dst = stage + NM * kTileBytes + (m * kTileRows + lane) * 4;
-                if (v.aligned) {
-                    copy4(dst, src, have ? 4 : 0);
-                } else {
-                    uint32_t w = 0u;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (have && b0 + i < v.blocks) w |= uint32_t(src[i]) << (8 * i);
-                    sts32(dst, w);
-                }
-            }
-        }
-    }
-
-    static __device__ __forceinline__ void load_tokens(const Piece<T, NM, NT>& p, int sub, int cols, bool aligned,
-                                                       int lane, uint4 (&x)[NT]) {
-        const int k = sub * 32 + (lane & 3) * 8;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-            if (n * 8 < p.count) x[n] = load_piece<T>(p.x[n], k, cols, aligned);
-    }
-
-    static __device__ __forceinline__ void multiply(float (&acc)[NM][NT][4], const uint4 (&x)[NT], uint32_t stage,
-                                                    int sub, int count, int lane) {
-        const int g = lane >> 2, q = lane & 3;
-        if constexpr (!MX) {
-#pragma unroll
-            for (int m = 0; m < NM; ++m) {
-                const uint4 lo = lds128(stage + m * kTileBytes + slot(g, q));
-                const uint4 hi = lds128(stage + m * kTileBytes + kTileBytes / 2 + slot(g, q));
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    if (n * 8 >= count) break;
-                    Num<T>::mma(acc[m][n], lo.x, hi.x, lo.y, hi.y, x[n].x, x[n].y);
-                    Num<T>::mma(acc[m][n], lo.z, hi.z, lo.w, hi.w, x[n].z, x[n].w);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int m = 0; m < NM; ++m) {
-                const uint32_t at = stage + m * kTileBytes + slot(g, sub) + q * 4;
-                uint32_t lo[4], hi[4];
-                Num<T>::decode(lds32(at), lo);
-                Num<T>::decode(lds32(at + kTileBytes / 2), hi);
-                const uint32_t sc = stage + NM * kTileBytes + (m * kTileRows + g) * 4;
-                const float sl = mx_scale((lds32(sc) >> (8 * sub)) & 255u);
-                const float sh = mx_scale((lds32(sc + 32) >> (8 * sub)) & 255u);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    if (n * 8 >= count) break;
-                    const uint4 b = Num<T>::order(x[n]);
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    Num<T>::mma(c, lo[0], hi[0], lo[1], hi[1], b.x, b.y);
-                    Num<T>::mma(c, lo[2], hi[2], lo[3], hi[3], b.z, b.w);
-                    acc[m][n][0] = fmaf(c[0], sl, acc[m][n][0]);
-                    acc[m][n][1] = fmaf(c[1], sl, acc[m][n][1]);
-                    acc[m][n][2] = fmaf(c[2], sh, acc[m][n][2]);
-                    acc[m][n][3] = fmaf(c[3], sh, acc[m][n][3]);
-                }
-            }
-        }
-    }
-
-    // Runs pieces 0, 1, ... of a warp: get(i, piece) -> false past the last one;
-    // done(i, piece, acc) after each, in order, with the piece's sums.
-    template <typename Get, typename Done>
-    static __device__ __forceinline__ void run(uint32_t ring, const WeightView& v, int cols, bool x_aligned,
-                                               Get&& get, Done&& done) {
-        const int lane = threadIdx.x & 31;
-        Piece<T, NM, NT> f;
-        int fi = 0;
-        bool more = get(fi, f);
-        int fs = more ? f.s0 : 0;
-        auto feed = [&](int stage) {
-            while (more && fs >= f.s1) {
-                more = get(++fi, f);
-                if (more) fs = f.s0;
-            }
-            if (more) {
-                fetch(f, fs, ring + stage * kStage, v, lane);
-                ++fs;
-            }
-            copy_commit();
-        };
-#pragma unroll 1
-        for (int s = 0; s < STAGES - 1; ++s) feed(s);
-        int stage = 0;
-        Piece<T, NM, NT> p;
-        for (int i = 0; get(i, p); ++i) {
-            float acc[NM][NT][4];
-#pragma unroll
-            for (int m = 0; m < NM; ++m)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[m][n][c] = 0.f;
-            uint4 x[NT];
-            if (p.s0 < p.s1) load_tokens(p, p.s0 * kSub, cols, x_aligned, lane, x);
-#pragma unroll 1
-            for (int s = p.s0; s < p.s1; ++s) {
-                copy_wait<STAGES - 2>();
-                __syncwarp();  // the step's copies by every lane have landed; the stage to refill is read
-                feed(stage == 0 ? STAGES - 1 : stage - 1);
-                const uint32_t at = ring + stage * kStage;
-#pragma unroll
-                for (int b = 0; b < kSub; ++b) {
-                    uint4 now[NT];
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) now[n] = x[n];
-                    if (b + 1 < kSub || s + 1 < p.s1) load_tokens(p, s * kSub + b + 1, cols, x_aligned, lane, x);
-                    multiply(acc, now, at, b, p.count, lane);
-                }
-                stage = stage + 1 == STAGES ? 0 : stage + 1;
-            }
-            done(i, p, acc);
-        }
-        copy_wait<0>();
-        __syncwarp();
-    }
-};
-
-// ------------------------------------------------------------ a CTA's share
-//
-// A CTA takes its items (16-row tiles) in rounds of W, W/2, ..., 1 so that W warps
-// share a round's items evenly, each item's steps split over the W / r warps that
-// share it. Partial sums meet in shared memory: part[warp][tile][token][17 rows].
+constexpr int kConsumers = 8;
+constexpr int kEpilogueThreads = 96;
+constexpr int kStreamThreads = (kConsumers + 4) * 32;  // consumers, producer, epilogue
 constexpr int kPartPitch = 17;
 
-struct Round {
-    int first, items;  // items [first, first + items) of the list
-};
+template <typename T, bool MX, int NT>
+struct Stream {
+    // A stage: 2 tiles of 16 rows by 1 KB, or one tile by 2 KB. Row pitches keep the
+    // consumers' reads free of bank conflicts and leave 16 bytes for a shifted row.
+    template <int NM>
+    struct Shape {
+        static constexpr int kChunk = 2048 / NM;
+        static constexpr int kPitch = kChunk + (MX ? 16 : 64);
+        static constexpr int kScalePitch = kChunk / kMxBlockBytes + 16;
+        static constexpr int kTile = kTileRows * kPitch;
+        static constexpr int kScales = NM * kTile;  // offset of the scales in a stage
+        static constexpr int kBytes = kScales + (MX ? NM * kTileRows * kScalePitch : 0);
+        static constexpr int kUnits = kChunk / kUnitBytes;
+        static constexpr int kPart = NM * NT * 8 * kPartPitch;  // floats of a consumer's partial sums
+    };
+    static constexpr int kStage = (Shape<2>::kBytes > Shape<1>::kBytes ? Shape<2>::kBytes : Shape<1>::kBytes) / 128 * 128 + 128;
+    static constexpr int kPartFloats = kConsumers * Shape<2>::kPart;
+    static constexpr int kParts = NT >= 4 ? 1 : 2;  // buffers of partial sums
+    static constexpr int kSub = MX ? 4 : 1;         // groups of 32 values in a unit
 
-__device__ __forceinline__ int round_count(int items, int warps) {
-    return items / warps + __popc(items & (warps - 1));
-}
+    // Shared memory: ring, partial sums, 16 zero bytes, barriers.
+    struct Layout {
+        uint32_t ring, part, zero, full, empty, part_full, part_empty;
+        int stages;
+    };
+    static constexpr size_t kFixed = size_t(kParts) * kPartFloats * 4 + 16 + 2 * kParts * 8;
+    __host__ __device__ static constexpr size_t bytes(int stages) { return size_t(stages) * (kStage + 16) + kFixed; }
+    // as many stages as fit beside `other` bytes, at most eight
+    __host__ __device__ static constexpr int stages(size_t other) {
+        int n = 8;
+        while (bytes(n) + other > 232448 - 1024) --n;
+        return n;
+    }
 
-__device__ __forceinline__ Round round_at(int i, int items, int warps) {  // warps: a power of two
-    const int full = items / warps;
-    if (i < full) return {i * warps, warps};
-    int first = full * warps, rest = items & (warps - 1), skip = i - full;
-    for (int bit = warps >> 1;; bit >>= 1) {
-        if (rest & bit) {
-            if (skip == 0) return {first, bit};
-            --skip;
-            first += bit;
+    static __device__ __forceinline__ Layout layout(uint32_t base, int stages) {
+        Layout l;
+        l.stages = stages;
+        l.ring = base;
+        l.part = base + stages * kStage;
+        l.zero = l.part + kParts * kPartFloats * 4;
+        l.full = l.zero + 16;
+        l.empty = l.full + stages * 8;
+        l.part_full = l.empty + stages * 8;
+        l.part_empty = l.part_full + kParts * 8;
+        return l;
+    }
+    // One thread; the CTA synchronises afterwards.
+    static __device__ __forceinline__ void init(const Layout& l) {
+        for (int i = 0; i < 4; ++i) sts32(l.zero + 4 * i, 0u);
+        for (int i = 0; i < l.stages; ++i) {
+            mbar_init(l.full + 8 * i, 1);
+            mbar_init(l.empty + 8 * i, kConsumers);
+        }
+        for (int i = 0; i < kParts; ++i) {
+            mbar_init(l.part_full + 8 * i, kConsumers);
+            mbar_init(l.part_empty + 8 * i, kEpilogueThreads / 32);
+        }
+        mbar_fence_init();
+    }
+
+    // Where a role stands in the ring and in the buffers of partial sums.
+    struct Place {
+        int stage = 0, part = 0;
+        uint32_t phase = 0, part_phase = 0;
+        int64_t issued = 0;
+        bool ok = true;
+        __device__ __forceinline__ void next_stage(int stages) {
+            if (++stage == stages) stage = 0, phase ^= 1u;
+        }
+        __device__ __forceinline__ void next_part() {
+            if (++part == kParts) part = 0, part_phase ^= 1u;
+        }
+    };
+
+    // Copies [from, from + bytes) of a tensor to dst, from the 16 bytes before `from` on;
+    // returns the bytes that complete on the barrier. Where that would leave the tensor, the
+    // lane copies them itself.
+    static __device__ __forceinline__ uint32_t copy_shifted(uint32_t dst, const unsigned char* from, int bytes,
+                                                            const unsigned char* begin, const unsigned char* end,
+                                                            uint32_t bar, uint64_t policy) {
+        const unsigned char* lo = from - (reinterpret_cast<uintptr_t>(from) & 15);
+        const int n = (int(from - lo) + bytes + 15) & ~15;
+        if (lo >= begin && lo + n <= end) {
+            mbar_expect_tx(bar, n);
+            bulk_copy_g2s(dst, lo, n, bar, policy);
+            return n;
+        }
+        const int at = int(from - lo);
+        for (int i = 0; i < bytes; ++i) sts8(dst + at + i, from[i]);
+        fence_proxy_async_smem();  // before a later bulk copy to the same place
+        return 0;
+    }
+
+    // Producer warp: the stages of one item. The copies are the only accesses to the weights.
+    template <int NM>
+    static __device__ __forceinline__ void produce(const Layout& l, Place& p, const Tiles<NM>& t,
+                                                   const WeightView (&v)[NM], uint64_t policy) {
+        using S = Shape<NM>;
+        const int lane = threadIdx.x & 31;
+        const int m = lane / kTileRows, r = lane % kTileRows;
+        const int chunks = (v[0].units + S::kUnits - 1) / S::kUnits;
+        const bool mine = NM == 2 ? r < (m ? t.rows[NM - 1] : t.rows[0]) : lane < kTileRows && r < t.rows[0];
+        const bool second = NM == 2 && m;  // this lane copies rows of the second tile
+        const int64_t row = (second ? t.row[NM - 1] : t.row[0]) + r;
+        const unsigned char* wb = second ? v[NM - 1].begin[0] : v[0].begin[0];
+        const unsigned char* we = second ? v[NM - 1].end[0] : v[0].end[0];
+        const unsigned char* sb = second ? v[NM - 1].begin[1] : v[0].begin[1];
+        const unsigned char* se = second ? v[NM - 1].end[1] : v[0].end[1];
+        const unsigned char* w = wb + row * v[0].pitch[0];
+        const unsigned char* s = sb + row * v[0].pitch[1];
+        for (int c = 0; c < chunks && p.ok; ++c) {
+            if (p.issued >= l.stages && !mbar_wait_warp(l.empty + 8 * p.stage, p.phase ^ 1u)) {
+                p.ok = false;
+                break;
+            }
+            const uint32_t bar = l.full + 8 * p.stage, at = l.ring + p.stage * kStage;
+            const int bytes = min(S::kChunk, v[0].pitch[0] - c * S::kChunk);
+            if (mine) {
+                const uint32_t dst = at + (NM == 2 ? m * S::kTile : 0) + r * S::kPitch;
+                if (MX || !v[0].shifted) {
+                    mbar_expect_tx(bar, bytes);
+                    bulk_copy_g2s(dst, w + c * S::kChunk, bytes, bar, policy);
+                } else {
+                    copy_shifted(dst, w + c * S::kChunk, bytes, wb, we, bar, policy);
+                }
+                if (MX) {
+                    const int n = bytes / kMxBlockBytes, off = c * (S::kChunk / kMxBlockBytes);
+                    const uint32_t to = at + S::kScales + (NM == 2 ? m * kTileRows + r : r) * S::kScalePitch;
+                    if (!v[0].shifted) {
+                        mbar_expect_tx(bar, n);
+                        bulk_copy_g2s(to, s + off, n, bar, policy);
+                    } else {
+                        copy_shifted(to, s + off, n, sb, se, bar, policy);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);  // the stage is full once every copy has landed
+            ++p.issued;
+            p.next_stage(l.stages);
         }
     }
-}
 
-template <int NM, int NT>
-__device__ __forceinline__ void store_partial(float* part, const float (&acc)[NM][NT][4], int count, int lane) {
-    const int g = lane >> 2, q = lane & 3;
-#pragma unroll
-    for (int m = 0; m < NM; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            if (n * 8 >= count) break;
-            float* p = part + (m * NT * 8 + n * 8 + 2 * q) * kPartPitch + g;
-            p[0] = acc[m][n][0];
-            p[kPartPitch] = acc[m][n][1];
-            p[8] = acc[m][n][2];
-            p[kPartPitch + 8] = acc[m][n][3];
+    // Producer, at its end: nothing stays in flight into shared memory if it gave up.
+    static __device__ __forceinline__ void drain(const Layout& l, const Place& p) {
+        if (p.ok) return;
+        for (int i = 0; i < l.stages && i < p.issued; ++i) {
+            const int64_t idx = p.issued - 1 - i;
+            mbar_wait(l.full + 8 * uint32_t(idx % l.stages), uint32_t(idx / l.stages) & 1u);
         }
-}
+    }
+
+    template <int NP>
+    static __device__ __forceinline__ void load_tokens(const T* const (&x)[NP], int count, int k, int cols, bool aligned,
+                                                       uint4 (&v)[NP]) {
+#pragma unroll
+        for (int n = 0; n < NP; ++n)
+            if (n % NT * 8 < count) v[n] = load_piece<T>(x[n], k, cols, aligned);
+    }
+
+    // Consumer warp: one item. x: this lane's token row of each group of eight (advanced to its
+    // quad's eight values); with SPLIT, x holds the rows of a second addend after the first NT,
+    // multiplied by the same weights. Leaves the partial sums in the next buffer.
+    template <int NM, bool SPLIT>
+    static __device__ __forceinline__ void consume(const Layout& l, Place& p, const Tiles<NM>& t,
+                                                   const WeightView (&v)[NM], const T* const (&x)[SPLIT ? 2 * NT : NT],
+                                                   int count, int x_cols, bool x_aligned) {
+        using S = Shape<NM>;
+        constexpr int NP = SPLIT ? 2 * NT : NT;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+        float acc[NM][NT][4];
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[m][n][c] = 0.f;
+        // how far rows g and g + 8 are shifted in their stage
+        uint32_t shift[NM][2];
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                shift[m][h] = v[0].shifted ? uint32_t(reinterpret_cast<uintptr_t>(v[m].begin[MX ? 1 : 0]) +
+                                                      (t.row[m] + g + 8 * h) * v[m].pitch[MX ? 1 : 0]) & 15u
+                                           : 0u;
+        const int chunks = (v[0].units + S::kUnits - 1) / S::kUnits;
+        for (int c = 0; c < chunks && p.ok; ++c) {
+            const int units = min(S::kUnits, v[0].units - c * S::kUnits);
+            uint4 xv[NP];
+            int k = (c * S::kUnits + warp) * (32 * kSub) + q * 8;
+            if (warp < units) load_tokens(x, count, k, x_cols, x_aligned, xv);
+            if (!mbar_wait_warp(l.full + 8 * p.stage, p.phase)) {
+                p.ok = false;
+                break;
+            }
+            const uint32_t at = l.ring + p.stage * kStage;
+#pragma unroll 1
+            for (int u = warp; u < units; u += kConsumers) {
+                if constexpr (MX) {
+                    uint32_t sc[NM][2];
+#pragma unroll
+                    for (int m = 0; m < NM; ++m)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t a = at + S::kScales + (m * kTileRows + g + 8 * h) * S::kScalePitch + u * 4;
+                            if (!v[0].shifted) {
+                                sc[m][h] = lds32(a);
+                            } else {
+                                const uint32_t b = a + shift[m][h];
+                                sc[m][h] = __funnelshift_r(lds32(b & ~3u), lds32((b & ~3u) + 4), (b & 3u) * 8);
+                            }
+                        }
+                    const int subs = min(kSub, v[0].pitch[1] - (c * S::kUnits + u) * kSub);
+#pragma unroll
+                    for (int b = 0; b < kSub; ++b) {
+                        if (b >= subs) break;
+                        uint4 now[NP];
+#pragma unroll
+                        for (int n = 0; n < NP; ++n) now[n] = Num<T>::order(xv[n]);
+                        if (b + 1 < subs)
+                            load_tokens(x, count, k + 32 * (b + 1), x_cols, x_aligned, xv);
+                        else if (u + kConsumers < units)
+                            load_tokens(x, count, k + 32 * kSub * kConsumers, x_cols, x_aligned, xv);
+#pragma unroll
+                        for (int m = 0; m < NM; ++m) {
+                            const uint32_t a = at + m * S::kTile + g * S::kPitch + u * kUnitBytes + b * 16 + q * 4;
+                            uint32_t lo[4], hi[4];
+                            Num<T>::decode(lds32(a), lo);
+                            Num<T>::decode(lds32(a + 8 * S::kPitch), hi);
+                            const float sl = mx_scale((sc[m][0] >> (8 * b)) & 255u);
+                            const float sh = mx_scale((sc[m][1] >> (8 * b)) & 255u);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                if (n * 8 >= count) break;
+                                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                                Num<T>::mma(d, lo[0], hi[0], lo[1], hi[1], now[n].x, now[n].y);
+                                Num<T>::mma(d, lo[2], hi[2], lo[3], hi[3], now[n].z, now[n].w);
+                                if (SPLIT) {
+                                    Num<T>::mma(d, lo[0], hi[0], lo[1], hi[1], now[NP - NT + n].x, now[NP - NT + n].y);
+                                    Num<T>::mma(d, lo[2], hi[2], lo[3], hi[3], now[NP - NT + n].z, now[NP - NT + n].w);
+                                }
+                                acc[m][n][0] = fmaf(d[0], sl, acc[m][n][0]);
+                                acc[m][n][1] = fmaf(d[1], sl, acc[m][n][1]);
+                                acc[m][n][2] = fmaf(d[2], sh, acc[m][n][2]);
+                                acc[m][n][3] = fmaf(d[3], sh, acc[m][n][3]);
+                            }
+                        }
+                    }
+                } else {
+                    uint4 now[NP];
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) now[n] = xv[n];
+                    if (u + kConsumers < units)
+                        load_tokens(x, count, k + 32 * kConsumers, x_cols, x_aligned, xv);
+                    const int left = v[0].cols - k;  // values of this lane's pieces that the row has
+#pragma unroll
+                    for (int m = 0; m < NM; ++m) {
+                        uint4 a[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t o = at + m * S::kTile + (g + 8 * h) * S::kPitch + u * kUnitBytes + q * 16;
+                            if (!v[0].shifted) {
+                                a[h] = lds128(left > 0 ? o : l.zero);
+                            } else {
+                                const uint32_t b = o + shift[m][h], s = (b & 2u) * 8;
+                                uint32_t w[5];
+#pragma unroll
+                                for (int i = 0; i < 5; ++i) w[i] = lds32((b & ~3u) + 4 * i);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    w[i] = __funnelshift_r(w[i], w[i + 1], s);
+                                    if (2 * i + 1 >= left) w[i] = 2 * i >= left ? 0u : w[i] & 0xFFFFu;
+                                }
+                                a[h] = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            if (n * 8 >= count) break;
+                            Num<T>::mma(acc[m][n], a[0].x, a[1].x, a[0].y, a[1].y, now[n].x, now[n].y);
+                            Num<T>::mma(acc[m][n], a[0].z, a[1].z, a[0].w, a[1].w, now[n].z, now[n].w);
+                            if (SPLIT) {
+                                Num<T>::mma(acc[m][n], a[0].x, a[1].x, a[0].y, a[1].y, now[NP - NT + n].x, now[NP - NT + n].y);
+                                Num<T>::mma(acc[m][n], a[0].z, a[1].z, a[0].w, a[1].w, now[NP - NT + n].z, now[NP - NT + n].w);
+                            }
+                        }
+                    }
+                }
+                k += 32 * kSub * kConsumers;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(l.empty + 8 * p.stage);
+            p.next_stage(l.stages);
+        }
+        if (!p.ok) return;
+        // the buffer's last sums are read
+        if (p.issued >= kParts && !mbar_wait_warp(l.part_empty + 8 * p.part, p.part_phase ^ 1u)) {
+            p.ok = false;
+            return;
+        }
+        const uint32_t part = l.part + (p.part * kPartFloats + warp * S::kPart) * 4;
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                if (n * 8 >= count) break;
+                const uint32_t a = part + ((m * NT * 8 + n * 8 + 2 * q) * kPartPitch + g) * 4;
+                sts32(a, __float_as_uint(acc[m][n][0]));
+                sts32(a + kPartPitch * 4, __float_as_uint(acc[m][n][1]));
+                sts32(a + 32, __float_as_uint(acc[m][n][2]));
+                sts32(a + (kPartPitch + 8) * 4, __float_as_uint(acc[m][n][3]));
+            }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(l.part_full + 8 * p.part);
+        p.issued++;
+        p.next_part();
+    }
+
+    // Epilogue threads: waits for an item's partial sums; sum(tile, token, row) adds them up;
+    // release() frees the buffer.
+    static __device__ __forceinline__ bool acquire(const Layout& l, Place& p) {
+        if (!mbar_wait_warp(l.part_full + 8 * p.part, p.part_phase)) p.ok = false;
+        return p.ok;
+    }
+    template <int NM>
+    static __device__ __forceinline__ float sum(const Layout& l, const Place& p, int m, int token, int row) {
+        const uint32_t a = l.part + (p.part * kPartFloats + (m * NT * 8 + token) * kPartPitch + row) * 4;
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kConsumers; ++w) s += __uint_as_float(lds32(a + w * Shape<NM>::kPart * 4));
+        return s;
+    }
+    static __device__ __forceinline__ void release(const Layout& l, Place& p) {
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(l.part_empty + 8 * p.part);
+        p.next_part();
+    }
+};
 
 }  // namespace swb

@@ -875,10 +875,12 @@ int swb_device_error(int clear, int* out) {
         e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof zero);
         if (e != cudaSuccess) return fail(SWB_E_CUDA, cudaGetErrorString(e));
     }
-    int moe = 0, matmul = 0;  // the other translation units' words
-    if (int rc = moe_device_error(clear, &moe)) return rc;
-    if (int rc = mx4_matmul_device_error(clear, &matmul)) return rc;
-    if (out) *out = v | moe | matmul;
+    for (auto other : {moe_device_error, mx4_device_error, mx4_matmul_device_error}) {
+        int more = 0;
+        if (int rc = other(clear, &more)) return rc;
+        v |= more;
+    }
+    if (out) *out = v;
     return SWB_OK;
 }
 
