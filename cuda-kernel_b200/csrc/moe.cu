@@ -28,7 +28,7 @@ static_assert(SWB_MOE_MAX_TOKENS == kMoeMaxTokens && SWB_MOE_MAX_EXPERTS == kMoe
 static_assert(1 + (kMoeMaxTokens + kRouteTokens - 1) / kRouteTokens <= 64, "sync words fit before the logits");
 
 template <typename T, bool MX, int NT>
-int launch_moe(const MoeParams& P, cudaStream_t stream) {
+int launch_moe(MoeParams P, cudaStream_t stream) {
     using S = MoeShape<T, MX, NT>;
     static std::atomic<uint64_t> smem_set{0};
     const int sms = sm_count();
@@ -36,8 +36,21 @@ int launch_moe(const MoeParams& P, cudaStream_t stream) {
     auto kernel = moe_kernel<T, MX, NT>;
     if (int rc = allow_smem(kernel, smem_set, S::kSmem)) return rc;
     static_assert(S::kStages >= 3, "a ring");
+    MoeMaps maps;
+    bool fast[3], deep[3];
+    for (int i = 0; i < 3; ++i) {
+        const int64_t rows = int64_t(P.experts) * (i < 2 ? P.inter : P.hidden), cols = i < 2 ? P.hidden : P.inter;
+        const int64_t blocks = mx_blocks(cols), pitch = MX ? blocks * kMxBlockBytes : cols * 2;
+        if (int rc = make_weight_maps(&maps.m[i], P.w[i], MX ? P.s[i] : nullptr, rows, pitch, blocks, &fast[i], &deep[i]))
+            return rc;
+    }
+    // one way of reading for the copies and the consumers of a phase
+    P.fast[0] = fast[0] && fast[1] && P.x_aligned;
+    P.fast[1] = fast[2];
+    P.deep[0] = deep[0];
+    P.deep[1] = deep[2];
     // every CTA resident at once: the cooperative launch makes the runtime check it
-    return launch_ex(kernel, unsigned(sms), kStreamThreads, S::kSmem, stream, true, P);
+    return launch_ex(kernel, unsigned(sms), kStreamThreads, S::kSmem, stream, true, maps, P);
 }
 
 template <typename T, bool MX>

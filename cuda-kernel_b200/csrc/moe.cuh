@@ -35,6 +35,10 @@ constexpr int kMoeMaxGroups = kMoeMaxExperts + kMoeMaxTokens * kMoeMaxTopk / kMo
 constexpr int kRouteExperts = 4, kRouteTokens = 4;  // of a router unit
 constexpr int kRouteThreads = kConsumers * 32;
 
+struct MoeMaps {
+    WeightMaps m[3];  // gate, up, down
+};
+
 struct MoeParams {
     const void* x;
     const void* router;
@@ -52,6 +56,7 @@ struct MoeParams {
     int tokens, hidden, inter, experts, topk, h_pitch;
     int renormalize;
     int x_aligned, router_aligned;  // 16-byte pieces of the rows of x, of Wr
+    bool fast[2], deep[2];          // make_weight_maps of gate and up, of down
 };
 
 // Offsets of the workspace's parts.
@@ -191,6 +196,11 @@ __device__ void moe_select(const MoeParams& P, int token, int lane) {
     }
 }
 
+template <typename T>
+__device__ __forceinline__ uint4 route_piece(const T* row, int k, int cols, int aligned) {
+    return aligned ? load_piece<T, true>(row, k, cols) : load_piece<T, false>(row, k, cols);
+}
+
 // The first kRouteThreads threads of the CTA.
 template <typename T>
 __device__ void moe_router(const MoeParams& P, double* scratch, int* flag) {
@@ -211,10 +221,10 @@ __device__ void moe_router(const MoeParams& P, double* scratch, int* flag) {
             uint4 wv[kRouteExperts], xv[kRouteTokens];
 #pragma unroll
             for (int a = 0; a < kRouteExperts; ++a)
-                wv[a] = load_piece<T>(r + size_t(min(e0 + a, P.experts - 1)) * P.hidden, k, P.hidden, P.router_aligned);
+                wv[a] = route_piece(r + size_t(min(e0 + a, P.experts - 1)) * P.hidden, k, P.hidden, P.router_aligned);
 #pragma unroll
             for (int b = 0; b < kRouteTokens; ++b)
-                xv[b] = load_piece<T>(x + (t0 + min(b, nt - 1)) * P.x_pitch, k, P.hidden, P.x_aligned);
+                xv[b] = route_piece(x + (t0 + min(b, nt - 1)) * P.x_pitch, k, P.hidden, P.x_aligned);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {  // zero beyond the row
                 double wd[kRouteExperts];
@@ -319,10 +329,11 @@ __device__ inline void moe_lists(const MoeParams& P, MoeRoute& R) {
 }
 
 template <typename T, bool MX, int NT>
-__global__ void __launch_bounds__(kStreamThreads, 1) moe_kernel(const MoeParams P) {
+__global__ void __launch_bounds__(kStreamThreads, 1)
+    moe_kernel(const __grid_constant__ MoeMaps maps, const MoeParams P) {
     using S = MoeShape<T, MX, NT>;
     using Pipe = typename S::Pipe;
-    extern __shared__ __align__(128) unsigned char smem[];
+    extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ double scratch[kRouteExperts * kRouteTokens * kConsumers];
     __shared__ int flag, sums_ok;
     MoeRoute& R = *reinterpret_cast<MoeRoute*>(smem + S::kRoute);
@@ -346,10 +357,12 @@ __global__ void __launch_bounds__(kStreamThreads, 1) moe_kernel(const MoeParams 
         group = f + j % k;
         row = j / k * kTileRows;
     };
-    WeightView gv[2] = {weight_view<MX>(P.w[0], P.s[0], int64_t(P.experts) * P.inter, P.hidden),
-                        weight_view<MX>(P.w[1], P.s[1], int64_t(P.experts) * P.inter, P.hidden)};
-    gv[0].shifted = gv[1].shifted = gv[0].shifted || gv[1].shifted;
-    const WeightView dv[1] = {weight_view<MX>(P.w[2], P.s[2], int64_t(P.experts) * P.hidden, P.inter)};
+    const WeightMaps* gm = P.fast[0] ? &maps.m[0] : nullptr;
+    const WeightView gv[2] = {
+        weight_view<MX>(P.w[0], P.s[0], int64_t(P.experts) * P.inter, P.hidden, gm, P.deep[0]),
+        weight_view<MX>(P.w[1], P.s[1], int64_t(P.experts) * P.inter, P.hidden, gm ? &maps.m[1] : nullptr, P.deep[0])};
+    const WeightView dv[1] = {weight_view<MX>(P.w[2], P.s[2], int64_t(P.experts) * P.hidden, P.inter,
+                                              P.fast[1] ? &maps.m[2] : nullptr, P.deep[1])};
     auto gate_rows = [&](int group, int row) {
         Tiles<2> t;
         t.row[0] = t.row[1] = int64_t(R.expert[group]) * P.inter + row;
@@ -387,7 +400,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1) moe_kernel(const MoeParams 
 #pragma unroll
             for (int n = 0; n < NT; ++n)
                 xg[n] = static_cast<const T*>(P.x) + R.token[start + min(n * 8 + (lane >> 2), count - 1)] * P.x_pitch;
-            Pipe::template consume<2, false>(l, place, gate_rows(group, row), gv, xg, count, P.hidden, P.x_aligned != 0);
+            if (gv[0].maps)
+                Pipe::template consume<2, false, true>(l, place, gate_rows(group, row), gv, xg, count, P.hidden);
+            else
+                Pipe::template consume<2, false, false>(l, place, gate_rows(group, row), gv, xg, count, P.hidden);
         }
         named_barrier_sync(2, kStreamThreads - 32);  // h is complete, or flag says that it will not be
         for (int d = d0; d < d1 && flag; ++d)
@@ -398,7 +414,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1) moe_kernel(const MoeParams 
                     x[n] = h + int64_t(start + min(n * 8 + (lane >> 2), count - 1)) * P.h_pitch;
                     x[NT + n] = x[n] + h_plane;
                 }
-                Pipe::template consume<1, true>(l, place, down_rows(a, d), dv, x, count, P.h_pitch, true);
+                if (dv[0].maps)
+                    Pipe::template consume<1, true, true>(l, place, down_rows(a, d), dv, x, count, P.h_pitch);
+                else
+                    Pipe::template consume<1, true, false>(l, place, down_rows(a, d), dv, x, count, P.h_pitch);
             }
     } else {
         const int thread = threadIdx.x - (kConsumers + 1) * 32;

@@ -249,8 +249,8 @@ struct ProjectParams {
     int rows, cols;
     int tiles;       // of 32 rows
     int64_t items;   // tiles x groups of NT * 8 tokens
-    int x_aligned;
-    int half_out;
+    bool x_aligned, fast, deep;  // 16-byte pieces of x; make_weight_maps
+    bool half_out;
 };
 
 template <typename T, int NT>
@@ -261,10 +261,11 @@ struct ProjectShape {
 };
 
 template <typename T, int NT>
-__global__ void __launch_bounds__(kStreamThreads, 1) project_kernel(const ProjectParams P) {
+__global__ void __launch_bounds__(kStreamThreads, 1)
+    project_kernel(const __grid_constant__ WeightMaps maps, const ProjectParams P) {
     using Shape = ProjectShape<T, NT>;
     using Pipe = typename Shape::Pipe;
-    extern __shared__ __align__(128) unsigned char smem[];
+    extern __shared__ __align__(1024) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const auto l = Pipe::layout(smem_u32(smem), Shape::kStages);
     if (threadIdx.x == 0) Pipe::init(l);
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) project_kernel(const Projec
 
     const int64_t first = int64_t(blockIdx.x) * P.items / gridDim.x;
     const int64_t last = int64_t(blockIdx.x + 1) * P.items / gridDim.x;
-    const WeightView one = weight_view<true>(P.w, P.s, P.rows, P.cols);
+    const WeightView one = weight_view<true>(P.w, P.s, P.rows, P.cols, P.fast ? &maps : nullptr, P.deep);
     const WeightView v[2] = {one, one};
     typename Pipe::Place place;
     auto tiles = [&](int64_t item) {
@@ -295,7 +296,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1) project_kernel(const Projec
 #pragma unroll
             for (int n = 0; n < NT; ++n)
                 x[n] = static_cast<const T*>(P.x) + (t0 + min(n * 8 + (lane >> 2), count - 1)) * P.x_pitch;
-            Pipe::template consume<2, false>(l, place, tiles(i), v, x, count, P.cols, P.x_aligned != 0);
+            if (P.x_aligned && P.fast)
+                Pipe::template consume<2, false, true>(l, place, tiles(i), v, x, count, P.cols);
+            else
+                Pipe::template consume<2, false, false>(l, place, tiles(i), v, x, count, P.cols);
         }
     } else {
         const int thread = threadIdx.x - (kConsumers + 1) * 32;
@@ -328,10 +332,15 @@ int launch_project(ProjectParams P, cudaStream_t stream) {
     auto kernel = project_kernel<T, NT>;
     static_assert(Shape::kStages >= 3, "a ring");
     if (int rc = allow_smem(kernel, smem_set, Shape::kSmem)) return rc;
+    WeightMaps maps;
+    const int64_t blocks = mx_blocks(P.cols);
+    if (int rc = make_weight_maps(&maps, P.w, P.s, P.rows, blocks * kMxBlockBytes, blocks, &P.fast, &P.deep)) return rc;
+    // one way of reading for the copies and the consumers
+    P.fast = P.fast && P.x_aligned;
     P.tiles = (P.rows + 31) / 32;
     P.items = int64_t(P.tiles) * ((P.tokens + NT * 8 - 1) / (NT * 8));
     const unsigned grid = unsigned(std::min<int64_t>(P.items, sms));
-    return launch_ex(kernel, grid, kStreamThreads, Shape::kSmem, stream, false, P);
+    return launch_ex(kernel, grid, kStreamThreads, Shape::kSmem, stream, false, maps, P);
 }
 
 template <typename T>

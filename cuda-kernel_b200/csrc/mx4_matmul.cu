@@ -17,14 +17,13 @@
 // Few tokens (W on the M side, N = 16 to 128 tokens): bound by the bytes of W. The
 // CTAs of a cluster split K, so that every SM streams, and add their parts through
 // each other's shared memory in a fixed order.
-#include <cuda.h>
-
 #include <algorithm>
 #include <cstring>
 
 #include "device.cuh"
 #include "host.h"
 #include "stream.cuh"
+#include "tensor_map.h"
 
 namespace swb {
 
@@ -64,12 +63,7 @@ struct MatmulParams {
     int splits;               // CTAs of a cluster that share a tile's K
 };
 
-// ------------------------------------------------------------ tcgen05 and TMA
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
-}
+// ------------------------------------------------------------ tcgen05
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t columns) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(columns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -227,8 +221,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     const uint32_t bar = smem_u32(full + s), at = base + s * S::kStage;
                     mbar_arrive_expect_tx(bar, S::kBytesA + S::kBytesB);
-                    tma_load_2d(at, &map_a, k * kRowBytes, a * S::kRowsA, bar);
-                    tma_load_2d(at + S::kBytesA, &map_b, k * kRowBytes, b * N, bar);
+                    tma_load_2d(at, &map_a, k * (kRowBytes / 4), a * S::kRowsA, bar);
+                    tma_load_2d(at + S::kBytesA, &map_b, k * (kRowBytes / 4), b * N, bar);
                     ++issued;
                     if (++s == S::kStages) s = 0, ph ^= 1u;
                 }
@@ -471,36 +465,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------ host
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encode_tiled() {
-    static const EncodeTiled fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess) {
-            (void)cudaGetLastError();
-            p = nullptr;
-        }
-        return reinterpret_cast<EncodeTiled>(p);
-    }();
-    return fn;
-}
-
-int make_map(CUtensorMap* map, const void* codes, int64_t rows, int64_t blocks, int box_rows) {
-    const EncodeTiled encode = encode_tiled();
-    if (!encode) return fail(SWB_E_UNSUPPORTED, "the driver has no tensor maps");
-    const cuuint64_t dims[2] = {cuuint64_t(blocks * kMxBlockBytes), cuuint64_t(rows)};
-    const cuuint64_t strides[1] = {cuuint64_t(blocks * kMxBlockBytes)};
-    const cuuint32_t box[2] = {cuuint32_t(kRowBytes), cuuint32_t(box_rows)}, one[2] = {1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, one,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? SWB_OK : fail(SWB_E_CUDA, "tensor map");
-}
-
 struct Side {
     const void* codes;
     const unsigned char* scales;
@@ -518,8 +482,8 @@ int launch_matmul(const Side& x, const Side& w, MatmulParams P, cudaStream_t str
     const Side& a = TOKENS_M ? x : w;
     const Side& b = TOKENS_M ? w : x;
     CUtensorMap map_a, map_b;
-    if (int rc = make_map(&map_a, a.codes, a.rows, P.blocks, S::kRowsA)) return rc;
-    if (int rc = make_map(&map_b, b.codes, b.rows, P.blocks, N)) return rc;
+    if (int rc = make_map(&map_a, a.codes, a.rows, int64_t(P.blocks) * kMxBlockBytes, kRowBytes, S::kRowsA)) return rc;
+    if (int rc = make_map(&map_b, b.codes, b.rows, int64_t(P.blocks) * kMxBlockBytes, kRowBytes, N)) return rc;
     P.sa = a.scales;
     P.sb = b.scales;
     P.rows_a = a.rows;

@@ -5,8 +5,8 @@
 // to NT * 8 tokens over the whole row. Few-token products are bound by the bytes of the
 // weights, so the CTA is a pipeline that never drains between items:
 //
-//   producer   one warp; each lane copies its row's next piece (1 or 2 KB, a bulk copy)
-//              into a ring of stages, running ahead across items as far as the ring goes
+//   producer   one thread brings the tiles' next 1 or 2 KB of each row, by TMA, into a ring
+//              of stages, running ahead across items as far as the ring goes
 //   consumers  kWarps warps share each stage by columns; weights are the m16n8k16 A operand,
 //              eight tokens the B operand, sums in fp32. The tokens, a few KB that every item
 //              reads again, come through L1 into registers. (With the weights on the same
@@ -22,11 +22,16 @@
 // roundings are the fp32 sums').
 //
 // Rows that do not start on 16 bytes (16-bit matrices of ragged sizes, scales of ragged
-// rows) are copied from the 16 bytes before and read back shifted. Waits are bounded.
+// rows) have no tensor map: each lane of the producer warp copies a row's piece from the 16
+// bytes before it (a bulk copy each, about half the rate), and consumers read it shifted.
+// Waits are bounded.
 #pragma once
+
+#include <cuda.h>
 
 #include "device.cuh"
 #include "mx4.cuh"
+#include "tensor_map.h"
 
 namespace swb {
 
@@ -41,7 +46,7 @@ struct Num<__half> {
     static __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
     static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                      "{%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -56,7 +61,7 @@ struct Num<__nv_bfloat16> {
     static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
     static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                      "{%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -68,16 +73,13 @@ struct Num<__nv_bfloat16> {
     }
 };
 
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-    return v;
+// Shared loads by 32-bit address, left to the compiler to schedule between barriers.
+__device__ __forceinline__ const void* smem_ptr(uint32_t a) {
+    extern __shared__ __align__(1024) unsigned char smem[];  // keeps the loads in the shared space
+    return smem + (a - smem_u32(smem));
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
-}
+__device__ __forceinline__ uint4 lds128(uint32_t a) { return *static_cast<const uint4*>(smem_ptr(a)); }
+__device__ __forceinline__ uint32_t lds32(uint32_t a) { return *static_cast<const uint32_t*>(smem_ptr(a)); }
 __device__ __forceinline__ void sts32(uint32_t a, uint32_t v) {
     asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
@@ -94,6 +96,24 @@ __device__ __forceinline__ uint64_t l2_normal_policy() {
     asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(pol));
     return pol;
 }
+// TMA tile loads; the barrier counts whole boxes.
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar,
+                                            uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar), "l"(policy) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar,
+                                            uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy) : "memory");
+}
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
@@ -106,12 +126,13 @@ struct WeightView {
     int pitch[2];                   // bytes of a row: values or codes, scales
     int cols;
     int units;                      // kUnitBytes pieces of a row, the last one ragged
-    bool shifted;                   // rows (16-bit) or rows of scales (MXFP4) not on 16 bytes
+    const WeightMaps* maps;         // null: rows (16-bit) or rows of scales (MXFP4) not on 16 bytes
+    bool deep;                      // WeightMaps: boxes of 1 KB of a row
 };
 
 template <bool MX>
-__host__ __device__ __forceinline__ WeightView weight_view(const unsigned char* w, const unsigned char* s, int64_t rows,
-                                                           int cols) {
+__device__ __forceinline__ WeightView weight_view(const unsigned char* w, const unsigned char* s, int64_t rows, int cols,
+                                                  const WeightMaps* maps, bool deep) {
     WeightView v;
     const int blocks = int(mx_blocks(cols));
     v.pitch[0] = MX ? blocks * kMxBlockBytes : cols * 2;
@@ -122,17 +143,17 @@ __host__ __device__ __forceinline__ WeightView weight_view(const unsigned char* 
     v.end[1] = s + (MX ? rows * blocks : 0);
     v.cols = cols;
     v.units = (v.pitch[0] + kUnitBytes - 1) / kUnitBytes;
-    const uintptr_t start = reinterpret_cast<uintptr_t>(MX ? s : w);
-    v.shifted = ((start | uintptr_t(v.pitch[MX ? 1 : 0])) & 15) != 0;
+    v.maps = maps;
+    v.deep = deep;
     return v;
 }
 
-// Eight values of a token's row from k on, zero beyond `cols`; `aligned`: 16-byte pieces.
-template <typename T>
-__device__ __forceinline__ uint4 load_piece(const T* row, int k, int cols, bool aligned) {
+// Eight values of a token's row from k on, zero beyond `cols`; ALIGNED: 16-byte pieces.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ uint4 load_piece(const T* row, int k, int cols) {
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (k >= cols) return v;
-    if (aligned) return *reinterpret_cast<const uint4*>(row + k);
+    if constexpr (ALIGNED) return *reinterpret_cast<const uint4*>(row + k);
     const unsigned short* r = reinterpret_cast<const unsigned short*>(row);
     uint32_t e[8];
 #pragma unroll
@@ -156,11 +177,13 @@ constexpr int kConsumers = 8;
 constexpr int kEpilogueThreads = 96;
 constexpr int kStreamThreads = (kConsumers + 4) * 32;  // consumers, producer, epilogue
 constexpr int kPartPitch = 17;
+constexpr int kRingTarget = 160 * 1024;
 
 template <typename T, bool MX, int NT>
 struct Stream {
-    // A stage: 2 tiles of 16 rows by 1 KB, or one tile by 2 KB. Row pitches keep the
-    // consumers' reads free of bank conflicts and leave 16 bytes for a shifted row.
+    // A stage: 2 tiles of 16 rows by 1 KB, or one tile by 2 KB. With maps: 128 bytes of 16 rows
+    // after another (kBox), swizzled by the copy; scales 64 bytes of 16 rows after another.
+    // Without: row after row, at pitches that leave 16 bytes for a shifted row.
     template <int NM>
     struct Shape {
         static constexpr int kChunk = 2048 / NM;
@@ -169,25 +192,32 @@ struct Stream {
         static constexpr int kTile = kTileRows * kPitch;
         static constexpr int kScales = NM * kTile;  // offset of the scales in a stage
         static constexpr int kBytes = kScales + (MX ? NM * kTileRows * kScalePitch : 0);
+        static constexpr int kBoxes = kChunk / 128;  // of a tile
         static constexpr int kUnits = kChunk / kUnitBytes;
         static constexpr int kPart = NM * NT * 8 * kPartPitch;  // floats of a consumer's partial sums
     };
-    static constexpr int kStage = (Shape<2>::kBytes > Shape<1>::kBytes ? Shape<2>::kBytes : Shape<1>::kBytes) / 128 * 128 + 128;
+    static constexpr int kBox = kTileRows * 128, kScaleBox = kTileRows * 64;
+    static constexpr int kBoxScales = 32 * 1024;  // offset of the scales in a stage
+    static constexpr int kStage = (Shape<2>::kBytes > Shape<1>::kBytes ? Shape<2>::kBytes : Shape<1>::kBytes) / 1024 * 1024 + 1024;
+    static_assert(kStage >= kBoxScales + (MX ? 2 * kScaleBox : 0), "a stage holds either layout");
+    // The tile's row that is row g of the A operand. 16-bit: eight lanes read 16 bytes of two
+    // operand rows at a time; rows four apart have their halves of 128 swizzled bytes apart.
+    static __device__ __forceinline__ int tile_row(int g) { return MX ? g : ((g & 1) << 2) | (g >> 1); }
     static constexpr int kPartFloats = kConsumers * Shape<2>::kPart;
     static constexpr int kParts = NT >= 4 ? 1 : 2;  // buffers of partial sums
     static constexpr int kSub = MX ? 4 : 1;         // groups of 32 values in a unit
 
-    // Shared memory: ring, partial sums, 16 zero bytes, barriers.
+    // Shared memory: ring (on 1 KB), partial sums, barriers.
     struct Layout {
-        uint32_t ring, part, zero, full, empty, part_full, part_empty;
+        uint32_t ring, part, full, empty, part_full, part_empty;
         int stages;
     };
-    static constexpr size_t kFixed = size_t(kParts) * kPartFloats * 4 + 16 + 2 * kParts * 8;
+    static constexpr size_t kFixed = size_t(kParts) * kPartFloats * 4 + 2 * kParts * 8;
     __host__ __device__ static constexpr size_t bytes(int stages) { return size_t(stages) * (kStage + 16) + kFixed; }
-    // as many stages as fit beside `other` bytes, at most eight
+    // as many stages as fit beside `other` bytes and the ring's share (L1 has the rest)
     __host__ __device__ static constexpr int stages(size_t other) {
         int n = 8;
-        while (bytes(n) + other > 232448 - 1024) --n;
+        while (bytes(n) + other > 232448 - 1024 || n * kStage > kRingTarget) --n;
         return n;
     }
 
@@ -196,8 +226,7 @@ struct Stream {
         l.stages = stages;
         l.ring = base;
         l.part = base + stages * kStage;
-        l.zero = l.part + kParts * kPartFloats * 4;
-        l.full = l.zero + 16;
+        l.full = l.part + kParts * kPartFloats * 4;
         l.empty = l.full + stages * 8;
         l.part_full = l.empty + stages * 8;
         l.part_empty = l.part_full + kParts * 8;
@@ -205,7 +234,6 @@ struct Stream {
     }
     // One thread; the CTA synchronises afterwards.
     static __device__ __forceinline__ void init(const Layout& l) {
-        for (int i = 0; i < 4; ++i) sts32(l.zero + 4 * i, 0u);
         for (int i = 0; i < l.stages; ++i) {
             mbar_init(l.full + 8 * i, 1);
             mbar_init(l.empty + 8 * i, kConsumers);
@@ -254,6 +282,46 @@ struct Stream {
     template <int NM>
     static __device__ __forceinline__ void produce(const Layout& l, Place& p, const Tiles<NM>& t,
                                                    const WeightView (&v)[NM], uint64_t policy) {
+        if (!v[0].maps) {
+            produce_rows<NM>(l, p, t, v, policy);
+            return;
+        }
+        using S = Shape<NM>;
+        const bool leader = (threadIdx.x & 31) == 0;  // issues; the others keep its place in the ring
+        const int chunks = (v[0].units + S::kUnits - 1) / S::kUnits;
+        for (int c = 0; c < chunks; ++c) {
+            if (p.issued >= l.stages && !mbar_wait_warp(l.empty + 8 * p.stage, p.phase ^ 1u)) {
+                p.ok = false;
+                break;
+            }
+            const uint32_t bar = l.full + 8 * p.stage, at = l.ring + p.stage * kStage;
+            const int left = v[0].pitch[0] - c * S::kChunk;  // bytes of each row from here on
+            const int boxes = v[0].deep ? (left + 1023) / 1024 * 8 : (left + 127) / 128, n = min(S::kBoxes, boxes);
+            const int scales = MX ? min(S::kChunk / 1024, (left + 1023) / 1024) : 0;
+            if (leader) mbar_arrive_expect_tx(bar, NM * (n * kBox + scales * kScaleBox));
+#pragma unroll
+            for (int m = 0; m < NM && leader; ++m) {
+                const int row = int(t.row[m]);
+                if (v[0].deep) {
+                    for (int i = 0; i < n; i += 8)
+                        tma_load_3d(at + (m * S::kBoxes + i) * kBox, &v[m].maps->w, 0, row, c * S::kBoxes + i, bar, policy);
+                } else {
+                    for (int i = 0; i < n; ++i)
+                        tma_load_2d(at + (m * S::kBoxes + i) * kBox, &v[m].maps->w, (c * S::kChunk + i * 128) / 4, row, bar, policy);
+                }
+                for (int i = 0; i < scales; ++i)
+                    tma_load_2d(at + kBoxScales + (m + i) * kScaleBox, &v[m].maps->s,
+                                (c * (S::kChunk / kMxBlockBytes) + i * 64) / 4, row, bar, policy);
+            }
+            __syncwarp();
+            ++p.issued;
+            p.next_stage(l.stages);
+        }
+    }
+
+    template <int NM>
+    static __device__ __noinline__ void produce_rows(const Layout& l, Place& p, const Tiles<NM>& t,
+                                                     const WeightView (&v)[NM], uint64_t policy) {
         using S = Shape<NM>;
         const int lane = threadIdx.x & 31;
         const int m = lane / kTileRows, r = lane % kTileRows;
@@ -276,7 +344,7 @@ struct Stream {
             const int bytes = min(S::kChunk, v[0].pitch[0] - c * S::kChunk);
             if (mine) {
                 const uint32_t dst = at + (NM == 2 ? m * S::kTile : 0) + r * S::kPitch;
-                if (MX || !v[0].shifted) {
+                if (MX) {  // codes always start on 16 bytes
                     mbar_expect_tx(bar, bytes);
                     bulk_copy_g2s(dst, w + c * S::kChunk, bytes, bar, policy);
                 } else {
@@ -285,12 +353,7 @@ struct Stream {
                 if (MX) {
                     const int n = bytes / kMxBlockBytes, off = c * (S::kChunk / kMxBlockBytes);
                     const uint32_t to = at + S::kScales + (NM == 2 ? m * kTileRows + r : r) * S::kScalePitch;
-                    if (!v[0].shifted) {
-                        mbar_expect_tx(bar, n);
-                        bulk_copy_g2s(to, s + off, n, bar, policy);
-                    } else {
-                        copy_shifted(to, s + off, n, sb, se, bar, policy);
-                    }
+                    copy_shifted(to, s + off, n, sb, se, bar, policy);
                 }
             }
             __syncwarp();
@@ -309,23 +372,61 @@ struct Stream {
         }
     }
 
-    template <int NP>
-    static __device__ __forceinline__ void load_tokens(const T* const (&x)[NP], int count, int k, int cols, bool aligned,
-                                                       uint4 (&v)[NP]) {
-#pragma unroll
-        for (int n = 0; n < NP; ++n)
-            if (n % NT * 8 < count) v[n] = load_piece<T>(x[n], k, cols, aligned);
+    // Scales as floats. A byte moved to the exponent field is the scale, but for the bytes 0
+    // (2^-127, subnormal) and 255 (NaN); a warp that meets one takes the exact conversion.
+    static __device__ __forceinline__ bool special_scale(uint32_t w) {
+        return (((w - 0x01010101u) & ~w) | ((~w - 0x01010101u) & w)) & 0x80808080u;
+    }
+    template <bool SPECIAL>
+    static __device__ __forceinline__ float scale_of(uint32_t w, int b) {
+        if constexpr (SPECIAL) return mx_scale((w >> (8 * b)) & 255u);
+        return __uint_as_float((b < 3 ? w << (23 - 8 * b) : w >> 1) & 0x7F800000u);
     }
 
-    // Consumer warp: one item. x: this lane's token row of each group of eight (advanced to its
-    // quad's eight values); with SPLIT, x holds the rows of a second addend after the first NT,
-    // multiplied by the same weights. Leaves the partial sums in the next buffer.
-    template <int NM, bool SPLIT>
+    // One group of 32 values of an MXFP4 unit: `a`: this lane's word of row g in the first tile.
+    template <int NM, bool SPLIT, bool SPECIAL, bool FAST, int NP>
+    static __device__ __forceinline__ void multiply_mx(float (&acc)[NM][NT][4], const uint4 (&x)[NP], uint32_t a,
+                                                       const uint32_t (&sc)[NM][2], int b, int count) {
+        using S = Shape<NM>;
+        constexpr int kTile = FAST ? S::kBoxes * kBox : S::kTile, kHalf = FAST ? 8 * 128 : 8 * S::kPitch;
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            uint32_t lo[4], hi[4];
+            Num<T>::decode(lds32(a + m * kTile), lo);
+            Num<T>::decode(lds32(a + m * kTile + kHalf), hi);
+            const float sl = scale_of<SPECIAL>(sc[m][0], b), sh = scale_of<SPECIAL>(sc[m][1], b);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                if (n * 8 >= count) break;
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                Num<T>::mma(d, lo[0], hi[0], lo[1], hi[1], x[n].x, x[n].y);
+                Num<T>::mma(d, lo[2], hi[2], lo[3], hi[3], x[n].z, x[n].w);
+                if (SPLIT) {
+                    Num<T>::mma(d, lo[0], hi[0], lo[1], hi[1], x[NP - NT + n].x, x[NP - NT + n].y);
+                    Num<T>::mma(d, lo[2], hi[2], lo[3], hi[3], x[NP - NT + n].z, x[NP - NT + n].w);
+                }
+                acc[m][n][0] = fmaf(d[0], sl, acc[m][n][0]);
+                acc[m][n][1] = fmaf(d[1], sl, acc[m][n][1]);
+                acc[m][n][2] = fmaf(d[2], sh, acc[m][n][2]);
+                acc[m][n][3] = fmaf(d[3], sh, acc[m][n][3]);
+            }
+        }
+    }
+
+    // Consumer warp: one item. x: this lane's token row of each group of eight; with SPLIT, x holds
+    // the rows of a second addend after the first NT, multiplied by the same weights. FAST: the
+    // weights have maps and the rows of x start on 16 bytes. Leaves the partial sums in the next buffer.
+    //
+    // A warp takes every kConsumers-th unit of a stage. Its tokens are loaded GROUP sub-steps of
+    // 32 values ahead: enough that they come from L2 in time, as many as the registers hold.
+    template <int NM, bool SPLIT, bool FAST>
     static __device__ __forceinline__ void consume(const Layout& l, Place& p, const Tiles<NM>& t,
                                                    const WeightView (&v)[NM], const T* const (&x)[SPLIT ? 2 * NT : NT],
-                                                   int count, int x_cols, bool x_aligned) {
+                                                   int count, int x_cols) {
         using S = Shape<NM>;
         constexpr int NP = SPLIT ? 2 * NT : NT;
+        constexpr int kSteps = S::kUnits / kConsumers * kSub;  // sub-steps of a warp in a full stage
+        constexpr int kGroup = NP >= 8 ? 1 : NP >= 4 ? 2 : kSteps < 4 ? kSteps : 4;
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
         float acc[NM][NT][4];
 #pragma unroll
@@ -334,119 +435,131 @@ struct Stream {
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) acc[m][n][c] = 0.f;
-        // how far rows g and g + 8 are shifted in their stage
+        const int row = tile_row(g);  // and row + 8
+        // how far these rows are shifted in their stage
         uint32_t shift[NM][2];
 #pragma unroll
         for (int m = 0; m < NM; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                shift[m][h] = v[0].shifted ? uint32_t(reinterpret_cast<uintptr_t>(v[m].begin[MX ? 1 : 0]) +
-                                                      (t.row[m] + g + 8 * h) * v[m].pitch[MX ? 1 : 0]) & 15u
-                                           : 0u;
+                shift[m][h] = FAST ? 0u
+                                   : uint32_t(reinterpret_cast<uintptr_t>(v[m].begin[MX ? 1 : 0]) +
+                                              (t.row[m] + row + 8 * h) * v[m].pitch[MX ? 1 : 0]) & 15u;
+        // k of this lane's piece in sub-step s of chunk c
+        auto k_of = [&](int c, int s) { return ((c * S::kUnits + warp + s / kSub * kConsumers) * kSub + s % kSub) * 32 + q * 8; };
+        uint4 next[kGroup][NP];
+        auto load = [&](int c, int s) {
+#pragma unroll
+            for (int i = 0; i < kGroup; ++i)
+#pragma unroll
+                for (int n = 0; n < NP; ++n)
+                    if (n % NT * 8 < count) next[i][n] = load_piece<T, FAST>(x[n], k_of(c, s + i), x_cols);
+        };
         const int chunks = (v[0].units + S::kUnits - 1) / S::kUnits;
-        for (int c = 0; c < chunks && p.ok; ++c) {
+        load(0, 0);
+        for (int c = 0; c < chunks; ++c) {
             const int units = min(S::kUnits, v[0].units - c * S::kUnits);
-            uint4 xv[NP];
-            int k = (c * S::kUnits + warp) * (32 * kSub) + q * 8;
-            if (warp < units) load_tokens(x, count, k, x_cols, x_aligned, xv);
             if (!mbar_wait_warp(l.full + 8 * p.stage, p.phase)) {
                 p.ok = false;
                 break;
             }
             const uint32_t at = l.ring + p.stage * kStage;
 #pragma unroll 1
-            for (int u = warp; u < units; u += kConsumers) {
+            for (int s = 0; s < kSteps; s += kGroup) {
+                uint4 now[kGroup][NP];
+#pragma unroll
+                for (int i = 0; i < kGroup; ++i)
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) now[i][n] = MX ? Num<T>::order(next[i][n]) : next[i][n];
+                if (s + kGroup < kSteps)
+                    load(c, s + kGroup);
+                else if (c + 1 < chunks)
+                    load(c + 1, 0);
                 if constexpr (MX) {
+                    const int u = warp + s / kSub * kConsumers;  // a group lies within a unit
+                    if (u >= units) continue;
                     uint32_t sc[NM][2];
+                    bool special = false;
 #pragma unroll
                     for (int m = 0; m < NM; ++m)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint32_t a = at + S::kScales + (m * kTileRows + g + 8 * h) * S::kScalePitch + u * 4;
-                            if (!v[0].shifted) {
-                                sc[m][h] = lds32(a);
+                            const int r = row + 8 * h;
+                            if (FAST) {
+                                sc[m][h] = lds32(at + kBoxScales + (m + u / 16) * kScaleBox + r * 64 +
+                                                 (((u >> 2) ^ (r >> 1)) & 3) * 16 + (u & 3) * 4);
                             } else {
-                                const uint32_t b = a + shift[m][h];
+                                const uint32_t b = at + S::kScales + (m * kTileRows + r) * S::kScalePitch + u * 4 + shift[m][h];
                                 sc[m][h] = __funnelshift_r(lds32(b & ~3u), lds32((b & ~3u) + 4), (b & 3u) * 8);
                             }
+                            special |= special_scale(sc[m][h]);
                         }
-                    const int subs = min(kSub, v[0].pitch[1] - (c * S::kUnits + u) * kSub);
+                    const int subs = v[0].pitch[1] - (c * S::kUnits + u) * kSub;  // blocks left in the row
+                    // this lane's word of block b: of its row, q-th in the block
+                    const uint32_t a = FAST ? at + (u >> 1) * kBox + row * 128 + q * 4 : at + row * S::kPitch + u * kUnitBytes + q * 4;
+                    auto block = [&](int b) { return FAST ? a + ((((u & 1) * 4 + b) ^ row) & 7) * 16 : a + b * 16; };
+                    if (__any_sync(0xFFFFFFFFu, special) || subs < kSub) {
 #pragma unroll
-                    for (int b = 0; b < kSub; ++b) {
-                        if (b >= subs) break;
-                        uint4 now[NP];
+                        for (int i = 0; i < kGroup; ++i) {
+                            const int b = s % kSub + i;
+                            if (b < subs) multiply_mx<NM, SPLIT, true, FAST>(acc, now[i], block(b), sc, b, count);
+                        }
+                    } else if constexpr (kGroup == kSub) {
 #pragma unroll
-                        for (int n = 0; n < NP; ++n) now[n] = Num<T>::order(xv[n]);
-                        if (b + 1 < subs)
-                            load_tokens(x, count, k + 32 * (b + 1), x_cols, x_aligned, xv);
-                        else if (u + kConsumers < units)
-                            load_tokens(x, count, k + 32 * kSub * kConsumers, x_cols, x_aligned, xv);
+                        for (int i = 0; i < kGroup; ++i)
+                            multiply_mx<NM, SPLIT, false, FAST>(acc, now[i], block(i), sc, i, count);
+                    } else {
 #pragma unroll
-                        for (int m = 0; m < NM; ++m) {
-                            const uint32_t a = at + m * S::kTile + g * S::kPitch + u * kUnitBytes + b * 16 + q * 4;
-                            uint32_t lo[4], hi[4];
-                            Num<T>::decode(lds32(a), lo);
-                            Num<T>::decode(lds32(a + 8 * S::kPitch), hi);
-                            const float sl = mx_scale((sc[m][0] >> (8 * b)) & 255u);
-                            const float sh = mx_scale((sc[m][1] >> (8 * b)) & 255u);
+                        for (int i = 0; i < kGroup; ++i) {
+                            uint32_t shifted[NM][2];  // this sub-step's bytes lowest
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) {
-                                if (n * 8 >= count) break;
-                                float d[4] = {0.f, 0.f, 0.f, 0.f};
-                                Num<T>::mma(d, lo[0], hi[0], lo[1], hi[1], now[n].x, now[n].y);
-                                Num<T>::mma(d, lo[2], hi[2], lo[3], hi[3], now[n].z, now[n].w);
-                                if (SPLIT) {
-                                    Num<T>::mma(d, lo[0], hi[0], lo[1], hi[1], now[NP - NT + n].x, now[NP - NT + n].y);
-                                    Num<T>::mma(d, lo[2], hi[2], lo[3], hi[3], now[NP - NT + n].z, now[NP - NT + n].w);
-                                }
-                                acc[m][n][0] = fmaf(d[0], sl, acc[m][n][0]);
-                                acc[m][n][1] = fmaf(d[1], sl, acc[m][n][1]);
-                                acc[m][n][2] = fmaf(d[2], sh, acc[m][n][2]);
-                                acc[m][n][3] = fmaf(d[3], sh, acc[m][n][3]);
-                            }
+                            for (int m = 0; m < NM; ++m)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) shifted[m][h] = sc[m][h] >> (8 * (s % kSub + i));
+                            multiply_mx<NM, SPLIT, false, FAST>(acc, now[i], block(s % kSub + i), shifted, 0, count);
                         }
                     }
                 } else {
-                    uint4 now[NP];
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) now[n] = xv[n];
-                    if (u + kConsumers < units)
-                        load_tokens(x, count, k + 32 * kConsumers, x_cols, x_aligned, xv);
-                    const int left = v[0].cols - k;  // values of this lane's pieces that the row has
+                    for (int i = 0; i < kGroup; ++i) {
+                        const int u = warp + (s + i) * kConsumers;
+                        if (u >= units) break;
+                        const int left = v[0].cols - k_of(c, s + i);  // values of this lane's pieces that the row has
 #pragma unroll
-                    for (int m = 0; m < NM; ++m) {
-                        uint4 a[2];
+                        for (int m = 0; m < NM; ++m) {
+                            uint4 a[2];
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint32_t o = at + m * S::kTile + (g + 8 * h) * S::kPitch + u * kUnitBytes + q * 16;
-                            if (!v[0].shifted) {
-                                a[h] = lds128(left > 0 ? o : l.zero);
-                            } else {
-                                const uint32_t b = o + shift[m][h], s = (b & 2u) * 8;
-                                uint32_t w[5];
+                            for (int h = 0; h < 2; ++h) {
+                                if (FAST) {
+                                    a[h] = lds128(at + (m * S::kBoxes + (u >> 1)) * kBox + (row + 8 * h) * 128 +
+                                                  ((((u & 1) * 4 + q) ^ row) & 7) * 16);
+                                } else {
+                                    const uint32_t b = at + m * S::kTile + (row + 8 * h) * S::kPitch + u * kUnitBytes + q * 16 + shift[m][h];
+                                    const uint32_t f = (b & 2u) * 8;
+                                    uint32_t w[5];
 #pragma unroll
-                                for (int i = 0; i < 5; ++i) w[i] = lds32((b & ~3u) + 4 * i);
+                                    for (int j = 0; j < 5; ++j) w[j] = lds32((b & ~3u) + 4 * j);
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    w[i] = __funnelshift_r(w[i], w[i + 1], s);
-                                    if (2 * i + 1 >= left) w[i] = 2 * i >= left ? 0u : w[i] & 0xFFFFu;
+                                    for (int j = 0; j < 4; ++j) {
+                                        w[j] = __funnelshift_r(w[j], w[j + 1], f);
+                                        if (2 * j + 1 >= left) w[j] = 2 * j >= left ? 0u : w[j] & 0xFFFFu;
+                                    }
+                                    a[h] = make_uint4(w[0], w[1], w[2], w[3]);
                                 }
-                                a[h] = make_uint4(w[0], w[1], w[2], w[3]);
                             }
-                        }
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            if (n * 8 >= count) break;
-                            Num<T>::mma(acc[m][n], a[0].x, a[1].x, a[0].y, a[1].y, now[n].x, now[n].y);
-                            Num<T>::mma(acc[m][n], a[0].z, a[1].z, a[0].w, a[1].w, now[n].z, now[n].w);
-                            if (SPLIT) {
-                                Num<T>::mma(acc[m][n], a[0].x, a[1].x, a[0].y, a[1].y, now[NP - NT + n].x, now[NP - NT + n].y);
-                                Num<T>::mma(acc[m][n], a[0].z, a[1].z, a[0].w, a[1].w, now[NP - NT + n].z, now[NP - NT + n].w);
+                            for (int n = 0; n < NT; ++n) {
+                                if (n * 8 >= count) break;
+                                Num<T>::mma(acc[m][n], a[0].x, a[1].x, a[0].y, a[1].y, now[i][n].x, now[i][n].y);
+                                Num<T>::mma(acc[m][n], a[0].z, a[1].z, a[0].w, a[1].w, now[i][n].z, now[i][n].w);
+                                if (SPLIT) {
+                                    Num<T>::mma(acc[m][n], a[0].x, a[1].x, a[0].y, a[1].y, now[i][NP - NT + n].x, now[i][NP - NT + n].y);
+                                    Num<T>::mma(acc[m][n], a[0].z, a[1].z, a[0].w, a[1].w, now[i][NP - NT + n].z, now[i][NP - NT + n].w);
+                                }
                             }
                         }
                     }
                 }
-                k += 32 * kSub * kConsumers;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(l.empty + 8 * p.stage);
@@ -464,7 +577,7 @@ struct Stream {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 if (n * 8 >= count) break;
-                const uint32_t a = part + ((m * NT * 8 + n * 8 + 2 * q) * kPartPitch + g) * 4;
+                const uint32_t a = part + ((m * NT * 8 + n * 8 + 2 * q) * kPartPitch + row) * 4;
                 sts32(a, __float_as_uint(acc[m][n][0]));
                 sts32(a + kPartPitch * 4, __float_as_uint(acc[m][n][1]));
                 sts32(a + 32, __float_as_uint(acc[m][n][2]));
