@@ -23,6 +23,8 @@
 // after the other, so that the second finds the weights in L2.
 #pragma once
 
+#include <type_traits>
+
 #include "stream.cuh"
 
 namespace swb {
@@ -77,10 +79,12 @@ __host__ __device__ inline MoeWorkspace moe_workspace(int tokens, int experts, i
 // What every CTA derives from the selection. Rows of h stand in the order of their experts,
 // then tokens; a group is up to 32 of an expert's rows.
 struct MoeRoute {
-    int groups;
+    unsigned long long taken[kMoeMaxExperts];          // an expert's tokens, a bit each
     float share[kMoeMaxTokens * kMoeMaxTopk];          // of each row of h: its expert's weight
-    short pick[kMoeMaxTokens * kMoeMaxTopk];           // [token, place]: the expert
-    short count[kMoeMaxExperts];                       // tokens of each expert
+    float shares[kMoeMaxTokens * kMoeMaxTopk];         // [token, place]: the same
+    int pick[kMoeMaxTokens * kMoeMaxTopk];             // [token, place]: the expert
+    int groups;
+    short row[kMoeMaxExperts];                         // an expert's first row of h
     short expert[kMoeMaxGroups];                       // of each group
     short start[kMoeMaxGroups + 1];                    // its first row of h, and the end
     short first[kMoeMaxGroups];                        // the expert's first group
@@ -139,10 +143,8 @@ __device__ __forceinline__ bool moe_above(double a, int ia, double b, int ib) {
     return a > b;
 }
 
-// One warp selects a token's experts from its logits.
-template <typename T>
-__device__ void moe_select(const MoeParams& P, int token, int lane) {
-    const double* l = P.logits + size_t(token) * P.experts;
+// One warp selects a token's experts from its logits `l` into picks and shares [topk].
+__device__ inline void moe_select(const MoeParams& P, const double* l, int* picks, float* shares, int lane) {
     constexpr int kPer = kMoeMaxExperts / 32;
     double v[kPer];
     uint32_t left = 0;  // which of this lane's logits are still in play
@@ -151,7 +153,7 @@ __device__ void moe_select(const MoeParams& P, int token, int lane) {
         const int e = lane + 32 * i;
         v[i] = 0.0;
         if (e < P.experts) {
-            v[i] = __ldcg(l + e);
+            v[i] = *reinterpret_cast<const volatile double*>(l + e);
             left |= 1u << i;
         }
     }
@@ -187,18 +189,44 @@ __device__ void moe_select(const MoeParams& P, int token, int lane) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
     if (lane < P.topk) {
-        const int at = token * P.topk + lane;
-        const float share = e / sum;
-        P.picks[at] = pick;
-        P.shares[at] = share;
-        if (P.ids) P.ids[at] = pick;
-        if (P.weights) P.weights[at] = share;
+        picks[lane] = pick;
+        shares[lane] = e / sum;
     }
 }
 
 template <typename T>
 __device__ __forceinline__ uint4 route_piece(const T* row, int k, int cols, int aligned) {
     return aligned ? load_piece<T, true>(row, k, cols) : load_piece<T, false>(row, k, cols);
+}
+
+// Router of a few (token, expert) pairs: every CTA takes all of them, a warp a pair at a time, and
+// selects for itself, which costs less than telling the others. Logits in 64 bits as above.
+constexpr int kRouteAlone = 32;  // pairs; 148 CTAs reading the router's rows from L2 is about a barrier's time
+template <typename T>
+__device__ void moe_router_alone(const MoeParams& P, double* logits, int* picks, float* shares) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const T* x = static_cast<const T*>(P.x);
+    const T* r = static_cast<const T*>(P.router);
+    for (int pair = warp; pair < P.tokens * P.experts; pair += kConsumers) {
+        const int t = pair / P.experts, e = pair % P.experts;
+        double sum[8] = {0., 0., 0., 0., 0., 0., 0., 0.};
+#pragma unroll 4
+        for (int k = lane * 8; k < P.hidden; k += 256) {
+            const uint4 wv = route_piece(r + size_t(e) * P.hidden, k, P.hidden, P.router_aligned);
+            const uint4 xv = route_piece(x + t * P.x_pitch, k, P.hidden, P.x_aligned);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                sum[i] = fma(double(Num<T>::to_float(reinterpret_cast<const T*>(&wv)[i])),
+                             double(Num<T>::to_float(reinterpret_cast<const T*>(&xv)[i])), sum[i]);
+        }
+        double s = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+        if (lane == 0) logits[pair] = s;
+    }
+    named_barrier_sync(1, kRouteThreads);
+    for (int t = warp; t < P.tokens; t += kConsumers)
+        moe_select(P, logits + t * P.experts, picks + t * P.topk, shares + t * P.topk, lane);
 }
 
 // The first kRouteThreads threads of the CTA.
@@ -267,29 +295,36 @@ __device__ void moe_router(const MoeParams& P, double* scratch, int* flag) {
             }
         }
         named_barrier_sync(1, kRouteThreads);
-        if (*flag && warp < nt) moe_select<T>(P, t0 + warp, lane);
+        if (*flag && warp < nt) {
+            const int t = t0 + warp;
+            moe_select(P, P.logits + size_t(t) * P.experts, P.picks + t * P.topk, P.shares + t * P.topk, lane);
+        }
         named_barrier_sync(1, kRouteThreads);
     }
 }
 
-// Groups of each expert's tokens, in token order, the same in every CTA.
+// Groups of each expert's tokens, in token order, the same in every CTA; R.pick and R.shares
+// are set. One CTA hands the selection to the caller.
 __device__ inline void moe_lists(const MoeParams& P, MoeRoute& R) {
     const int n = P.tokens * P.topk, t = threadIdx.x;
-    for (int i = t; i < n; i += kStreamThreads) R.pick[i] = short(__ldcg(P.picks + i));
+    if (t < kMoeMaxExperts) R.taken[t] = 0ull;
     __syncthreads();
-    if (t < kMoeMaxExperts) {
-        int mine = 0;
-        for (int i = 0; i < n; ++i) mine += R.pick[i] == t;
-        R.count[t] = short(mine);
+    for (int i = t; i < n; i += kStreamThreads) {
+        atomicOr(&R.taken[R.pick[i]], 1ull << (i / P.topk));  // a token takes an expert once: the bits are its rows
+        if (blockIdx.x == 0) {
+            if (P.ids) P.ids[i] = R.pick[i];
+            if (P.weights) P.weights[i] = R.shares[i];
+        }
     }
     __syncthreads();
     if (t < 32) {  // eight experts a lane: rows and groups before them
         constexpr int kPer = kMoeMaxExperts / 32;
-        int rows = 0, groups = 0;
+        int count[kPer], rows = 0, groups = 0;
+#pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int c = R.count[t * kPer + i];
-            rows += c;
-            groups += (c + kMoeGroup - 1) / kMoeGroup;
+            count[i] = __popcll(R.taken[t * kPer + i]);
+            rows += count[i];
+            groups += (count[i] + kMoeGroup - 1) / kMoeGroup;
         }
         int row = rows, a = groups;
 #pragma unroll
@@ -303,8 +338,10 @@ __device__ inline void moe_lists(const MoeParams& P, MoeRoute& R) {
         }
         row -= rows;
         a -= groups;
+#pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int e = t * kPer + i, c = R.count[e], k = (c + kMoeGroup - 1) / kMoeGroup;
+            const int e = t * kPer + i, k = (count[i] + kMoeGroup - 1) / kMoeGroup;
+            R.row[e] = short(row);
             for (int j = 0; j < k; ++j) {
                 R.expert[a + j] = short(e);
                 R.start[a + j] = short(row + j * kMoeGroup);
@@ -312,18 +349,15 @@ __device__ inline void moe_lists(const MoeParams& P, MoeRoute& R) {
                 R.of_expert[a + j] = short(k);
             }
             a += k;
-            row += c;
+            row += count[i];
         }
     }
     __syncthreads();
-    if (t < R.groups && R.first[t] == t) {
-        const int e = R.expert[t];
-        int row = R.start[t];
-        for (int i = 0; i < n; ++i)
-            if (R.pick[i] == e) {
-                R.token[row] = static_cast<unsigned char>(i / P.topk);
-                R.share[row++] = __ldcg(P.shares + i);
-            }
+    for (int i = t; i < n; i += kStreamThreads) {
+        const int e = R.pick[i], token = i / P.topk;
+        const int row = R.row[e] + __popcll(R.taken[e] & ((1ull << token) - 1ull));
+        R.token[row] = static_cast<unsigned char>(token);
+        R.share[row] = R.shares[i];
     }
     __syncthreads();
 }
@@ -343,8 +377,18 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     const auto l = Pipe::layout(smem_u32(smem), S::kStages);
     if (threadIdx.x == kStreamThreads - 1) Pipe::init(l);
 
-    if (warp < kConsumers) moe_router<T>(P, scratch, &flag);
-    if (!moe_grid_barrier(P.sync, &flag)) return;
+    if (P.tokens * P.experts <= kRouteAlone) {
+        if (warp < kConsumers) moe_router_alone<T>(P, scratch, R.pick, R.shares);
+        __syncthreads();
+    } else {
+        if (warp < kConsumers) moe_router<T>(P, scratch, &flag);
+        if (!moe_grid_barrier(P.sync, &flag)) return;
+        for (int i = threadIdx.x; i < P.tokens * P.topk; i += kStreamThreads) {
+            R.pick[i] = __ldcg(P.picks + i);
+            R.shares[i] = __ldcg(P.shares + i);
+        }
+        __syncthreads();
+    }
     moe_lists(P, R);
 
     // gate: items [g0, g1) are (expert, tile, group); down: tiles [d0, d1) times every group
@@ -391,34 +435,60 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
                 Pipe::template produce<1>(l, place, down_rows(a, d), dv, policy);
         Pipe::drain(l, place);
     } else if (warp < kConsumers) {
-        const T* x[2 * NT];
-        for (int i = g0; i < g1 && place.ok; ++i) {
-            int group, row;
-            gate_item(i, group, row);
-            const int start = R.start[group], count = R.start[group + 1] - start;
-            const T* xg[NT];
+        auto gate = [&](auto fast) {
+            typename Pipe::template Tokens<2, false> tokens;
+            auto turn_to = [&](int i) {
+                tokens.count = 0;
+                if (i >= g1) return;
+                int group, row;
+                gate_item(i, group, row);
+                const int start = R.start[group];
+                tokens.count = R.start[group + 1] - start;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-                xg[n] = static_cast<const T*>(P.x) + R.token[start + min(n * 8 + (lane >> 2), count - 1)] * P.x_pitch;
-            if (gv[0].maps)
-                Pipe::template consume<2, false, true>(l, place, gate_rows(group, row), gv, xg, count, P.hidden);
-            else
-                Pipe::template consume<2, false, false>(l, place, gate_rows(group, row), gv, xg, count, P.hidden);
-        }
+                for (int n = 0; n < NT; ++n)
+                    tokens.x[n] = static_cast<const T*>(P.x) + R.token[start + min(n * 8 + (lane >> 2), tokens.count - 1)] * P.x_pitch;
+            };
+            turn_to(g0);
+            tokens.template load<decltype(fast)::value>(0, 0, P.hidden);
+            for (int i = g0; i < g1 && place.ok; ++i) {
+                int group, row;
+                gate_item(i, group, row);
+                Pipe::template consume<2, false, decltype(fast)::value>(l, place, gate_rows(group, row), gv, tokens, P.hidden,
+                                                                        [&](auto&) { turn_to(i + 1); });
+            }
+        };
+        if (gv[0].maps)
+            gate(std::true_type{});
+        else
+            gate(std::false_type{});
         named_barrier_sync(2, kStreamThreads - 32);  // h is complete, or flag says that it will not be
-        for (int d = d0; d < d1 && flag; ++d)
-            for (int a = 0; a < R.groups && place.ok; ++a) {
-                const int start = R.start[a], count = R.start[a + 1] - start;
+        auto down = [&](auto fast) {
+            typename Pipe::template Tokens<1, true> tokens;
+            auto turn_to = [&](int d, int a) {
+                if (a == R.groups) ++d, a = 0;
+                tokens.count = 0;
+                if (d >= d1) return;
+                const int start = R.start[a];
+                tokens.count = R.start[a + 1] - start;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    x[n] = h + int64_t(start + min(n * 8 + (lane >> 2), count - 1)) * P.h_pitch;
-                    x[NT + n] = x[n] + h_plane;
+                    tokens.x[n] = h + int64_t(start + min(n * 8 + (lane >> 2), tokens.count - 1)) * P.h_pitch;
+                    tokens.x[NT + n] = tokens.x[n] + h_plane;
                 }
-                if (dv[0].maps)
-                    Pipe::template consume<1, true, true>(l, place, down_rows(a, d), dv, x, count, P.h_pitch);
-                else
-                    Pipe::template consume<1, true, false>(l, place, down_rows(a, d), dv, x, count, P.h_pitch);
-            }
+            };
+            turn_to(d0, 0);
+            tokens.template load<decltype(fast)::value>(0, 0, P.h_pitch);
+            for (int d = d0; d < d1; ++d)
+                for (int a = 0; a < R.groups && place.ok; ++a)
+                    Pipe::template consume<1, true, decltype(fast)::value>(l, place, down_rows(a, d), dv, tokens, P.h_pitch,
+                                                                           [&](auto&) { turn_to(d, a + 1); });
+        };
+        if (flag) {
+            if (dv[0].maps)
+                down(std::true_type{});
+            else
+                down(std::false_type{});
+        }
     } else {
         const int thread = threadIdx.x - (kConsumers + 1) * 32;
         for (int i = g0; i < g1 && Pipe::acquire(l, place); ++i) {

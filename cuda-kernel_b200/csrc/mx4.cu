@@ -2,6 +2,7 @@
 // weight matrix with 16-bit tokens (declarations: include/swiglu_b200.h).
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 #include "host.h"
 #include "stream.cuh"
@@ -289,18 +290,25 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         for (int64_t i = first; i < last && place.ok; ++i) Pipe::template produce<2>(l, place, tiles(i), v, policy);
         Pipe::drain(l, place);
     } else if (warp < kConsumers) {
-        const T* x[NT];
-        for (int64_t i = first; i < last && place.ok; ++i) {
-            const int64_t t0 = i / P.tiles * (NT * 8);
-            const int count = int(min(int64_t(NT * 8), P.tokens - t0));
+        auto items = [&](auto fast) {
+            typename Pipe::template Tokens<2, false> tokens;
+            auto turn_to = [&](int64_t i) {
+                const int64_t t0 = i / P.tiles * (NT * 8);
+                tokens.count = i < last ? int(min(int64_t(NT * 8), P.tokens - t0)) : 0;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-                x[n] = static_cast<const T*>(P.x) + (t0 + min(n * 8 + (lane >> 2), count - 1)) * P.x_pitch;
-            if (P.x_aligned && P.fast)
-                Pipe::template consume<2, false, true>(l, place, tiles(i), v, x, count, P.cols);
-            else
-                Pipe::template consume<2, false, false>(l, place, tiles(i), v, x, count, P.cols);
-        }
+                for (int n = 0; n < NT; ++n)
+                    tokens.x[n] = static_cast<const T*>(P.x) + (t0 + min(n * 8 + (lane >> 2), max(tokens.count - 1, 0))) * P.x_pitch;
+            };
+            turn_to(first);
+            tokens.template load<decltype(fast)::value>(0, 0, P.cols);
+            for (int64_t i = first; i < last && place.ok; ++i)
+                Pipe::template consume<2, false, decltype(fast)::value>(l, place, tiles(i), v, tokens, P.cols,
+                                                                        [&](auto&) { turn_to(i + 1); });
+        };
+        if (P.fast)
+            items(std::true_type{});
+        else
+            items(std::false_type{});
     } else {
         const int thread = threadIdx.x - (kConsumers + 1) * 32;
         for (int64_t i = first; i < last && Pipe::acquire(l, place); ++i) {

@@ -413,20 +413,44 @@ struct Stream {
         }
     }
 
-    // Consumer warp: one item. x: this lane's token row of each group of eight; with SPLIT, x holds
-    // the rows of a second addend after the first NT, multiplied by the same weights. FAST: the
-    // weights have maps and the rows of x start on 16 bytes. Leaves the partial sums in the next buffer.
-    //
-    // A warp takes every kConsumers-th unit of a stage. Its tokens are loaded GROUP sub-steps of
-    // 32 values ahead: enough that they come from L2 in time, as many as the registers hold.
-    template <int NM, bool SPLIT, bool FAST>
+    // The tokens of an item as a consumer lane reads them: its row of each group of eight; with
+    // SPLIT, the rows of a second addend after the first NT, multiplied by the same weights. A warp
+    // takes every kConsumers-th unit of a stage and loads its tokens kGroup sub-steps of 32 values
+    // ahead, into the next item too: enough that they come from L2 in time.
+    template <int NM, bool SPLIT>
+    struct Tokens {
+        static constexpr int kRows = SPLIT ? 2 * NT : NT;
+        static constexpr int kSteps = Shape<NM>::kUnits / kConsumers * kSub;  // sub-steps of a warp in a full stage
+        static constexpr int kGroup = kRows >= 8 ? 1 : kRows >= 4 ? 2 : kSteps < 4 ? kSteps : 4;
+        const T* x[kRows];  // this lane's rows
+        int count;          // tokens; 0: no item
+        uint4 ahead[kGroup][kRows];
+
+        // k of this lane's piece in sub-step s of chunk c
+        static __device__ __forceinline__ int k_of(int c, int s) {
+            const int warp = threadIdx.x >> 5, q = threadIdx.x & 3;
+            return ((c * Shape<NM>::kUnits + warp + s / kSub * kConsumers) * kSub + s % kSub) * 32 + q * 8;
+        }
+        template <bool FAST>
+        __device__ __forceinline__ void load(int c, int s, int cols) {
+#pragma unroll
+            for (int i = 0; i < kGroup; ++i)
+#pragma unroll
+                for (int n = 0; n < kRows; ++n)
+                    if (n % NT * 8 < count) ahead[i][n] = load_piece<T, FAST>(x[n], k_of(c, s + i), cols);
+        }
+    };
+
+    // Consumer warp: one item. tokens.ahead holds its first values; following(tokens) turns tokens to
+    // the next item (count 0: none). FAST: the weights have maps and the rows of x start on 16
+    // bytes. Leaves the partial sums in the next buffer.
+    template <int NM, bool SPLIT, bool FAST, typename Next>
     static __device__ __forceinline__ void consume(const Layout& l, Place& p, const Tiles<NM>& t,
-                                                   const WeightView (&v)[NM], const T* const (&x)[SPLIT ? 2 * NT : NT],
-                                                   int count, int x_cols) {
+                                                   const WeightView (&v)[NM], Tokens<NM, SPLIT>& tokens, int x_cols,
+                                                   Next&& following) {
         using S = Shape<NM>;
-        constexpr int NP = SPLIT ? 2 * NT : NT;
-        constexpr int kSteps = S::kUnits / kConsumers * kSub;  // sub-steps of a warp in a full stage
-        constexpr int kGroup = NP >= 8 ? 1 : NP >= 4 ? 2 : kSteps < 4 ? kSteps : 4;
+        constexpr int NP = Tokens<NM, SPLIT>::kRows, kSteps = Tokens<NM, SPLIT>::kSteps, kGroup = Tokens<NM, SPLIT>::kGroup;
+        const int count = tokens.count;
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
         float acc[NM][NT][4];
 #pragma unroll
@@ -445,18 +469,7 @@ struct Stream {
                 shift[m][h] = FAST ? 0u
                                    : uint32_t(reinterpret_cast<uintptr_t>(v[m].begin[MX ? 1 : 0]) +
                                               (t.row[m] + row + 8 * h) * v[m].pitch[MX ? 1 : 0]) & 15u;
-        // k of this lane's piece in sub-step s of chunk c
-        auto k_of = [&](int c, int s) { return ((c * S::kUnits + warp + s / kSub * kConsumers) * kSub + s % kSub) * 32 + q * 8; };
-        uint4 next[kGroup][NP];
-        auto load = [&](int c, int s) {
-#pragma unroll
-            for (int i = 0; i < kGroup; ++i)
-#pragma unroll
-                for (int n = 0; n < NP; ++n)
-                    if (n % NT * 8 < count) next[i][n] = load_piece<T, FAST>(x[n], k_of(c, s + i), x_cols);
-        };
         const int chunks = (v[0].units + S::kUnits - 1) / S::kUnits;
-        load(0, 0);
         for (int c = 0; c < chunks; ++c) {
             const int units = min(S::kUnits, v[0].units - c * S::kUnits);
             if (!mbar_wait_warp(l.full + 8 * p.stage, p.phase)) {
@@ -470,11 +483,15 @@ struct Stream {
 #pragma unroll
                 for (int i = 0; i < kGroup; ++i)
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) now[i][n] = MX ? Num<T>::order(next[i][n]) : next[i][n];
-                if (s + kGroup < kSteps)
-                    load(c, s + kGroup);
-                else if (c + 1 < chunks)
-                    load(c + 1, 0);
+                    for (int n = 0; n < NP; ++n) now[i][n] = MX ? Num<T>::order(tokens.ahead[i][n]) : tokens.ahead[i][n];
+                if (s + kGroup < kSteps) {
+                    tokens.template load<FAST>(c, s + kGroup, x_cols);
+                } else if (c + 1 < chunks) {
+                    tokens.template load<FAST>(c + 1, 0, x_cols);
+                } else {
+                    following(tokens);
+                    tokens.template load<FAST>(0, 0, x_cols);
+                }
                 if constexpr (MX) {
                     const int u = warp + s / kSub * kConsumers;  // a group lies within a unit
                     if (u >= units) continue;
@@ -524,7 +541,7 @@ struct Stream {
                     for (int i = 0; i < kGroup; ++i) {
                         const int u = warp + (s + i) * kConsumers;
                         if (u >= units) break;
-                        const int left = v[0].cols - k_of(c, s + i);  // values of this lane's pieces that the row has
+                        const int left = v[0].cols - Tokens<NM, SPLIT>::k_of(c, s + i);  // values of this lane's pieces that the row has
 #pragma unroll
                         for (int m = 0; m < NM; ++m) {
                             uint4 a[2];
