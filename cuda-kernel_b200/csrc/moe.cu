@@ -50,7 +50,7 @@ int launch_moe(MoeParams P, cudaStream_t stream) {
     P.deep[0] = deep[0];
     P.deep[1] = deep[2];
     // every CTA resident at once: the cooperative launch makes the runtime check it
-    return launch_ex(kernel, unsigned(sms), kStreamThreads, S::kSmem, stream, true, maps, P);
+    return launch_ex(kernel, unsigned(sms), S::Pipe::kThreads, S::kSmem, stream, true, maps, P);
 }
 
 template <typename T, bool MX>

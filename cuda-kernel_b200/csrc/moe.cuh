@@ -35,7 +35,7 @@ constexpr int kMoeMaxTopk = 16;
 constexpr int kMoeGroup = 32;  // tokens of an item
 constexpr int kMoeMaxGroups = kMoeMaxExperts + kMoeMaxTokens * kMoeMaxTopk / kMoeGroup;
 constexpr int kRouteExperts = 4, kRouteTokens = 4;  // of a router unit
-constexpr int kRouteThreads = kConsumers * 32;
+constexpr int kRouteWarps = 8, kRouteThreads = kRouteWarps * 32;  // that compute logits
 
 struct MoeMaps {
     WeightMaps m[3];  // gate, up, down
@@ -207,7 +207,7 @@ __device__ void moe_router_alone(const MoeParams& P, double* logits, int* picks,
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const T* x = static_cast<const T*>(P.x);
     const T* r = static_cast<const T*>(P.router);
-    for (int pair = warp; pair < P.tokens * P.experts; pair += kConsumers) {
+    for (int pair = warp; pair < P.tokens * P.experts; pair += kRouteWarps) {
         const int t = pair / P.experts, e = pair % P.experts;
         double sum[8] = {0., 0., 0., 0., 0., 0., 0., 0.};
 #pragma unroll 4
@@ -225,7 +225,7 @@ __device__ void moe_router_alone(const MoeParams& P, double* logits, int* picks,
         if (lane == 0) logits[pair] = s;
     }
     named_barrier_sync(1, kRouteThreads);
-    for (int t = warp; t < P.tokens; t += kConsumers)
+    for (int t = warp; t < P.tokens; t += kRouteWarps)
         moe_select(P, logits + t * P.experts, picks + t * P.topk, shares + t * P.topk, lane);
 }
 
@@ -274,14 +274,14 @@ __device__ void moe_router(const MoeParams& P, double* scratch, int* flag) {
                 if (b >= nt) break;
 #pragma unroll
                 for (int d = 16; d > 0; d >>= 1) sum[a][b] += __shfl_xor_sync(0xFFFFFFFFu, sum[a][b], d);
-                if (lane == 0) scratch[(a * kRouteTokens + b) * kConsumers + warp] = sum[a][b];
+                if (lane == 0) scratch[(a * kRouteTokens + b) * kRouteWarps + warp] = sum[a][b];
             }
         named_barrier_sync(1, kRouteThreads);
         if (threadIdx.x < kRouteExperts * kRouteTokens) {
             const int a = threadIdx.x / kRouteTokens, b = threadIdx.x % kRouteTokens;
             if (e0 + a < P.experts && b < nt) {
                 double s = 0.0;
-                for (int j = 0; j < kConsumers; ++j) s += scratch[(a * kRouteTokens + b) * kConsumers + j];
+                for (int j = 0; j < kRouteWarps; ++j) s += scratch[(a * kRouteTokens + b) * kRouteWarps + j];
                 P.logits[size_t(t0 + b) * P.experts + e0 + a] = s;
             }
             __threadfence();
@@ -309,7 +309,7 @@ __device__ inline void moe_lists(const MoeParams& P, MoeRoute& R) {
     const int n = P.tokens * P.topk, t = threadIdx.x;
     if (t < kMoeMaxExperts) R.taken[t] = 0ull;
     __syncthreads();
-    for (int i = t; i < n; i += kStreamThreads) {
+    for (int i = t; i < n; i += blockDim.x) {
         atomicOr(&R.taken[R.pick[i]], 1ull << (i / P.topk));  // a token takes an expert once: the bits are its rows
         if (blockIdx.x == 0) {
             if (P.ids) P.ids[i] = R.pick[i];
@@ -353,7 +353,7 @@ __device__ inline void moe_lists(const MoeParams& P, MoeRoute& R) {
         }
     }
     __syncthreads();
-    for (int i = t; i < n; i += kStreamThreads) {
+    for (int i = t; i < n; i += blockDim.x) {
         const int e = R.pick[i], token = i / P.topk;
         const int row = R.row[e] + __popcll(R.taken[e] & ((1ull << token) - 1ull));
         R.token[row] = static_cast<unsigned char>(token);
@@ -363,27 +363,28 @@ __device__ inline void moe_lists(const MoeParams& P, MoeRoute& R) {
 }
 
 template <typename T, bool MX, int NT>
-__global__ void __launch_bounds__(kStreamThreads, 1)
+__global__ void __launch_bounds__(Stream<T, MX, NT>::kThreads, 1)
     moe_kernel(const __grid_constant__ MoeMaps maps, const MoeParams P) {
     using S = MoeShape<T, MX, NT>;
     using Pipe = typename S::Pipe;
+    constexpr int kConsumers = Pipe::kConsumers, kThreads = Pipe::kThreads;
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ double scratch[kRouteExperts * kRouteTokens * kConsumers];
+    __shared__ double scratch[kRouteExperts * kRouteTokens * kRouteWarps];
     __shared__ int flag, sums_ok;
     MoeRoute& R = *reinterpret_cast<MoeRoute*>(smem + S::kRoute);
     float* total = reinterpret_cast<float*>(smem + S::kTotal);  // [token][16 rows of y]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = gridDim.x, b = blockIdx.x;
     const auto l = Pipe::layout(smem_u32(smem), S::kStages);
-    if (threadIdx.x == kStreamThreads - 1) Pipe::init(l);
+    if (threadIdx.x == kThreads - 1) Pipe::init(l);
 
     if (P.tokens * P.experts <= kRouteAlone) {
-        if (warp < kConsumers) moe_router_alone<T>(P, scratch, R.pick, R.shares);
+        if (warp < kRouteWarps) moe_router_alone<T>(P, scratch, R.pick, R.shares);
         __syncthreads();
     } else {
-        if (warp < kConsumers) moe_router<T>(P, scratch, &flag);
+        if (warp < kRouteWarps) moe_router<T>(P, scratch, &flag);
         if (!moe_grid_barrier(P.sync, &flag)) return;
-        for (int i = threadIdx.x; i < P.tokens * P.topk; i += kStreamThreads) {
+        for (int i = threadIdx.x; i < P.tokens * P.topk; i += kThreads) {
             R.pick[i] = __ldcg(P.picks + i);
             R.shares[i] = __ldcg(P.shares + i);
         }
@@ -461,7 +462,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
             gate(std::true_type{});
         else
             gate(std::false_type{});
-        named_barrier_sync(2, kStreamThreads - 32);  // h is complete, or flag says that it will not be
+        named_barrier_sync(2, kThreads - 32);  // h is complete, or flag says that it will not be
         auto down = [&](auto fast) {
             typename Pipe::template Tokens<1, true> tokens;
             auto turn_to = [&](int d, int a) {
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
             flag = place.ok && moe_grid_arrive_wait(P.sync);
             __threadfence();
         }
-        named_barrier_sync(2, kStreamThreads - 32);
+        named_barrier_sync(2, kThreads - 32);
         T* y = static_cast<T*>(P.y);
         for (int d = d0; d < d1 && flag; ++d) {
             for (int c = thread; c < P.tokens * kTileRows; c += kEpilogueThreads) total[c] = 0.f;

@@ -262,11 +262,12 @@ struct ProjectShape {
 };
 
 template <typename T, int NT>
-__global__ void __launch_bounds__(kStreamThreads, 1)
+__global__ void __launch_bounds__(Stream<T, true, NT>::kThreads, 1)
     project_kernel(const __grid_constant__ WeightMaps maps, const ProjectParams P) {
     using Shape = ProjectShape<T, NT>;
     using Pipe = typename Shape::Pipe;
     extern __shared__ __align__(1024) unsigned char smem[];
+    constexpr int kConsumers = Pipe::kConsumers;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const auto l = Pipe::layout(smem_u32(smem), Shape::kStages);
     if (threadIdx.x == 0) Pipe::init(l);
@@ -348,7 +349,7 @@ int launch_project(ProjectParams P, cudaStream_t stream) {
     P.tiles = (P.rows + 31) / 32;
     P.items = int64_t(P.tiles) * ((P.tokens + NT * 8 - 1) / (NT * 8));
     const unsigned grid = unsigned(std::min<int64_t>(P.items, sms));
-    return launch_ex(kernel, grid, kStreamThreads, Shape::kSmem, stream, false, maps, P);
+    return launch_ex(kernel, grid, Shape::Pipe::kThreads, Shape::kSmem, stream, false, maps, P);
 }
 
 template <typename T>

@@ -173,14 +173,15 @@ struct Tiles {
     int rows[NM];
 };
 
-constexpr int kConsumers = 8;
 constexpr int kEpilogueThreads = 96;
-constexpr int kStreamThreads = (kConsumers + 4) * 32;  // consumers, producer, epilogue
 constexpr int kPartPitch = 17;
 constexpr int kRingTarget = 160 * 1024;
 
 template <typename T, bool MX, int NT>
 struct Stream {
+    // Decoding four-bit codes for few tokens keeps the schedulers busy only with four warps each.
+    static constexpr int kConsumers = MX && NT <= 2 ? 16 : 8;
+    static constexpr int kThreads = (kConsumers + 4) * 32;  // consumers, producer, epilogue
     // A stage: 2 tiles of 16 rows by 1 KB, or one tile by 2 KB. With maps: 128 bytes of 16 rows
     // after another (kBox), swizzled by the copy; scales 64 bytes of 16 rows after another.
     // Without: row after row, at pitches that leave 16 bytes for a shifted row.
@@ -421,7 +422,8 @@ struct Stream {
     struct Tokens {
         static constexpr int kRows = SPLIT ? 2 * NT : NT;
         static constexpr int kSteps = Shape<NM>::kUnits / kConsumers * kSub;  // sub-steps of a warp in a full stage
-        static constexpr int kGroup = kRows >= 8 ? 1 : kRows >= 4 ? 2 : kSteps < 4 ? kSteps : 4;
+        static constexpr int kMost = kConsumers == 16 ? 4 / kRows : 8 / kRows;  // that the registers hold
+        static constexpr int kGroup = kMost < 1 ? 1 : kMost > 4 ? (kSteps < 4 ? kSteps : 4) : kMost < kSteps ? kMost : kSteps;
         const T* x[kRows];  // this lane's rows
         int count;          // tokens; 0: no item
         uint4 ahead[kGroup][kRows];
