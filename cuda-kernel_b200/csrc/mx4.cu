@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "host.h"
+#include "project.h"
 #include "stream.cuh"
 
 namespace swb {
@@ -239,21 +240,6 @@ int convert(int type, const void* from, void* to, int64_t pitch, const void* cod
 }
 
 // ---------------------------------------------------------------- product
-struct ProjectParams {
-    const unsigned char* w;
-    const unsigned char* s;
-    const void* x;
-    const void* bias;
-    const void* residual;
-    void* out;
-    int64_t x_pitch, tokens;
-    int rows, cols;
-    int tiles;       // of 32 rows
-    int64_t items;   // tiles x groups of NT * 8 tokens
-    bool x_aligned, fast, deep;  // 16-byte pieces of x; make_weight_maps
-    bool half_out;
-};
-
 template <typename T, int NT>
 struct ProjectShape {
     using Pipe = Stream<T, true, NT>;
@@ -428,6 +414,7 @@ int swb_mx4_project(int type, const void* codes, const void* scales, const void*
     P.half_out = half;
     P.x_aligned = cols % 8 == 0 && x_pitch % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
     auto s = static_cast<cudaStream_t>(stream);
+    if (project_wide_takes(P)) return project_wide(type, P, s);
     return type == SWB_F16 ? dispatch_project<__half>(P, s) : dispatch_project<__nv_bfloat16>(P, s);
 }
 

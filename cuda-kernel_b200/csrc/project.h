@@ -1,0 +1,29 @@
+// Arguments of the product of a four-bit matrix with 16-bit tokens, shared by its kernels.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace swb {
+
+struct ProjectParams {
+    const unsigned char* w;
+    const unsigned char* s;
+    const void* x;
+    const void* bias;
+    const void* residual;
+    void* out;
+    int64_t x_pitch, tokens;
+    int rows, cols;
+    int tiles;       // of rows
+    int64_t items;   // tiles x groups of tokens
+    bool x_aligned, fast, deep;  // 16-byte pieces of x; make_weight_maps
+    bool half_out;
+};
+
+// The tensor-core kernel (mx4_wide.cu): takes codes whose rows are whole 64 bytes, on 32 bytes.
+bool project_wide_takes(const ProjectParams& P);
+int project_wide(int type, ProjectParams P, cudaStream_t stream);
+
+}  // namespace swb

@@ -46,6 +46,20 @@ inline int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t pi
     return r == CUDA_SUCCESS ? SWB_OK : fail(SWB_E_CUDA, "tensor map");
 }
 
+// Rows of `cols` elements, `pitch` bytes apart, in boxes of box_rows by box_cols (128 bytes of shared
+// memory, swizzled over as many); zero beyond the matrix.
+inline int make_typed_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t cols, int64_t rows,
+                          int64_t pitch, int box_cols, int box_rows) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return fail(SWB_E_UNSUPPORTED, "the driver has no tensor maps");
+    const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)}, strides[1] = {cuuint64_t(pitch)};
+    const cuuint32_t box[2] = {cuuint32_t(box_cols), cuuint32_t(box_rows)}, one[2] = {1, 1};
+    const CUresult r = encode(map, type, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? SWB_OK : fail(SWB_E_CUDA, "tensor map");
+}
+
 // The maps of a streamed weight tensor (Stream::produce), where its rows allow them.
 struct WeightMaps {
     CUtensorMap w, s;

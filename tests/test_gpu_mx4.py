@@ -4,12 +4,16 @@ Rounding and reading back are exact (whole codes, power-of-two scales), so they 
 bit for bit; reading back as fp16 rounds what fp16 cannot hold, and is compared with numpy's
 rounding of the exact value.
 
-Products with 16-bit tokens: a value is a sum of exact products. Inside a block the tensor core adds 32 of them
-in two instructions, each of which may lose 17 2^-24 relative to the magnitudes it adds
-(16 products and the running sum aligned to the largest, truncated); a block's sum is then added
-in fp32, one rounding (2^-24) a block, and the eight warps' parts, bias and residual add at
-most ten more. So |out - exact| <= (34 + K/32 + 10) 2^-24 sum|w x| (+ |bias| + |residual| terms in
-that sum) + half a step of the output type (eps/2 relative, or half of the smallest subnormal).
+Products with 16-bit tokens sum exact products in fp32. One tensor-core step of k products and the
+running sum may lose (k + 2) 2^-24 of the magnitudes it adds (aligned to the largest, truncated);
+k is 16 or 32, so K values lose at most 1.125 K 2^-24 of sum|w x|, and the parts of clusters or
+warps, bias and residual add at most 76 roundings more. Where a token is split into e4m3 pieces, a
+value within 13 binades of its block's largest is exact, and another is off by at most half the
+last piece's smallest step: 2^-10 of the piece's unit, which is 2^10 (three pieces, fp16) or
+2^5 (two, bf16) below the first's, where the largest is at least 2^7: 2^-27 or 2^-22 of it.
+So |out - exact| <= (1.125 K + 76) 2^-24 sum|w x| + d sum over blocks of max|x| sum|w| (+ |bias| +
+|residual| in the first sum) + half a step of the output type (eps/2 relative, or half of the
+smallest subnormal).
 
 Products of two four-bit matrices: one tensor-core step adds 64 exact products to the running sum
 and may lose 66 2^-24 of the magnitudes it adds; the cluster's eight parts, bias and residual
@@ -112,8 +116,13 @@ def test_quantize_spaced_rows_three_dims_and_bounds():
     assert empty[0].shape == (0, 32)
 
 
-def project_bound(x, w, extra, rel=0.0):
-    return (44 + x.shape[1] / 32) * 2.0 ** -24 * (np.abs(x) @ np.abs(w).T + extra)
+def project_bound(x, w, extra, dtype):
+    n = -(-x.shape[1] // 32)
+    pad = ((0, 0), (0, n * 32 - x.shape[1]))
+    largest = np.abs(np.pad(x, pad)).reshape(x.shape[0], n, 32).max(2)
+    weights = np.abs(np.pad(w, pad)).reshape(w.shape[0], n, 32).sum(2)
+    pieces = (2.0 ** -27 if dtype == torch.float16 else 2.0 ** -22) * (largest @ weights.T)
+    return (1.125 * x.shape[1] + 76) * 2.0 ** -24 * (np.abs(x) @ np.abs(w).T + extra) + pieces
 
 
 def half_step(v, dtype):
@@ -122,13 +131,14 @@ def half_step(v, dtype):
 
 
 def check_product(got, x, w, bias, residual, dtype):
+    kind, x = x.dtype, np64(x)
     want = x @ w.T
     extra = np.zeros_like(want)
     for t in (bias, residual):
         if t is not None:
             want = want + t
             extra = extra + np.abs(t)
-    bound = project_bound(x, w, extra)
+    bound = project_bound(x, w, extra, kind)
     err = np.abs(np64(got) - want)
     limit = bound + half_step(np.abs(want) + bound, dtype)
     assert np.isfinite(np64(got)).all() and (err <= limit).all(), float((err / limit).max())
@@ -137,18 +147,20 @@ def check_product(got, x, w, bias, residual, dtype):
 @pytest.mark.parametrize("kind", ["fp16", "bf16"])
 @pytest.mark.parametrize("tokens,rows,cols", [
     (1, 1, 1), (1, 32, 128), (1, 33, 31), (2, 16, 32), (3, 65, 130), (8, 48, 1024), (9, 100, 257), (16, 31, 160),
-    (17, 512, 96), (33, 40, 72), (64, 64, 544), (65, 17, 33), (130, 96, 1030), (1, 5632, 2048)])
+    (17, 512, 96), (33, 40, 72), (64, 64, 544), (65, 17, 33), (130, 96, 1030), (1, 5632, 2048),
+    (3, 200, 128), (16, 129, 384), (20, 300, 512), (33, 64, 256), (64, 260, 640), (100, 130, 1024), (513, 65, 128),
+    (5, 4100, 2048), (2, 128, 100), (12, 192, 4064)])
 def test_project(kind, tokens, rows, cols):
     dtype = TYPES[kind]
     codes, scales, w = packed((rows, cols), rows + cols, cols ** -0.5)
     x = sample((tokens, cols), dtype, tokens)
     bias, residual = sample((rows,), dtype, 3, 0.1), sample((tokens, rows), dtype, 4)
-    check_product(S.mx4_project(x, codes, scales), np64(x), w, None, None, dtype)
-    check_product(S.mx4_project(x, codes, scales, bias, residual, torch.float32), np64(x), w, np64(bias), np64(residual),
+    check_product(S.mx4_project(x, codes, scales), x, w, None, None, dtype)
+    check_product(S.mx4_project(x, codes, scales, bias, residual, torch.float32), x, w, np64(bias), np64(residual),
                   torch.float32)
     out = residual.clone()
     S.mx4_project_out(x, codes, scales, out, bias, out)  # in place
-    check_product(out, np64(x), w, np64(bias), np64(residual), dtype)
+    check_product(out, x, w, np64(bias), np64(residual), dtype)
 
 
 def test_project_views_and_bounds():
@@ -162,7 +174,7 @@ def test_project_views_and_bounds():
         for s in (scales, odd):
             buf = torch.full((7, 40), 9.0, dtype=torch.float32, device="cuda")
             S.mx4_project_out(x, codes, s, buf[1:6])
-            check_product(buf[1:6], np64(x), w, None, None, torch.float32)
+            check_product(buf[1:6], x, w, None, None, torch.float32)
             assert (buf[0] == 9).all() and (buf[6] == 9).all()
 
 
@@ -182,7 +194,7 @@ def test_project_special_values():
         want = np64(x) @ w.T
         assert np.isnan(got[:, 1]).all()
         keep = [i for i in range(48) if i != 1]
-        bound = project_bound(np64(x), w[keep], 0)
+        bound = project_bound(np64(x), w[keep], 0, dtype)
         # the smallest scale's products are subnormal in fp32: half of its smallest step each
         assert (np.abs(got[:, keep] - want[:, keep]) <= bound + half_step(want[:, keep], torch.float32) + cols * 2.0 ** -149).all()
         x[2, 5], x[3, 7] = float("inf"), float("nan")
@@ -190,6 +202,21 @@ def test_project_special_values():
         rest = S.mx4_project(x[:2].contiguous(), codes.cuda(), scales.cuda(), dtype=torch.float32)
         assert torch.equal(got[:2].nan_to_num(), rest.nan_to_num()) and torch.isnan(got[3]).all()
         assert not torch.isfinite(got[2]).any()
+
+
+def test_project_far_binades():
+    """Tokens whose values span far more binades than a piece holds, block by block."""
+    codes, scales, w = packed((70, 256), 11, 0.1)
+    for dtype, low in ((torch.float16, -14), (torch.bfloat16, -100)):
+        g = torch.Generator().manual_seed(5)
+        e = torch.randint(low, 12, (6, 256), generator=g).double()
+        x = (torch.randn((6, 256), generator=g).double() * 2.0 ** e).to(dtype).cuda()
+        x[1, 32:64] = 0
+        x[2] = torch.finfo(dtype).max / 1e4
+        x[3] = torch.finfo(dtype).tiny
+        for out in (torch.float32, torch.bfloat16):
+            check_product(S.mx4_project(x, codes, scales, dtype=out if out == torch.float32 or dtype == out else None), x, w,
+                          None, None, torch.float32 if out == torch.float32 else dtype)
 
 
 def test_project_refusals():
