@@ -5,6 +5,7 @@
 #include <cstring>
 
 #include "host.h"
+#include "moe_wide.h"
 
 namespace swb {
 
@@ -150,6 +151,7 @@ int swb_moe(int type, unsigned flags, const void* x, int64_t x_pitch, const void
     P.x_aligned = hidden % 8 == 0 && x_pitch % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
     P.router_aligned = hidden % 8 == 0 && reinterpret_cast<uintptr_t>(router) % 16 == 0;
     auto s = static_cast<cudaStream_t>(stream);
+    if (moe_wide_takes(P, mx)) return moe_wide(type, mx, P, s);
     if (type == SWB_F16) return mx ? dispatch_moe<__half, true>(P, s) : dispatch_moe<__half, false>(P, s);
     return mx ? dispatch_moe<__nv_bfloat16, true>(P, s) : dispatch_moe<__nv_bfloat16, false>(P, s);
 }

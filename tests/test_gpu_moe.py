@@ -4,6 +4,8 @@ Bound on y (mx4_reference.moe): fp32 sums of K products lose at most gamma(K) = 
 to the sum of magnitudes for 16-bit weights (each mma step of 16 may truncate 17 2^-24 of what it
 adds: 1.07 K 2^-24 in all, and the parts of up to eight warps are added once more), less for
 four-bit ones; h is rounded once to the layer's type (eps/2 relative) and y once more.
+For more than eight tokens h goes on as three e4m3 pieces (four-bit weights) or two values of the
+type, and tokens as pieces too: within 2^-13, far below the type's rounding that the bound has for h.
 Inputs have few bits, so that the 64-bit logits of kernel and plain form are the same number
 and ties are real ties.
 """
@@ -82,7 +84,8 @@ def check(d, v, topk, renormalize, got):
 @pytest.mark.parametrize("tokens,experts,topk,hidden,inter", [
     (1, 1, 1, 1, 1), (1, 2, 1, 32, 16), (1, 8, 2, 64, 96), (2, 4, 4, 33, 31), (3, 5, 2, 130, 70), (8, 8, 2, 128, 160),
     (9, 16, 3, 64, 40), (16, 12, 4, 72, 100), (17, 3, 2, 96, 48), (33, 40, 8, 64, 24), (64, 8, 2, 96, 129),
-    (64, 256, 16, 32, 16), (1, 8, 2, 512, 1376)])
+    (64, 256, 16, 32, 16), (1, 8, 2, 512, 1376), (9, 4, 2, 128, 128), (12, 8, 3, 256, 384), (33, 4, 2, 384, 256),
+    (64, 2, 2, 256, 640), (20, 16, 4, 640, 128), (64, 32, 8, 128, 200), (40, 3, 1, 136, 1032)])
 def test_layer(kind, four_bit, tokens, experts, topk, hidden, inter):
     d, v = layer(tokens + experts, tokens, experts, hidden, inter, TYPES[kind], four_bit)
     for renormalize in (True, False):
@@ -100,6 +103,19 @@ def test_all_tokens_to_one_expert_and_ties():
     got = call(d, 1)
     assert got[1].tolist() == [[4]] * 20
     check(d, v, 1, True, got)
+
+
+@pytest.mark.parametrize("tokens,hidden,four_bit", [(4, 64, False), (4, 64, True), (12, 128, False), (12, 128, True)])
+def test_non_finite_tokens(tokens, hidden, four_bit):
+    """A NaN or infinite value makes its token NaN or infinite and leaves the others as they are."""
+    d, v = layer(12, tokens, 5, hidden, 128, torch.float16, four_bit)
+    clean = call(d, 2)
+    d["x"][1, 3], d["x"][3, 40] = float("nan"), float("inf")
+    y, ids, w = call(d, 2)
+    assert not torch.isfinite(y[1]).any() and not torch.isfinite(y[3]).any()
+    for t in [i for i in range(tokens) if i not in (1, 3)]:
+        # rows of h move with the others' selections, sums do not
+        assert torch.equal(y[t], clean[0][t]) and torch.equal(ids[t], clean[1][t]) and torch.equal(w[t], clean[2][t])
 
 
 def test_non_finite_logits():
