@@ -51,6 +51,7 @@ struct GateWork {
     int blocks, cols;
     int64_t rows_a;
     bool x_aligned;
+    int halves;
     const MoeParams* P;
     const MoeRoute* R;
     int tiles, steps, g0, g1;
@@ -129,6 +130,7 @@ struct DownWork {
     int blocks, cols;
     int64_t rows_a;
     bool x_aligned;
+    int halves;
     const MoeParams* P;
     const MoeRoute* R;
     int64_t row0;    // of y
@@ -174,10 +176,11 @@ struct DownShape {
 };
 
 template <typename T, bool MX>
-__global__ void __launch_bounds__(kWideThreads, 1)
+__global__ void __launch_bounds__(Wide<GateWork<T, MX>>::kThreads, 1)
     moe_gate_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ MoeParams P) {
     using S = GateShape<T, MX>;
     using Work = GateWork<T, MX>;
+    constexpr int kWideThreads = S::Pipe::kThreads;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ typename S::Pipe::Shared sh;
     __shared__ double scratch[kRouteExperts * kRouteTokens * kRouteWarps];
@@ -202,6 +205,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         work.cols = P.hidden;
         work.rows_a = int64_t(P.experts) * P.inter;
         work.x_aligned = P.x_aligned != 0;
+        work.halves = 2;
         work.P = &P;
         work.R = &R;
         work.tiles = (P.inter + kWideHalf - 1) / kWideHalf;
@@ -217,11 +221,12 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 }
 
 template <typename T, bool MX>
-__global__ void __launch_bounds__(kWideThreads, 1)
+__global__ void __launch_bounds__(Wide<DownWork<T, MX>>::kThreads, 1)
     moe_down_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_h,
-                    const __grid_constant__ MoeParams P, int splits) {
+                    const __grid_constant__ MoeParams P, int splits, int halves) {
     using S = DownShape<T, MX>;
     using Work = DownWork<T, MX>;
+    constexpr int kWideThreads = S::Pipe::kThreads;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ typename S::Pipe::Shared sh;
     MoeRoute& R = *reinterpret_cast<MoeRoute*>(smem + S::kRoute);
@@ -243,9 +248,11 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     work.cols = P.inter;
     work.rows_a = int64_t(P.experts) * P.hidden;
     work.x_aligned = true;
+    work.halves = halves;
     work.P = &P;
     work.R = &R;
-    work.row0 = int64_t(blockIdx.x / splits) * kWideM;
+    const int tile_rows = halves * kWideHalf;
+    work.row0 = int64_t(blockIdx.x / splits) * tile_rows;
     work.steps = (P.inter + S::Pipe::kValues - 1) / S::Pipe::kValues;
     const long long all = (long long)R.groups * work.steps;
     work.f0 = int(rank * all / splits);
@@ -259,7 +266,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     if (!sh.failed) {
         for (int i = rank * kWideThreads + threadIdx.x; i < P.tokens * kWideM; i += splits * kWideThreads) {
             const int64_t row = work.row0 + i % kWideM;
-            if (row >= P.hidden) continue;
+            if (i % kWideM >= tile_rows || row >= P.hidden) continue;
             float v = 0.f;
             for (int j = 0; j < splits; ++j) {
                 uint32_t remote;
@@ -296,14 +303,18 @@ int launch_moe_wide(const MoeParams& P, cudaStream_t stream) {
                                 rows, int64_t(P.h_pitch) * (MX ? 1 : 2), MX ? 128 : 64, 16))
         return rc;
     // every CTA resident at once: the cooperative launch makes the runtime check it
-    if (int rc = launch_ex(gate, unsigned(sms), kWideThreads, G::kSmem, stream, true, maps, P)) return rc;
+    if (int rc = launch_ex(gate, unsigned(sms), G::Pipe::kThreads, G::kSmem, stream, true, maps, P)) return rc;
 
-    const int tiles = (P.hidden + kWideM - 1) / kWideM;
+    // 128 rows of y a cluster, or 64 where that leaves SMs without work. Clusters of four: the SMs
+    // of a GPC hold few of eight (16 clusters of eight took two waves, 113 us for 309 MB).
+    constexpr int kMostSplits = 4;
+    const int halves = (P.hidden + kWideM - 1) / kWideM * kMostSplits > sms / 2 ? 2 : 1;
+    const int tiles = (P.hidden + halves * kWideHalf - 1) / (halves * kWideHalf);
     int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= sms) splits *= 2;
+    while (splits < kMostSplits && tiles * splits * 2 <= sms) splits *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(tiles * splits));
-    cfg.blockDim = dim3(kWideThreads);
+    cfg.blockDim = dim3(D::Pipe::kThreads);
     cfg.dynamicSmemBytes = D::kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -315,7 +326,7 @@ int launch_moe_wide(const MoeParams& P, cudaStream_t stream) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, down, map_w, map_h, P, splits);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, down, map_w, map_h, P, splits, halves);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         return fail(SWB_E_CUDA, cudaGetErrorString(e));

@@ -42,6 +42,7 @@ struct ProjectWork {
     bool x_aligned;
     const T* x;
     int64_t x_pitch;
+    int halves;
     WideItem only;
     int64_t token0;
     uint32_t part;  // [token][kWidePartPitch]
@@ -67,10 +68,11 @@ struct ProjectWide {
 };
 
 template <typename T, int TOK>
-__global__ void __launch_bounds__(kWideThreads, ProjectWork<T, TOK>::kPerSm)
+__global__ void __launch_bounds__(Wide<ProjectWork<T, TOK>>::kThreads, ProjectWork<T, TOK>::kPerSm)
     project_wide_kernel(const __grid_constant__ CUtensorMap map, const ProjectParams P, int splits, int steps) {
     using Work = ProjectWork<T, TOK>;
     using Pipe = Wide<Work>;
+    constexpr int kWideThreads = Pipe::kThreads;
     extern __shared__ unsigned char raw[];
     __shared__ typename Pipe::Shared sh;
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -81,6 +83,7 @@ __global__ void __launch_bounds__(kWideThreads, ProjectWork<T, TOK>::kPerSm)
     Work work;
     work.sa[0] = work.sa[1] = P.s;
     work.sb = nullptr;
+    work.halves = 2;
     work.blocks = int(mx_blocks(P.cols));
     work.cols = P.cols;
     work.rows_a = P.rows;
@@ -150,7 +153,7 @@ int launch_wide(ProjectParams P, cudaStream_t stream) {
     if (P.items * splits > 0x7FFFFFFF) return fail(SWB_E_SHAPE);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(P.items * splits));
-    cfg.blockDim = dim3(kWideThreads);
+    cfg.blockDim = dim3(Shape::Pipe::kThreads);
     cfg.dynamicSmemBytes = Shape::kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

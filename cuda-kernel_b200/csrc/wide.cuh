@@ -10,10 +10,10 @@
 // 2^-27 of the largest beyond), two hold 9 (bf16). A piece is a column of its own; the epilogue
 // adds a token's columns. Every product is exact and the sums are the tensor core's fp32.
 //
-// Roles of a CTA (10 warps), through a ring of stages of 128 bytes of every row:
+// Roles of a CTA (10 or 14 warps), through a ring of stages of 128 bytes of every row:
 //   copies     one thread, TMA: two halves of 64 rows of W (gate and up rows, or neighbours), and
 //              the tokens where they lie prepared in memory
-//   loaders    four warps: tokens from their rows (gathered, split into pieces), scale bytes of
+//   loaders    four warps, or eight that split tokens: tokens from their rows (gathered, split into pieces), scale bytes of
 //              both sides into the 32 x 16-byte blocks that tcgen05.cp spreads over TMEM
 //   products   one thread
 //   epilogue   four warps, a TMEM quadrant each
@@ -27,8 +27,7 @@ namespace swb {
 constexpr int kWideM = 128, kWideHalf = 64;
 constexpr int kWideRowBytes = 128;                     // of a row in a stage, in shared memory
 constexpr int kWideA = kWideM * kWideRowBytes;
-constexpr int kWideEpilogue = 4, kWideLoaders = 4;     // warps
-constexpr int kWideThreads = (kWideEpilogue + kWideLoaders + 2) * 32;
+constexpr int kWideEpilogue = 4;                       // warps
 constexpr int kWidePartPitch = kWideM + 1;             // floats of a token's column
 
 // ------------------------------------------------------------ tokens in e4m3 pieces
@@ -67,6 +66,66 @@ __device__ __forceinline__ void split_pieces(float (&f)[8], uint32_t scale, uint
     }
 }
 
+// Eight values of a token (`raw`) -> pieces; the four lanes of a quad hold a block and agree on
+// the scale byte, which is returned. bf16 goes through fp32. fp16 stays packed: what a piece leaves
+// is exact in fp16 (at most 11 bits), and so are the scalings but for values 2^-32 below the
+// block's largest; the first factor is at most 2^15, which holds every bit of smaller blocks too.
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+    v = max(v, __shfl_xor_sync(0xFFFFFFFFu, v, 1));
+    return max(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
+}
+template <int PIECES>
+__device__ __forceinline__ uint32_t split_token(const uint4& raw, uint2 (&out)[PIECES], __nv_bfloat16) {
+    float f[8];
+    uint32_t top = 0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        f[e] = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(&raw)[e]);
+        top = max(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+    }
+    const uint32_t scale = piece_scale(quad_max(top));
+    split_pieces<PIECES>(f, scale, out);
+    return scale;
+}
+template <int PIECES>
+__device__ __forceinline__ uint32_t split_token(const uint4& raw, uint2 (&out)[PIECES], __half) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    // magnitudes as integers order like the values; NaN and infinity lie above all
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = __vmaxu2(top, w[i] & 0x7FFF7FFFu);
+    top = quad_max(max(top & 0xFFFFu, top >> 16));
+    const int e = int(top >> 10) - 15;                    // floor(log2) of the largest (or less: subnormal)
+    const int up = top >= 0x7C00u ? 0 : min(7 - e, 15);   // it goes to [2^7, 2^8)
+    const uint32_t factor = uint32_t(up + 15) << 10 | uint32_t(up + 15) << 26;
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(v[i]) : "r"(w[i]), "r"(factor));
+    if (top >= 0x7C00u) {  // a block with a NaN or an infinity: those become NaN
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if ((v[i] & 0x7C00u) == 0x7C00u) v[i] |= 0x7FFFu;
+            if ((v[i] & 0x7C000000u) == 0x7C000000u) v[i] |= 0x7FFF0000u;
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        uint16_t b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(b[i]) : "r"(v[i]));
+            if (p + 1 < PIECES) {
+                uint32_t back;
+                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(b[i]));
+                asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(v[i]) : "r"(back));
+                asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(v[i]) : "r"(0x50005000u));  // times 32
+            }
+        }
+        out[p] = make_uint2(uint32_t(b[0]) | uint32_t(b[1]) << 16, uint32_t(b[2]) | uint32_t(b[3]) << 16);
+    }
+    return uint32_t(127 - up);
+}
+
 // Where row r's 16-byte piece c lies in a tile of 128-byte rows as the 128-byte swizzle has it.
 __device__ __forceinline__ uint32_t swizzled(int r, int c) { return uint32_t(r * 128 + ((c ^ r) & 7) * 16); }
 // Byte of row r, block b of 128 values, in its 512-byte block of scales.
@@ -86,7 +145,7 @@ struct WideItem {
 //   types      T; kMx; kPieces; kTok (tokens of an item, a multiple of 16); kLoad (tokens by the
 //              loaders; else rows `first * kPieces` on of a tensor map); kAccs; kStages; kPerSm
 //   item(i, it) -> false past the last one;  token(it, n): row of token n (kLoad)
-//   scales of W: sa[2], blocks, rows_a;  of tokens that lie prepared: sb
+//   halves: 1 or 2 of 64 rows;  scales of W: sa[2], blocks, rows_a;  of tokens that lie prepared: sb
 //   begin(it) / value(it, n, row, v) / end(it): epilogue threads, by their row
 template <typename W>
 struct Wide {
@@ -103,6 +162,8 @@ struct Wide {
     static constexpr int kValues = kMx ? 128 : 64;   // of a row in a stage
     static constexpr int kRowSource = kMx ? 64 : 128;  // their bytes in W
     static constexpr bool kLoaders = W::kLoad || kMx;
+    static constexpr int kWideLoaders = kMx && W::kLoad ? 8 : 4;  // warps
+    static constexpr int kThreads = (kWideEpilogue + kWideLoaders + 2) * 32;
     static_assert(kUsed <= 512 && kColumns * W::kPerSm <= 512, "TMEM columns");
     static constexpr size_t kRing = size_t(W::kStages) * kStage;
 
@@ -166,9 +227,9 @@ struct Wide {
                             break;
                         }
                         const uint32_t bar = smem_u32(sh.full + s), at = base + s * kStage;
-                        mbar_arrive_expect_tx(bar, kWideM * kRowSource + (W::kLoad ? 0 : n * kWideRowBytes));
+                        mbar_arrive_expect_tx(bar, work.halves * kWideHalf * kRowSource + (W::kLoad ? 0 : n * kWideRowBytes));
                         tma_load_2d(at, map0, k * kValues, int(it.row[0]), bar, policy);
-                        tma_load_2d(at + kWideA / 2, map1, k * kValues, int(it.row[1]), bar, policy);
+                        if (work.halves == 2) tma_load_2d(at + kWideA / 2, map1, k * kValues, int(it.row[1]), bar, policy);
                         if (!W::kLoad) {
                             for (int r = 0; r < n; r += 16)
                                 tma_load_2d(at + kWideA + r * kWideRowBytes, map_b, k * kValues, it.first * W::kPieces + r, bar);
@@ -280,17 +341,17 @@ struct Wide {
 #pragma unroll
                 for (int u = 0; u < kTurns; ++u) x[u] = work.token(it, min(n0 + u * kStride, it.count - 1));
             }
-            if constexpr (kMx) {
+            if (kMx && t < kWideM) {
                 const int half = t / kWideHalf;
                 const int64_t r = (half ? it.row[1] : it.row[0]) + t % kWideHalf;
-                if (r < work.rows_a) row_a = (half ? work.sa[1] : work.sa[0]) + r * work.blocks;
+                if (r < work.rows_a && half < work.halves) row_a = (half ? work.sa[1] : work.sa[0]) + r * work.blocks;
 #pragma unroll
                 for (int u = 0; u < kRowsB; ++u) {
                     const int b = t + 128 * u;
                     row_b[u] = !W::kLoad && b < it.count * W::kPieces ? work.sb + int64_t(it.first * W::kPieces + b) * work.blocks : nullptr;
                 }
             }
-            uint4 xv[kTurns], win_a = {}, win_b[kRowsB] = {};
+            uint4 xv[kTurns];
             auto load_x = [&](int k) {
                 if constexpr (W::kLoad) {
 #pragma unroll
@@ -301,35 +362,39 @@ struct Wide {
                     }
                 }
             };
-            auto load_windows = [&](int k) {  // 16 scale bytes: stages k & ~3 to k | 3
+            // Windows of 16 scale bytes, four stages each, two windows ahead: W's come from DRAM.
+            uint4 win_a[3] = {}, win_b[3][kRowsB] = {};
+            auto load_windows = [&](int w, int k) {
                 if constexpr (kMx) {
-                    win_a = row_a ? load_scales(row_a, k / 4 * 16, work.blocks) : make_uint4(0u, 0u, 0u, 0u);
+                    const bool have = k < it.s1;
+                    win_a[w] = row_a && have ? load_scales(row_a, k / 4 * 16, work.blocks) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
                     for (int u = 0; u < kRowsB; ++u)
-                        win_b[u] = row_b[u] ? load_scales(row_b[u], k / 4 * 16, work.blocks) : make_uint4(0u, 0u, 0u, 0u);
+                        win_b[w][u] = row_b[u] && have ? load_scales(row_b[u], k / 4 * 16, work.blocks) : make_uint4(0u, 0u, 0u, 0u);
                 }
             };
             load_x(it.s0);
-            load_windows(it.s0);
-            uint4 now_a = {}, now_b[kRowsB] = {};
+            load_windows(0, it.s0);
+            load_windows(1, (it.s0 | 3) + 1);
+            load_windows(2, (it.s0 | 3) + 5);
             for (int k = it.s0; k < it.s1; ++k) {
                 uint4 now[kTurns];
 #pragma unroll
                 for (int u = 0; u < kTurns; ++u) now[u] = xv[u];
-                if (kMx && (k == it.s0 || k % 4 == 0)) {
-                    now_a = win_a;
+                if (kMx && k > it.s0 && k % 4 == 0) {
+                    win_a[0] = win_a[1], win_a[1] = win_a[2];
 #pragma unroll
-                    for (int u = 0; u < kRowsB; ++u) now_b[u] = win_b[u];
-                    if ((k | 3) + 1 < it.s1) load_windows((k | 3) + 1);
+                    for (int u = 0; u < kRowsB; ++u) win_b[0][u] = win_b[1][u], win_b[1][u] = win_b[2][u];
+                    load_windows(2, k + 8);
                 }
                 if (k + 1 < it.s1) load_x(k + 1);
                 if (issued >= W::kStages && !mbar_wait_warp(smem_u32(sh.empty + s), ph ^ 1u)) return false;
                 const uint32_t b = base + s * kStage + kWideA, sc = b + kBytesB;
-                if constexpr (kMx) sts32(sc + scale_place(t), word_of(now_a, k));
+                if (kMx && t < kWideM) sts32(sc + scale_place(t), word_of(win_a[0], k));
                 if constexpr (kMx && !W::kLoad) {
 #pragma unroll
                     for (int u = 0; u < kRowsB; ++u)
-                        if (t + 128 * u < kN) sts32(sc + kScaleBlock + scale_place(t + 128 * u), word_of(now_b[u], k));
+                        if (t + 128 * u < kN) sts32(sc + kScaleBlock + scale_place(t + 128 * u), word_of(win_b[0][u], k));
                 }
                 if constexpr (W::kLoad) {
 #pragma unroll
@@ -340,18 +405,8 @@ struct Wide {
                             if (n < it.count)
                                 asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(b + swizzled(n, j)), "r"(now[u].x), "r"(now[u].y), "r"(now[u].z), "r"(now[u].w) : "memory");
                         } else {
-                            float f[8];
-                            uint32_t top = 0u;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                f[e] = Num<T>::to_float(reinterpret_cast<const T*>(now + u)[e]);
-                                top = max(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
-                            }
-                            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                            const uint32_t scale = piece_scale(top);
                             uint2 piece[W::kPieces];
-                            split_pieces<W::kPieces>(f, scale, piece);
+                            const uint32_t scale = split_token<W::kPieces>(now[u], piece, T());
                             if (n < it.count) {
 #pragma unroll
                                 for (int p = 0; p < W::kPieces; ++p) {
