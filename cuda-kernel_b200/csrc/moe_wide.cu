@@ -44,7 +44,8 @@ struct GateWork {
     static constexpr bool kMx = MX, kLoad = true;
     static constexpr int kPieces = MX ? (std::is_same<T, __half>::value ? 3 : 2) : 1;
     static constexpr int kTok = kMoeGroup, kAccs = 2, kPerSm = 1;
-    static constexpr int kStages = MX ? 6 : 8;
+    static constexpr int kStages = MX ? 3 : 8, kRaw = 4, kTokenStages = MX ? 5 : 6;
+    static constexpr int kSplitters = MX ? 5 : 4, kGroupWarps = 1;
 
     const unsigned char* sa[2];
     const unsigned char* sb;
@@ -123,7 +124,8 @@ struct DownWork {
     static constexpr bool kMx = MX, kLoad = false;
     static constexpr int kPieces = h_pieces(MX);
     static constexpr int kTok = kMoeGroup, kAccs = 2, kPerSm = 1;
-    static constexpr int kStages = MX ? 6 : 7;
+    static constexpr int kStages = MX ? 3 : 7, kRaw = 4, kTokenStages = MX ? 4 : 6;
+    static constexpr int kSplitters = 4, kGroupWarps = 1;
 
     const unsigned char* sa[2];
     const unsigned char* sb;

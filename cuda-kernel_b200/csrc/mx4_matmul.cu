@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == kEpilogueWarps + kScaleWarps) {
         // ------------------------------------------------------- codes, by TMA
-        if (lane == 0) {
+        if (elect_one()) {
             int s = 0, issued = 0;
             uint32_t ph = 0;
             bool ok = true;
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == kEpilogueWarps + kScaleWarps + 1) {
         // ------------------------------------------------------- products
-        if (lane == 0) {
+        if (elect_one()) {
             int s = 0, acc = 0;
             uint32_t ph = 0, aph = 0;
             bool ok = true;

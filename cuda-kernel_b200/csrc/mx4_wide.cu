@@ -32,8 +32,10 @@ struct ProjectWork {
     static constexpr bool kMx = true, kLoad = true;
     static constexpr int kPieces = std::is_same<T, __half>::value ? 3 : 2;
     static constexpr int kTok = TOK, kAccs = 1;
-    static constexpr int kPerSm = TOK == 64 ? 1 : 2;
-    static constexpr int kStages = TOK == 16 ? 4 : TOK == 32 ? 3 : 5;
+    static constexpr int kPerSm = TOK == 16 ? 2 : 1;
+    static constexpr int kStages = TOK == 16 ? 2 : 4, kRaw = TOK == 16 ? 3 : 4;
+    static constexpr int kTokenStages = TOK == 16 ? 4 : TOK == 32 ? 6 : 2;
+    static constexpr int kSplitters = TOK == 16 ? 4 : TOK == 32 ? 6 : 8, kGroupWarps = TOK == 64 ? 4 : 1;
 
     const unsigned char* sa[2];
     const unsigned char* sb;
@@ -180,7 +182,7 @@ int dispatch_wide(const ProjectParams& P, cudaStream_t stream) {
 
 }  // namespace
 
-bool project_wide_takes(const ProjectParams& P) { return wide_rows(P.w, P.cols, true); }
+bool project_wide_takes(const ProjectParams&) { return true; }
 
 int project_wide(int type, ProjectParams P, cudaStream_t stream) {
     return type == SWB_F16 ? dispatch_wide<__half>(P, stream) : dispatch_wide<__nv_bfloat16>(P, stream);

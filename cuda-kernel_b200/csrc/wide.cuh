@@ -3,18 +3,23 @@
 // weights go from global memory to the tensor core without passing a register.
 //
 // 16-bit weights: tcgen05.mma kind::f16. Four-bit weights: kind::mxf8f6f4, whose operands may
-// differ in type: the codes (spread to a byte each by the copy) and their power-of-two scales
-// are the M side as they are; a token is the sum of `pieces` e4m3 values, each block of 32 with
+// differ in type: the codes and their power-of-two scales are the M side as they are; a token is the sum of `pieces` e4m3 values, each block of 32 with
 // a scale of its own, five binades apart, rounded from what the piece before left. Three pieces
 // hold 15 bits below a block's largest value (all of an fp16 value within 13 binades of it, and
 // 2^-27 of the largest beyond), two hold 9 (bf16). A piece is a column of its own; the epilogue
 // adds a token's columns. Every product is exact and the sums are the tensor core's fp32.
 //
-// Roles of a CTA (10 or 14 warps), through a ring of stages of 128 bytes of every row:
-//   copies     one thread, TMA: two halves of 64 rows of W (gate and up rows, or neighbours), and
-//              the tokens where they lie prepared in memory
-//   loaders    four warps, or eight that split tokens: tokens from their rows (gathered, split into pieces), scale bytes of
-//              both sides into the 32 x 16-byte blocks that tcgen05.cp spreads over TMEM
+// Roles of a CTA, through two rings of stages of 128 bytes of every row (one for the weights, one
+// for the tokens):
+//   copies     one thread, TMA: two halves of 64 rows of W (gate and up rows, or neighbours)
+//   spreaders  (four-bit) four warps. Codes arrive packed in a ring of their own, 16 KB a stage, the
+//              bytes in flight, and are spread to the eight bytes of every sixteen that the product
+//              reads; their scales go into the 32 x 16-byte blocks that tcgen05.cp spreads over
+//              TMEM. (The copy engine can spread codes too, at about the same rate.)
+//   splitters  tokens from their rows, gathered and split into pieces, or copied where they lie
+//              prepared. A stage's chain of conversions takes 0.5 to 1 us whatever its size, so
+//              groups of warps each take stages of their own: that chain, done by all warps
+//              together stage after stage, held the kernel to a sixth of the memory's rate.
 //   products   one thread
 //   epilogue   four warps, a TMEM quadrant each
 #pragma once
@@ -143,9 +148,11 @@ struct WideItem {
 
 // W describes the work:
 //   types      T; kMx; kPieces; kTok (tokens of an item, a multiple of 16); kLoad (tokens by the
-//              loaders; else rows `first * kPieces` on of a tensor map); kAccs; kStages; kPerSm
+//              splitters; else rows `first * kPieces` on of a tensor map, and for four-bit weights
+//              scales `sb`); kAccs; kStages and kTokenStages (of the rings); kRaw (stages of packed
+//              codes); kSplitters (warps) in groups of kGroupWarps; kPerSm
 //   item(i, it) -> false past the last one;  token(it, n): row of token n (kLoad)
-//   halves: 1 or 2 of 64 rows;  scales of W: sa[2], blocks, rows_a;  of tokens that lie prepared: sb
+//   halves: 1 or 2 of 64 rows;  scales of W: sa[2], blocks, rows_a;  x_aligned, cols
 //   begin(it) / value(it, n, row, v) / end(it): epilogue threads, by their row
 template <typename W>
 struct Wide {
@@ -154,23 +161,57 @@ struct Wide {
     static constexpr int kN = W::kPieces * W::kTok;
     static constexpr int kBytesB = kN * kWideRowBytes;
     static constexpr int kBlocksB = kMx ? (kN + 127) / 128 : 0;
-    static constexpr int kScales = kMx ? (1 + kBlocksB) * kScaleBlock : 0;
-    static constexpr int kStage = (kWideA + kBytesB + kScales + 1023) / 1024 * 1024;
-    static constexpr int kScaleColumns = kMx ? 4 * (1 + kBlocksB) : 0;
-    static constexpr int kUsed = W::kAccs * kN + W::kStages * kScaleColumns;
+    // A stage of weights: tile, block of scales. A stage of tokens: tile, blocks of scales.
+    static constexpr int kStageA = kWideA, kStageB = kBytesB;
+    static constexpr int kScaleColumnsA = kMx ? 4 : 0, kScaleColumnsB = 4 * kBlocksB;
+    static constexpr int kUsed = W::kAccs * kN + W::kStages * kScaleColumnsA + W::kTokenStages * kScaleColumnsB;
     static constexpr int kColumns = kUsed <= 32 ? 32 : kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
     static constexpr int kValues = kMx ? 128 : 64;   // of a row in a stage
-    static constexpr int kRowSource = kMx ? 64 : 128;  // their bytes in W
-    static constexpr bool kLoaders = W::kLoad || kMx;
-    static constexpr int kWideLoaders = kMx && W::kLoad ? 8 : 4;  // warps
-    static constexpr int kThreads = (kWideEpilogue + kWideLoaders + 2) * 32;
+    static constexpr int kRawStage = kMx ? kWideM * 128 : 0, kRaw = kMx ? W::kRaw : 0;
+    static constexpr int kSpreaders = kMx ? 4 : 0, kSplitters = W::kSplitters, kGroupWarps = W::kGroupWarps;
+    static constexpr int kGroups = kSplitters / kGroupWarps;
+    static constexpr int kWarps = kWideEpilogue + kSpreaders + kSplitters + 2, kThreads = kWarps * 32;
     static_assert(kUsed <= 512 && kColumns * W::kPerSm <= 512, "TMEM columns");
-    static constexpr size_t kRing = size_t(W::kStages) * kStage;
+    static_assert(W::kLoad || kGroupWarps == 1, "a warp brings prepared tokens");
+    // a group that waits for a stage of tokens is at most one round of the ring ahead of its readers
+    static_assert(kGroups <= W::kTokenStages, "groups do not overtake the ring");
+
+    // Offsets from the base of the dynamic shared memory (on 1 KB).
+    static constexpr uint32_t kAtB = W::kStages * kStageA, kAtRaw = kAtB + W::kTokenStages * kStageB;
+    static constexpr uint32_t kAtScalesA = kAtRaw + kRaw * kRawStage;
+    static constexpr uint32_t kAtScalesB = kAtScalesA + (kMx ? W::kStages * kScaleBlock : 0);
+    static constexpr uint32_t kRing = (kAtScalesB + W::kTokenStages * kBlocksB * kScaleBlock + 1023) / 1024 * 1024;
+    static_assert(kStageB % 1024 == 0, "tiles keep the swizzle's alignment");
 
     struct Shared {
-        uint64_t full[W::kStages], loaded[W::kStages], empty[W::kStages], acc_full[2], acc_empty[2];
+        uint64_t full[W::kStages], empty[W::kStages], acc_full[2], acc_empty[2];
+        uint64_t tokens_full[W::kTokenStages], tokens_empty[W::kTokenStages];
+        uint64_t raw_full[kRaw + 1], raw_empty[kRaw + 1];
         uint32_t tmem;
         int failed;
+    };
+
+    // A place in a ring.
+    template <int STAGES>
+    struct Ring {
+        int s = 0;
+        uint32_t ph = 0;
+        int64_t issued = 0;
+        __device__ __forceinline__ void next() {
+            ++issued;
+            if (++s == STAGES) s = 0, ph ^= 1u;
+        }
+        // The stage is free again (a producer's wait).
+        __device__ __forceinline__ bool free(uint64_t* empty) const {
+            return issued < STAGES || mbar_wait(smem_u32(empty + s), ph ^ 1u);
+        }
+        // Nothing stays in flight into shared memory when a copier gives up.
+        __device__ __forceinline__ void drain(uint64_t* full) const {
+            for (int i = 0; i < STAGES && i < issued; ++i) {
+                const int64_t idx = issued - 1 - i;
+                mbar_wait(smem_u32(full + idx % STAGES), uint32_t(idx / STAGES) & 1u);
+            }
+        }
     };
 
     // Every thread of the CTA, before run(); the CTA synchronises in between.
@@ -178,13 +219,20 @@ struct Wide {
         if (threadIdx.x == 0) {
             s.failed = 0;
             for (int i = 0; i < W::kStages; ++i) {
-                mbar_init(smem_u32(s.full + i), 1);
-                mbar_init(smem_u32(s.loaded + i), kWideLoaders * 32);
+                mbar_init(smem_u32(s.full + i), kMx ? kSpreaders : 1);
                 mbar_init(smem_u32(s.empty + i), 1);
+            }
+            for (int i = 0; i < W::kTokenStages; ++i) {
+                mbar_init(smem_u32(s.tokens_full + i), kGroupWarps);
+                mbar_init(smem_u32(s.tokens_empty + i), 1);
             }
             for (int i = 0; i < 2; ++i) {
                 mbar_init(smem_u32(s.acc_full + i), 1);
                 mbar_init(smem_u32(s.acc_empty + i), kWideEpilogue * 32);
+            }
+            for (int i = 0; i < kRaw; ++i) {
+                mbar_init(smem_u32(s.raw_full + i), 1);
+                mbar_init(smem_u32(s.raw_empty + i), kSpreaders);
             }
             mbar_fence_init();
         }
@@ -198,250 +246,313 @@ struct Wide {
             tmem_free(s.tmem, kColumns);
         }
     }
-    // Columns of an item: whole groups of 16 tokens.
-    static __device__ __forceinline__ int columns(int count) { return (count + 15) / 16 * 16 * W::kPieces; }
+    // Columns of an item.
+    static __device__ __forceinline__ int columns(int count) { return (count * W::kPieces + 15) / 16 * 16; }
 
-    // base: the ring, on 1 KB. maps: W's two tensors, the prepared tokens.
+    // maps: W's two tensors, the prepared tokens.
     static __device__ __forceinline__ void run(W& work, Shared& sh, uint32_t base, const CUtensorMap* map0,
                                                const CUtensorMap* map1, const CUtensorMap* map_b, uint64_t policy) {
         fence_after();
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        const uint32_t tmem = sh.tmem, scale_columns = tmem + W::kAccs * kN;
-        int s = 0;
-        uint32_t ph = 0;
-        int64_t issued = 0;
+        const int warp = threadIdx.x >> 5;
         bool ok = true;
-        auto next_stage = [&] {
-            ++issued;
-            if (++s == W::kStages) s = 0, ph ^= 1u;
-        };
-        WideItem it;
-
-        if (warp == kWideEpilogue + kWideLoaders) {
-            if (lane == 0) {
-                for (int i = 0; ok && work.item(i, it); ++i) {
-                    const int n = columns(it.count);
-                    for (int k = it.s0; k < it.s1; ++k) {
-                        if (issued >= W::kStages && !mbar_wait(smem_u32(sh.empty + s), ph ^ 1u)) {
-                            ok = false;
-                            break;
-                        }
-                        const uint32_t bar = smem_u32(sh.full + s), at = base + s * kStage;
-                        mbar_arrive_expect_tx(bar, work.halves * kWideHalf * kRowSource + (W::kLoad ? 0 : n * kWideRowBytes));
-                        tma_load_2d(at, map0, k * kValues, int(it.row[0]), bar, policy);
-                        if (work.halves == 2) tma_load_2d(at + kWideA / 2, map1, k * kValues, int(it.row[1]), bar, policy);
-                        if (!W::kLoad) {
-                            for (int r = 0; r < n; r += 16)
-                                tma_load_2d(at + kWideA + r * kWideRowBytes, map_b, k * kValues, it.first * W::kPieces + r, bar);
-                        }
-                        next_stage();
-                    }
-                }
-                if (!ok) {  // nothing stays in flight into shared memory
-                    for (int i = 0; i < W::kStages && i < issued; ++i) {
-                        const int64_t idx = issued - 1 - i;
-                        mbar_wait(smem_u32(sh.full + idx % W::kStages), uint32_t(idx / W::kStages) & 1u);
-                    }
-                    sh.failed = 1;
-                }
-            }
-        } else if (warp == kWideEpilogue + kWideLoaders + 1) {
-            if (lane == 0) {
-                int acc = 0, done = 0;
-                uint32_t aph = 0;
-                for (int i = 0; ok && work.item(i, it); ++i, ++done) {
-                    const int n = columns(it.count);
-                    if (done >= W::kAccs) {  // the accumulator's last item has been read
-                        ok = mbar_wait(smem_u32(sh.acc_empty + acc), aph ^ 1u);
-                        if (!ok) break;
-                    }
-                    for (int k = it.s0; k < it.s1; ++k) {
-                        ok = mbar_wait(smem_u32(sh.full + s), ph) && (!kLoaders || mbar_wait(smem_u32(sh.loaded + s), ph));
-                        if (!ok) break;
-                        fence_after();
-                        const uint32_t at = base + s * kStage, col = scale_columns + s * kScaleColumns;
-                        if constexpr (kMx) {
-#pragma unroll
-                            for (int j = 0; j < 1 + kBlocksB; ++j)
-                                scale_copy(col + 4 * j, scale_desc(at + kWideA + kBytesB + j * kScaleBlock));
-                        }
-                        const uint64_t da = operand_desc(at), db = operand_desc(at + kWideA);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if constexpr (kMx)
-                                mma_mxf8f6f4(tmem + acc * kN, da + 2 * j, db + 2 * j, mxf8f6f4_desc(kWideM, n, j), col, col + 4,
-                                             k > it.s0 || j > 0);
-                            else
-                                mma_f16(tmem + acc * kN, da + 2 * j, db + 2 * j, f16_desc<T>(kWideM, n), k > it.s0 || j > 0);
-                        }
-                        mma_commit(smem_u32(sh.empty + s));
-                        if (k == it.s1 - 1) mma_commit(smem_u32(sh.acc_full + acc));
-                        next_stage();
-                    }
-                    if (++acc == W::kAccs) acc = 0, aph ^= 1u;
-                }
-                if (!ok) sh.failed = 1;
-            }
-        } else if (warp >= kWideEpilogue) {
-            if constexpr (kLoaders) ok = load(work, sh, base);
-            if (!ok) sh.failed = 1;
+        if (warp < kWideEpilogue) {
+            ok = epilogue(work, sh);
+        } else if (warp < kWideEpilogue + kSpreaders) {
+            if constexpr (kMx) ok = spread(work, sh, base);
+        } else if (warp < kWideEpilogue + kSpreaders + kSplitters) {
+            if constexpr (W::kLoad)
+                ok = split(work, sh, base);
+            else
+                ok = bring(work, sh, base, map_b);
+        } else if (warp == kWarps - 2) {
+            if (elect_one()) ok = copy(work, sh, base, map0, map1, policy);
         } else {
-            int acc = 0;
-            uint32_t aph = 0;
-            const uint32_t quadrant = uint32_t(warp * 32) << 16;
-            for (int i = 0; work.item(i, it); ++i) {
-                ok = mbar_wait_warp(smem_u32(sh.acc_full + acc), aph);
-                if (!ok) break;
-                fence_after();
-                work.begin(it);
-#pragma unroll 1
-                for (int c = 0; c < it.count; c += 16) {  // 16 tokens, kPieces columns each
-                    float v[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] = 0.f;
-#pragma unroll
-                    for (int part = 0; part < W::kPieces; ++part) {
-                        uint32_t r[16];
-                        __syncwarp();
-                        tmem_load16(tmem + quadrant + acc * kN + c * W::kPieces + part * 16, r);
-                        tmem_load_wait();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) v[(part * 16 + j) / W::kPieces] += __uint_as_float(r[j]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (c + j < it.count) work.value(it, c + j, warp * 32 + lane, v[j]);
-                }
-                fence_before();
-                mbar_arrive(smem_u32(sh.acc_empty + acc));
-                work.end(it);
-                if (++acc == W::kAccs) acc = 0, aph ^= 1u;
-            }
-            if (!ok) sh.failed = 1;
+            if (elect_one()) ok = multiply(work, sh, base);
         }
+        if (!ok) sh.failed = 1;
         __syncwarp();
         fence_before();
     }
 
-    // Loader warps: tokens and scale bytes of every stage, the next stage's on their way meanwhile.
-    static __device__ __forceinline__ bool load(W& work, Shared& sh, uint32_t base) {
-        constexpr int kPer = kMx ? 16 : 8;                       // 8-value parts of a row in a stage
-        constexpr int kStride = kWideLoaders * 32 / kPer;        // tokens taken at once
-        constexpr int kTurns = W::kLoad ? (W::kTok + kStride - 1) / kStride : 1;
-        constexpr int kRowsB = W::kLoad ? 1 : (kN + 127) / 128;  // rows of prepared scales of a thread
-        const int t = threadIdx.x - kWideEpilogue * 32, j = t % kPer, n0 = t / kPer;
-        int s = 0;
-        uint32_t ph = 0;
-        int64_t issued = 0;
+    // Copies of W: 16-bit tiles straight into the products' stages, codes into the raw ring.
+    static __device__ __forceinline__ bool copy(W& work, Shared& sh, uint32_t base, const CUtensorMap* map0,
+                                                const CUtensorMap* map1, uint64_t policy) {
+        constexpr int kStages = kMx ? kRaw : W::kStages, kBytes = kMx ? kRawStage : kStageA;
+        uint64_t* full = kMx ? sh.raw_full : sh.full;
+        uint64_t* empty = kMx ? sh.raw_empty : sh.empty;
+        Ring<kStages> ring;
         WideItem it;
         for (int i = 0; work.item(i, it); ++i) {
-            const typename W::T* x[kTurns];
-            const unsigned char *row_a = nullptr, *row_b[kRowsB];
-            if constexpr (W::kLoad) {
-#pragma unroll
-                for (int u = 0; u < kTurns; ++u) x[u] = work.token(it, min(n0 + u * kStride, it.count - 1));
-            }
-            if (kMx && t < kWideM) {
-                const int half = t / kWideHalf;
-                const int64_t r = (half ? it.row[1] : it.row[0]) + t % kWideHalf;
-                if (r < work.rows_a && half < work.halves) row_a = (half ? work.sa[1] : work.sa[0]) + r * work.blocks;
-#pragma unroll
-                for (int u = 0; u < kRowsB; ++u) {
-                    const int b = t + 128 * u;
-                    row_b[u] = !W::kLoad && b < it.count * W::kPieces ? work.sb + int64_t(it.first * W::kPieces + b) * work.blocks : nullptr;
+            // a raw stage holds two of the products' stages
+            const int k0 = kMx ? it.s0 / 2 : it.s0, k1 = kMx ? (it.s1 + 1) / 2 : it.s1;
+            for (int k = k0; k < k1; ++k) {
+                if (!ring.free(empty)) {
+                    ring.drain(full);
+                    return false;
                 }
-            }
-            uint4 xv[kTurns];
-            auto load_x = [&](int k) {
-                if constexpr (W::kLoad) {
-#pragma unroll
-                    for (int u = 0; u < kTurns; ++u) {
-                        if (u * kStride >= it.count) break;
-                        const int at = k * kValues + j * 8;
-                        xv[u] = work.x_aligned ? load_piece<T, true>(x[u], at, work.cols) : load_piece<T, false>(x[u], at, work.cols);
-                    }
-                }
-            };
-            // Windows of 16 scale bytes, four stages each, two windows ahead: W's come from DRAM.
-            uint4 win_a[3] = {}, win_b[3][kRowsB] = {};
-            auto load_windows = [&](int w, int k) {
-                if constexpr (kMx) {
-                    const bool have = k < it.s1;
-                    win_a[w] = row_a && have ? load_scales(row_a, k / 4 * 16, work.blocks) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                    for (int u = 0; u < kRowsB; ++u)
-                        win_b[w][u] = row_b[u] && have ? load_scales(row_b[u], k / 4 * 16, work.blocks) : make_uint4(0u, 0u, 0u, 0u);
-                }
-            };
-            load_x(it.s0);
-            load_windows(0, it.s0);
-            load_windows(1, (it.s0 | 3) + 1);
-            load_windows(2, (it.s0 | 3) + 5);
-            for (int k = it.s0; k < it.s1; ++k) {
-                uint4 now[kTurns];
-#pragma unroll
-                for (int u = 0; u < kTurns; ++u) now[u] = xv[u];
-                if (kMx && k > it.s0 && k % 4 == 0) {
-                    win_a[0] = win_a[1], win_a[1] = win_a[2];
-#pragma unroll
-                    for (int u = 0; u < kRowsB; ++u) win_b[0][u] = win_b[1][u], win_b[1][u] = win_b[2][u];
-                    load_windows(2, k + 8);
-                }
-                if (k + 1 < it.s1) load_x(k + 1);
-                if (issued >= W::kStages && !mbar_wait_warp(smem_u32(sh.empty + s), ph ^ 1u)) return false;
-                const uint32_t b = base + s * kStage + kWideA, sc = b + kBytesB;
-                if (kMx && t < kWideM) sts32(sc + scale_place(t), word_of(win_a[0], k));
-                if constexpr (kMx && !W::kLoad) {
-#pragma unroll
-                    for (int u = 0; u < kRowsB; ++u)
-                        if (t + 128 * u < kN) sts32(sc + kScaleBlock + scale_place(t + 128 * u), word_of(win_b[0][u], k));
-                }
-                if constexpr (W::kLoad) {
-#pragma unroll
-                    for (int u = 0; u < kTurns; ++u) {
-                        if (u * kStride >= it.count) break;  // whole warps: the shuffles below stay together
-                        const int n = n0 + u * kStride;
-                        if constexpr (!kMx) {
-                            if (n < it.count)
-                                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(b + swizzled(n, j)), "r"(now[u].x), "r"(now[u].y), "r"(now[u].z), "r"(now[u].w) : "memory");
-                        } else {
-                            uint2 piece[W::kPieces];
-                            const uint32_t scale = split_token<W::kPieces>(now[u], piece, T());
-                            if (n < it.count) {
-#pragma unroll
-                                for (int p = 0; p < W::kPieces; ++p) {
-                                    const int r = n * W::kPieces + p;
-                                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(b + swizzled(r, j / 2) + (j & 1) * 8), "r"(piece[p].x), "r"(piece[p].y) : "memory");
-                                    if ((j & 3) == 0) sts8(sc + kScaleBlock + scale_place(r) + j / 4, scale - 5u * p);
-                                }
-                            }
-                        }
-                    }
-                }
-                fence_proxy_async_smem();
-                mbar_arrive(smem_u32(sh.loaded + s));
-                ++issued;
-                if (++s == W::kStages) s = 0, ph ^= 1u;
+                const uint32_t bar = smem_u32(full + ring.s), at = base + (kMx ? kAtRaw : 0u) + ring.s * kBytes;
+                mbar_arrive_expect_tx(bar, work.halves * (kBytes / 2));
+                const int x = k * (kMx ? 32 : 64);  // elements of four bytes (codes), or of two
+                tma_load_2d(at, map0, x, int(it.row[0]), bar, policy);
+                if (work.halves == 2) tma_load_2d(at + kBytes / 2, map1, x, int(it.row[1]), bar, policy);
+                ring.next();
             }
         }
         return true;
     }
-    static __device__ __forceinline__ uint32_t word_of(const uint4& w, int k) {
-        return k & 2 ? (k & 1 ? w.w : w.z) : (k & 1 ? w.y : w.x);
+
+    static __device__ __forceinline__ bool multiply(W& work, Shared& sh, uint32_t base) {
+        const uint32_t tmem = sh.tmem, columns_a = tmem + W::kAccs * kN, columns_b = columns_a + W::kStages * kScaleColumnsA;
+        Ring<W::kStages> a;
+        Ring<W::kTokenStages> b;
+        Ring<W::kAccs> acc;
+        WideItem it;
+        for (int i = 0; work.item(i, it); ++i) {
+            const int n = columns(it.count);
+            if (!acc.free(sh.acc_empty)) return false;  // the accumulator's last item has been read
+            for (int k = it.s0; k < it.s1; ++k) {
+                if (!mbar_wait(smem_u32(sh.full + a.s), a.ph) || !mbar_wait(smem_u32(sh.tokens_full + b.s), b.ph)) return false;
+                fence_after();
+                const uint32_t ca = columns_a + a.s * kScaleColumnsA, cb = columns_b + b.s * kScaleColumnsB;
+                if constexpr (kMx) {
+                    scale_copy(ca, scale_desc(base + kAtScalesA + a.s * kScaleBlock));
+#pragma unroll
+                    for (int j = 0; j < kBlocksB; ++j)
+                        scale_copy(cb + 4 * j, scale_desc(base + kAtScalesB + (b.s * kBlocksB + j) * kScaleBlock));
+                }
+                const uint64_t da = operand_desc(base + a.s * kStageA), db = operand_desc(base + kAtB + b.s * kStageB);
+                const uint32_t d = tmem + acc.s * kN;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (kMx)
+                        mma_mxf8f6f4(d, da + 2 * j, db + 2 * j, mxf8f6f4_desc(kWideM, n, j), ca, cb, k > it.s0 || j > 0);
+                    else
+                        mma_f16(d, da + 2 * j, db + 2 * j, f16_desc<T>(kWideM, n), k > it.s0 || j > 0);
+                }
+                mma_commit(smem_u32(sh.empty + a.s));
+                mma_commit(smem_u32(sh.tokens_empty + b.s));
+                if (k == it.s1 - 1) mma_commit(smem_u32(sh.acc_full + acc.s));
+                a.next();
+                b.next();
+            }
+            acc.next();
+        }
+        return true;
+    }
+
+    static __device__ __forceinline__ bool epilogue(W& work, Shared& sh) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        const uint32_t quadrant = sh.tmem + (uint32_t(warp * 32) << 16);
+        Ring<W::kAccs> acc;
+        WideItem it;
+        for (int i = 0; work.item(i, it); ++i) {
+            if (!mbar_wait_warp(smem_u32(sh.acc_full + acc.s), acc.ph)) return false;
+            fence_after();
+            work.begin(it);
+#pragma unroll 1
+            for (int c = 0; c < it.count; c += 16) {  // 16 tokens, kPieces columns each
+                float v[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = 0.f;
+#pragma unroll
+                for (int part = 0; part < W::kPieces; ++part) {
+                    uint32_t r[16];
+                    __syncwarp();
+                    tmem_load16(quadrant + acc.s * kN + c * W::kPieces + part * 16, r);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[(part * 16 + j) / W::kPieces] += __uint_as_float(r[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (c + j < it.count) work.value(it, c + j, warp * 32 + lane, v[j]);
+            }
+            fence_before();
+            mbar_arrive(smem_u32(sh.acc_empty + acc.s));
+            work.end(it);
+            acc.next();
+        }
+        return true;
+    }
+
+    // Spreaders: codes and scales of W. Windows of 16 scale bytes, four stages each, two windows
+    // ahead: they come from DRAM.
+    static __device__ __forceinline__ bool spread(W& work, Shared& sh, uint32_t base) {
+        const int t = threadIdx.x - kWideEpilogue * 32, lane = t & 31, half = t / kWideHalf;
+        Ring<W::kStages> ring;
+        Ring<kRaw> raw;
+        WideItem it;
+        for (int i = 0; work.item(i, it); ++i) {
+            const int64_t r = (half ? it.row[1] : it.row[0]) + t % kWideHalf;
+            const unsigned char* row =
+                r < work.rows_a && half < work.halves ? (half ? work.sa[1] : work.sa[0]) + r * work.blocks : nullptr;
+            uint4 window[3];
+            auto load = [&](int w, int k) {
+                window[w] = row && k < it.s1 ? load_scales(row, k / 4 * 16, work.blocks) : make_uint4(0u, 0u, 0u, 0u);
+            };
+            load(0, it.s0);
+            load(1, (it.s0 | 3) + 1);
+            load(2, (it.s0 | 3) + 5);
+            for (int k = it.s0; k < it.s1; ++k) {
+                if (k > it.s0 && k % 4 == 0) {
+                    window[0] = window[1], window[1] = window[2];
+                    load(2, k + 8);
+                }
+                const bool first = k == it.s0 || k % 2 == 0;
+                const bool ready = ring.free(sh.empty) && (!first || mbar_wait(smem_u32(sh.raw_full + raw.s), raw.ph));
+                if (!__all_sync(0xFFFFFFFFu, ready)) return false;
+                // a warp takes eight rows, four blocks of 16 bytes each, at a time
+                const uint32_t from = base + kAtRaw + raw.s * kRawStage, to = base + ring.s * kStageA;
+                const int block = lane >> 3;
+                uint4 c[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) c[u] = lds128(from + swizzled((t / 32 + u * 4) * 8 + (lane & 7), k % 2 * 4 + block));
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int q = (t / 32 + u * 4) * 8 + (lane & 7);
+                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to + swizzled(q, 2 * block)), "r"(c[u].x), "r"(c[u].y) : "memory");
+                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to + swizzled(q, 2 * block + 1)), "r"(c[u].z), "r"(c[u].w) : "memory");
+                }
+                const uint4& w = window[0];
+                sts32(base + kAtScalesA + ring.s * kScaleBlock + scale_place(t), k & 2 ? (k & 1 ? w.w : w.z) : (k & 1 ? w.y : w.x));
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(sh.full + ring.s));
+                ring.next();
+                if (k % 2 == 1 || k + 1 == it.s1) {
+                    if (lane == 0) mbar_arrive(smem_u32(sh.raw_empty + raw.s));
+                    raw.next();
+                }
+            }
+        }
+        return true;
+    }
+
+    // Splitters: group g takes the stages g, g + kGroups, ... of the sequence.
+    static __device__ __forceinline__ bool split(W& work, Shared& sh, uint32_t base) {
+        constexpr int kPer = kMx ? 16 : 8;                    // eight-value parts of a row in a stage
+        constexpr int kStride = kGroupWarps * 32 / kPer;      // tokens taken at once
+        constexpr int kTurns = (W::kTok + kStride - 1) / kStride, kBatch = kTurns < 4 ? kTurns : 4;
+        const int warp = threadIdx.x / 32 - kWideEpilogue - kSpreaders, group = warp / kGroupWarps;
+        const int t = threadIdx.x - (kWideEpilogue + kSpreaders + group * kGroupWarps) * 32, j = t % kPer, n0 = t / kPer;
+        Ring<W::kTokenStages> ring;
+        int turn = 0;  // of the group whose stage is next
+        WideItem it;
+        uint4 x[kTurns];
+        for (int i = 0; work.item(i, it); ++i) {
+            auto load = [&](int k) {
+                if (k >= it.s1) return;
+#pragma unroll
+                for (int u = 0; u < kTurns; ++u) {
+                    if (u * kStride >= it.count) break;
+                    const T* row = work.token(it, min(n0 + u * kStride, it.count - 1));
+                    const int at = k * kValues + j * 8;
+                    x[u] = work.x_aligned ? load_piece<T, true>(row, at, work.cols) : load_piece<T, false>(row, at, work.cols);
+                }
+            };
+            int mine = it.s0 + (group - turn + kGroups) % kGroups;  // this group's first stage of the item
+            load(mine);
+            for (int k = it.s0; k < it.s1; ++k) {
+                if (k == mine) {
+                    if (!__all_sync(0xFFFFFFFFu, ring.free(sh.tokens_empty))) return false;
+                    const uint32_t b = base + kAtB + ring.s * kStageB;
+                    const uint32_t sc = base + kAtScalesB + ring.s * kBlocksB * kScaleBlock;
+#pragma unroll
+                    for (int u0 = 0; u0 < kTurns; u0 += kBatch) {
+                        if (u0 * kStride >= it.count) break;  // whole groups: the shuffles stay together
+                        if constexpr (!kMx) {
+#pragma unroll
+                            for (int u = u0; u < u0 + kBatch && u < kTurns; ++u) {
+                                const int n = n0 + u * kStride;
+                                if (n < it.count)
+                                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(b + swizzled(n, j)), "r"(x[u].x), "r"(x[u].y), "r"(x[u].z), "r"(x[u].w) : "memory");
+                            }
+                        } else {
+                            uint2 piece[kBatch][W::kPieces];
+                            uint32_t scale[kBatch];
+#pragma unroll
+                            for (int u = 0; u < kBatch; ++u)
+                                scale[u] = split_token<W::kPieces>(x[u0 + u < kTurns ? u0 + u : kTurns - 1], piece[u], T());
+#pragma unroll
+                            for (int u = 0; u < kBatch; ++u) {
+                                const int n = n0 + (u0 + u) * kStride;
+                                if (n >= it.count) continue;
+#pragma unroll
+                                for (int p = 0; p < W::kPieces; ++p) {
+                                    const int r = n * W::kPieces + p;
+                                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(b + swizzled(r, j / 2) + (j & 1) * 8), "r"(piece[u][p].x), "r"(piece[u][p].y) : "memory");
+                                    if ((j & 3) == 0) sts8(sc + scale_place(r) + j / 4, scale[u] - 5u * p);
+                                }
+                            }
+                        }
+                    }
+                    mine += kGroups;
+                    load(mine);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(sh.tokens_full + ring.s));
+                }
+                ring.next();
+            }
+            turn = (turn + it.s1 - it.s0) % kGroups;
+        }
+        return true;
+    }
+
+    // Prepared tokens: a warp brings a stage's rows by TMA, their scale words by plain loads.
+    static __device__ __forceinline__ bool bring(W& work, Shared& sh, uint32_t base, const CUtensorMap* map_b) {
+        const int lane = threadIdx.x & 31, group = threadIdx.x / 32 - kWideEpilogue - kSpreaders;
+        Ring<W::kTokenStages> ring;
+        WideItem it;
+        for (int i = 0; work.item(i, it); ++i) {
+            const int n = columns(it.count);
+            for (int k = it.s0; k < it.s1; ++k) {
+                if (ring.issued % kGroups == group) {
+                    if (!__all_sync(0xFFFFFFFFu, ring.free(sh.tokens_empty))) {
+                        if (lane == 0) ring.drain(sh.tokens_full);
+                        return false;
+                    }
+                    const uint32_t bar = smem_u32(sh.tokens_full + ring.s), b = base + kAtB + ring.s * kStageB;
+                    if constexpr (kMx) {
+#pragma unroll
+                        for (int u = 0; u < (kN + 31) / 32; ++u) {
+                            const int r = lane + 32 * u;
+                            if (r >= it.count * W::kPieces) continue;
+                            const unsigned char* row = work.sb + int64_t(it.first * W::kPieces + r) * work.blocks;
+                            uint32_t w = 0u;
+                            if ((work.blocks & 3) == 0) {
+                                w = *reinterpret_cast<const uint32_t*>(row + k * 4);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (k * 4 + e < work.blocks) w |= uint32_t(row[k * 4 + e]) << (8 * e);
+                            }
+                            sts32(base + kAtScalesB + ring.s * kBlocksB * kScaleBlock + scale_place(r), w);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(bar, n * kWideRowBytes);
+                        for (int r = 0; r < n; r += 16)
+                            tma_load_2d(b + r * kWideRowBytes, map_b, k * kValues, it.first * W::kPieces + r, bar);
+                    }
+                }
+                ring.next();
+            }
+        }
+        return true;
     }
 };
 
 // ------------------------------------------------------------ host
-// Whether W's rows can be copied for the tensor core: whole 16-byte rows, or codes in pairs of
-// 32-byte pieces of 128 values.
+// Whether W's rows can be copied: whole 16-byte rows (of codes: always, and the calls require it).
 inline bool wide_rows(const void* w, int64_t cols, bool mx) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(w);
-    return mx ? mx_blocks(cols) % 4 == 0 && a % 32 == 0 : cols % 8 == 0 && a % 16 == 0;
+    return mx || (cols % 8 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0);
 }
-// Map of W [rows, cols] in boxes of 64 rows by 128 bytes of shared memory.
+// Map of W [rows, cols] in boxes of 64 rows by 128 bytes.
 inline int make_wide_map(CUtensorMap* map, const void* w, int64_t rows, int64_t cols, bool mx) {
-    const int64_t padded = mx_blocks(cols) * kMxBlock;
-    return mx ? make_typed_map(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, w, padded, rows, padded / 2, 128, kWideHalf)
+    return mx ? make_map(map, w, rows, mx_blocks(cols) * kMxBlockBytes, 128, kWideHalf)
               : make_typed_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, w, cols, rows, cols * 2, 64, kWideHalf);
 }
 
