@@ -140,6 +140,7 @@ int swb_moe(int type, unsigned flags, const void* x, int64_t x_pitch, const void
     P.picks = reinterpret_cast<int*>(base + w.picks);
     P.shares = reinterpret_cast<float*>(base + w.shares);
     P.h = base + w.h;
+    P.pieces = base + w.pieces;
     P.x_pitch = x_pitch;
     P.tokens = tokens;
     P.hidden = hidden;

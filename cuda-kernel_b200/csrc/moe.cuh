@@ -54,6 +54,7 @@ struct MoeParams {
     int* picks;      // [tokens, topk]
     float* shares;   // [tokens, topk]
     void* h;         // [2][tokens * topk, h_pitch]: rounded, then what is left
+    void* pieces;    // tokens split into e4m3 values (moe_wide.cu)
     int64_t x_pitch;
     int tokens, hidden, inter, experts, topk, h_pitch;
     int renormalize;
@@ -63,8 +64,9 @@ struct MoeParams {
 
 // Offsets of the workspace's parts.
 struct MoeWorkspace {
-    size_t logits, picks, shares, h, total;
+    size_t logits, picks, shares, h, pieces, total;
 };
+constexpr int kMoePieceDim = 8192;  // values of a token whose pieces the workspace holds
 __host__ __device__ inline int moe_h_pitch(int inter) { return (inter + kTileRows - 1) / kTileRows * kTileRows; }
 __host__ __device__ inline MoeWorkspace moe_workspace(int tokens, int experts, int topk, int inter) {
     MoeWorkspace m;
@@ -72,7 +74,8 @@ __host__ __device__ inline MoeWorkspace moe_workspace(int tokens, int experts, i
     m.picks = m.logits + size_t(tokens) * experts * 8;
     m.shares = m.picks + size_t(tokens) * topk * 4;
     m.h = (m.shares + size_t(tokens) * topk * 4 + 255) / 256 * 256;
-    m.total = m.h + size_t(tokens) * topk * moe_h_pitch(inter) * 4;
+    m.pieces = (m.h + size_t(tokens) * topk * moe_h_pitch(inter) * 4 + 255) / 256 * 256;
+    m.total = m.pieces + (tokens > 8 ? size_t(tokens) * 3 * (kMoePieceDim + kMoePieceDim / 32) : 0);
     return m;
 }
 

@@ -38,17 +38,20 @@ struct WideMaps {
     CUtensorMap gate, up;
 };
 
-template <typename T_, bool MX>
+// SPLIT: tokens are split into pieces at each use; else once, ahead of the items, into the
+// workspace, which holds the pieces of kMoePieceDim values a token.
+template <typename T_, bool MX, bool SPLIT>
 struct GateWork {
     using T = T_;
-    static constexpr bool kMx = MX, kLoad = true;
+    static constexpr bool kMx = MX, kLoad = SPLIT || !MX, kGather = MX && !SPLIT;
     static constexpr int kPieces = MX ? (std::is_same<T, __half>::value ? 3 : 2) : 1;
     static constexpr int kTok = kMoeGroup, kAccs = 2, kPerSm = 1;
     static constexpr int kStages = MX ? 3 : 8, kRaw = 4, kTokenStages = MX ? 5 : 6;
-    static constexpr int kSplitters = MX ? 5 : 4, kGroupWarps = 1;
+    static constexpr int kSpreadGroups = 2, kSplitters = MX ? 5 : 6, kGroupWarps = 1;
 
     const unsigned char* sa[2];
-    const unsigned char* sb;
+    const unsigned char *sb, *pieces;
+    int pitch, pitch_b;
     int blocks, cols;
     int64_t rows_a;
     bool x_aligned;
@@ -69,6 +72,7 @@ struct GateWork {
         it.count = R->start[group + 1] - it.first;
         return true;
     }
+    __device__ __forceinline__ int place(const WideItem& it, int n) const { return R->token[it.first + n]; }
     __device__ __forceinline__ const T* token(const WideItem& it, int n) const {
         return static_cast<const T*>(P->x) + R->token[it.first + n] * P->x_pitch;
     }
@@ -121,14 +125,15 @@ struct GateWork {
 template <typename T_, bool MX>
 struct DownWork {
     using T = T_;
-    static constexpr bool kMx = MX, kLoad = false;
+    static constexpr bool kMx = MX, kLoad = false, kGather = false;
     static constexpr int kPieces = h_pieces(MX);
     static constexpr int kTok = kMoeGroup, kAccs = 2, kPerSm = 1;
     static constexpr int kStages = MX ? 3 : 7, kRaw = 4, kTokenStages = MX ? 4 : 6;
-    static constexpr int kSplitters = 4, kGroupWarps = 1;
+    static constexpr int kSpreadGroups = 2, kSplitters = 4, kGroupWarps = 1;
 
     const unsigned char* sa[2];
-    const unsigned char* sb;
+    const unsigned char *sb, *pieces;
+    int pitch, pitch_b;
     int blocks, cols;
     int64_t rows_a;
     bool x_aligned;
@@ -150,7 +155,7 @@ struct DownWork {
         it.count = R->start[group + 1] - it.first;
         return true;
     }
-    __device__ __forceinline__ const T* token(const WideItem&, int) const { return nullptr; }
+    __device__ __forceinline__ int place(const WideItem&, int) const { return 0; }
     __device__ __forceinline__ void begin(const WideItem&) const {}
     // a thread owns a row of y; items come in the order of their experts
     __device__ __forceinline__ void value(const WideItem& it, int n, int row, float v) const {
@@ -160,9 +165,33 @@ struct DownWork {
     __device__ __forceinline__ void end(const WideItem&) const {}
 };
 
-template <typename T, bool MX>
+// Every token's pieces, whole stages of them: [token * PIECES + piece][piece_pitch] and their scales.
+__host__ __device__ inline int piece_pitch(int hidden) { return (hidden + 127) / 128 * 128; }
+template <typename T, int PIECES>
+__device__ void split_tokens(const MoeParams& P) {
+    const int pitch = piece_pitch(P.hidden), parts = pitch / 8, all = P.tokens * parts;
+    unsigned char* to = static_cast<unsigned char*>(P.pieces);
+    unsigned char* scales = to + int64_t(P.tokens) * PIECES * pitch;
+    // whole quads: a block's four lanes stay together (parts is a multiple of 16)
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i - int(threadIdx.x & 31) < all; i += gridDim.x * blockDim.x) {
+        const int token = min(i, all - 1) / parts, part = min(i, all - 1) % parts;
+        const T* row = static_cast<const T*>(P.x) + token * P.x_pitch;
+        const uint4 v = P.x_aligned ? load_piece<T, true>(row, part * 8, P.hidden) : load_piece<T, false>(row, part * 8, P.hidden);
+        uint2 piece[PIECES];
+        const uint32_t scale = split_token<PIECES>(v, piece, T());
+        if (i >= all) continue;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int64_t r = int64_t(token) * PIECES + p;
+            *reinterpret_cast<uint2*>(to + r * pitch + part * 8) = piece[p];
+            if (part % 4 == 0) scales[r * (pitch / kMxBlock) + part / 4] = static_cast<unsigned char>(scale - 5u * p);
+        }
+    }
+}
+
+template <typename T, bool MX, bool SPLIT>
 struct GateShape {
-    using Pipe = Wide<GateWork<T, MX>>;
+    using Pipe = Wide<GateWork<T, MX, SPLIT>>;
     static constexpr size_t kPart = Pipe::kRing;
     static constexpr size_t kRoute = (kPart + kMoeGroup * kWidePartPitch * 4 + 15) / 16 * 16;
     static constexpr size_t kSmem = kRoute + sizeof(MoeRoute) + 1024;
@@ -177,11 +206,11 @@ struct DownShape {
     static_assert(kSmem + 1024 <= kSmemPerCtaMax, "shared memory");
 };
 
-template <typename T, bool MX>
-__global__ void __launch_bounds__(Wide<GateWork<T, MX>>::kThreads, 1)
+template <typename T, bool MX, bool SPLIT>
+__global__ void __launch_bounds__(Wide<GateWork<T, MX, SPLIT>>::kThreads, 1)
     moe_gate_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ MoeParams P) {
-    using S = GateShape<T, MX>;
-    using Work = GateWork<T, MX>;
+    using S = GateShape<T, MX, SPLIT>;
+    using Work = GateWork<T, MX, SPLIT>;
     constexpr int kWideThreads = S::Pipe::kThreads;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ typename S::Pipe::Shared sh;
@@ -189,6 +218,7 @@ __global__ void __launch_bounds__(Wide<GateWork<T, MX>>::kThreads, 1)
     __shared__ int flag;
     MoeRoute& R = *reinterpret_cast<MoeRoute*>(smem + S::kRoute);
     S::Pipe::init(sh);
+    if constexpr (Work::kGather) split_tokens<T, Work::kPieces>(P);
     if (threadIdx.x < kRouteThreads) moe_router<T>(P, scratch, &flag);
     const bool routed = moe_grid_barrier(P.sync, &flag);
     griddep_launch_dependents();
@@ -202,7 +232,10 @@ __global__ void __launch_bounds__(Wide<GateWork<T, MX>>::kThreads, 1)
         Work work;
         work.sa[0] = P.s[0];
         work.sa[1] = P.s[1];
-        work.sb = nullptr;
+        work.pitch = piece_pitch(P.hidden);
+        work.pitch_b = work.pitch / kMxBlock;
+        work.pieces = static_cast<const unsigned char*>(P.pieces);
+        work.sb = work.pieces + int64_t(P.tokens) * Work::kPieces * work.pitch;
         work.blocks = int(mx_blocks(P.hidden));
         work.cols = P.hidden;
         work.rows_a = int64_t(P.experts) * P.inter;
@@ -246,7 +279,9 @@ __global__ void __launch_bounds__(Wide<DownWork<T, MX>>::kThreads, 1)
     Work work;
     work.sa[0] = work.sa[1] = P.s[2];
     work.sb = static_cast<const unsigned char*>(P.h) + int64_t(P.tokens) * P.topk * 3 * P.h_pitch;
-    work.blocks = int(mx_blocks(P.inter));
+    work.blocks = work.pitch_b = int(mx_blocks(P.inter));
+    work.pitch = 0;
+    work.pieces = nullptr;
     work.cols = P.inter;
     work.rows_a = int64_t(P.experts) * P.hidden;
     work.x_aligned = true;
@@ -284,14 +319,14 @@ __global__ void __launch_bounds__(Wide<DownWork<T, MX>>::kThreads, 1)
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-template <typename T, bool MX>
+template <typename T, bool MX, bool SPLIT>
 int launch_moe_wide(const MoeParams& P, cudaStream_t stream) {
     static std::atomic<uint64_t> gate_set{0}, down_set{0};
     const int sms = sm_count();
     if (sms <= 0) return check_launch();
-    using G = GateShape<T, MX>;
+    using G = GateShape<T, MX, SPLIT>;
     using D = DownShape<T, MX>;
-    auto gate = moe_gate_kernel<T, MX>;
+    auto gate = moe_gate_kernel<T, MX, SPLIT>;
     auto down = moe_down_kernel<T, MX>;
     if (int rc = allow_smem(gate, gate_set, G::kSmem)) return rc;
     if (int rc = allow_smem(down, down_set, D::kSmem)) return rc;
@@ -346,8 +381,13 @@ bool moe_wide_takes(const MoeParams& P, bool mx) {
 }
 
 int moe_wide(int type, bool mx, const MoeParams& P, cudaStream_t stream) {
-    if (type == SWB_F16) return mx ? launch_moe_wide<__half, true>(P, stream) : launch_moe_wide<__half, false>(P, stream);
-    return mx ? launch_moe_wide<__nv_bfloat16, true>(P, stream) : launch_moe_wide<__nv_bfloat16, false>(P, stream);
+    const bool half = type == SWB_F16;
+    if (!mx) return half ? launch_moe_wide<__half, false, false>(P, stream) : launch_moe_wide<__nv_bfloat16, false, false>(P, stream);
+    // longer tokens than the workspace's pieces are split at each use: every item of an expert repeats
+    // the conversions (four-bit experts of 14336 x 4096, 32 tokens: 330 us of gate against 190)
+    if (P.hidden > kMoePieceDim)
+        return half ? launch_moe_wide<__half, true, true>(P, stream) : launch_moe_wide<__nv_bfloat16, true, true>(P, stream);
+    return half ? launch_moe_wide<__half, true, false>(P, stream) : launch_moe_wide<__nv_bfloat16, true, false>(P, stream);
 }
 
 }  // namespace swb

@@ -29,16 +29,15 @@ namespace {
 template <typename T_, int TOK>
 struct ProjectWork {
     using T = T_;
-    static constexpr bool kMx = true, kLoad = true;
+    static constexpr bool kMx = true, kLoad = true, kGather = false;
     static constexpr int kPieces = std::is_same<T, __half>::value ? 3 : 2;
     static constexpr int kTok = TOK, kAccs = 1;
     static constexpr int kPerSm = TOK == 16 ? 2 : 1;
     static constexpr int kStages = TOK == 16 ? 2 : 4, kRaw = TOK == 16 ? 3 : 4;
-    static constexpr int kTokenStages = TOK == 16 ? 4 : TOK == 32 ? 6 : 2;
+    static constexpr int kSpreadGroups = 1, kTokenStages = TOK == 16 ? 4 : TOK == 32 ? 6 : 2;
     static constexpr int kSplitters = TOK == 16 ? 4 : TOK == 32 ? 6 : 8, kGroupWarps = TOK == 64 ? 4 : 1;
 
     const unsigned char* sa[2];
-    const unsigned char* sb;
     int blocks, cols;
     int64_t rows_a;
     bool x_aligned;
@@ -84,7 +83,6 @@ __global__ void __launch_bounds__(Wide<ProjectWork<T, TOK>>::kThreads, ProjectWo
 
     Work work;
     work.sa[0] = work.sa[1] = P.s;
-    work.sb = nullptr;
     work.halves = 2;
     work.blocks = int(mx_blocks(P.cols));
     work.cols = P.cols;

@@ -12,7 +12,7 @@
 // Roles of a CTA, through two rings of stages of 128 bytes of every row (one for the weights, one
 // for the tokens):
 //   copies     one thread, TMA: two halves of 64 rows of W (gate and up rows, or neighbours)
-//   spreaders  (four-bit) four warps. Codes arrive packed in a ring of their own, 16 KB a stage, the
+//   spreaders  (four-bit) one or two groups of four warps, stage about. Codes arrive packed in a ring of their own, 16 KB a stage, the
 //              bytes in flight, and are spread to the eight bytes of every sixteen that the product
 //              reads; their scales go into the 32 x 16-byte blocks that tcgen05.cp spreads over
 //              TMEM. (The copy engine can spread codes too, at about the same rate.)
@@ -138,6 +138,19 @@ __device__ __forceinline__ uint32_t scale_place(int r) {
     return uint32_t((r >> 7) * kScaleBlock + (r & 31) * 16 + ((r >> 5) & 3) * 4);
 }
 
+// Whether a phase has completed, without waiting.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
 // One piece of work: 128 rows of W (two halves of 64) by `count` tokens over stages [s0, s1).
 struct WideItem {
     int64_t row[2];  // first row of each half in its tensor
@@ -148,9 +161,10 @@ struct WideItem {
 
 // W describes the work:
 //   types      T; kMx; kPieces; kTok (tokens of an item, a multiple of 16); kLoad (tokens by the
-//              splitters; else rows `first * kPieces` on of a tensor map, and for four-bit weights
-//              scales `sb`); kAccs; kStages and kTokenStages (of the rings); kRaw (stages of packed
-//              codes); kSplitters (warps) in groups of kGroupWarps; kPerSm
+//              splitters; else rows `first * kPieces` on of a tensor map, or with kGather rows
+//              place(it, n) * kPieces on of `pieces`, `pitch` bytes apart, and for four-bit
+//              weights scales `sb`, `pitch_b` apart); kAccs; kStages and kTokenStages (of the rings); kRaw (stages of packed
+//              codes); kSpreadGroups; kSplitters (warps) in groups of kGroupWarps; kPerSm
 //   item(i, it) -> false past the last one;  token(it, n): row of token n (kLoad)
 //   halves: 1 or 2 of 64 rows;  scales of W: sa[2], blocks, rows_a;  x_aligned, cols
 //   begin(it) / value(it, n, row, v) / end(it): epilogue threads, by their row
@@ -168,11 +182,12 @@ struct Wide {
     static constexpr int kColumns = kUsed <= 32 ? 32 : kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
     static constexpr int kValues = kMx ? 128 : 64;   // of a row in a stage
     static constexpr int kRawStage = kMx ? kWideM * 128 : 0, kRaw = kMx ? W::kRaw : 0;
-    static constexpr int kSpreaders = kMx ? 4 : 0, kSplitters = W::kSplitters, kGroupWarps = W::kGroupWarps;
+    static constexpr int kSpreadGroups = kMx ? W::kSpreadGroups : 0, kSpreaders = 4 * kSpreadGroups, kSplitters = W::kSplitters, kGroupWarps = W::kGroupWarps;
     static constexpr int kGroups = kSplitters / kGroupWarps;
     static constexpr int kWarps = kWideEpilogue + kSpreaders + kSplitters + 2, kThreads = kWarps * 32;
     static_assert(kUsed <= 512 && kColumns * W::kPerSm <= 512, "TMEM columns");
     static_assert(W::kLoad || kGroupWarps == 1, "a warp brings prepared tokens");
+    static_assert(!W::kGather || kMx, "gathered rows are pieces");
     // a group that waits for a stage of tokens is at most one round of the ring ahead of its readers
     static_assert(kGroups <= W::kTokenStages, "groups do not overtake the ring");
 
@@ -219,7 +234,7 @@ struct Wide {
         if (threadIdx.x == 0) {
             s.failed = 0;
             for (int i = 0; i < W::kStages; ++i) {
-                mbar_init(smem_u32(s.full + i), kMx ? kSpreaders : 1);
+                mbar_init(smem_u32(s.full + i), kMx ? 4 : 1);
                 mbar_init(smem_u32(s.empty + i), 1);
             }
             for (int i = 0; i < W::kTokenStages; ++i) {
@@ -307,20 +322,28 @@ struct Wide {
         Ring<W::kTokenStages> b;
         Ring<W::kAccs> acc;
         WideItem it;
+        // a stage's barriers are asked for while the stage before is being issued
+        bool have_a = false, have_b = false;
         for (int i = 0; work.item(i, it); ++i) {
             const int n = columns(it.count);
             if (!acc.free(sh.acc_empty)) return false;  // the accumulator's last item has been read
             for (int k = it.s0; k < it.s1; ++k) {
-                if (!mbar_wait(smem_u32(sh.full + a.s), a.ph) || !mbar_wait(smem_u32(sh.tokens_full + b.s), b.ph)) return false;
+                if (!have_a && !mbar_wait(smem_u32(sh.full + a.s), a.ph)) return false;
+                if (!have_b && !mbar_wait(smem_u32(sh.tokens_full + b.s), b.ph)) return false;
+                const int as = a.s, bs = b.s;
+                a.next();
+                b.next();
+                have_a = mbar_test(smem_u32(sh.full + a.s), a.ph);
+                have_b = mbar_test(smem_u32(sh.tokens_full + b.s), b.ph);
                 fence_after();
-                const uint32_t ca = columns_a + a.s * kScaleColumnsA, cb = columns_b + b.s * kScaleColumnsB;
+                const uint32_t ca = columns_a + as * kScaleColumnsA, cb = columns_b + bs * kScaleColumnsB;
                 if constexpr (kMx) {
-                    scale_copy(ca, scale_desc(base + kAtScalesA + a.s * kScaleBlock));
+                    scale_copy(ca, scale_desc(base + kAtScalesA + as * kScaleBlock));
 #pragma unroll
                     for (int j = 0; j < kBlocksB; ++j)
-                        scale_copy(cb + 4 * j, scale_desc(base + kAtScalesB + (b.s * kBlocksB + j) * kScaleBlock));
+                        scale_copy(cb + 4 * j, scale_desc(base + kAtScalesB + (bs * kBlocksB + j) * kScaleBlock));
                 }
-                const uint64_t da = operand_desc(base + a.s * kStageA), db = operand_desc(base + kAtB + b.s * kStageB);
+                const uint64_t da = operand_desc(base + as * kStageA), db = operand_desc(base + kAtB + bs * kStageB);
                 const uint32_t d = tmem + acc.s * kN;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -329,11 +352,9 @@ struct Wide {
                     else
                         mma_f16(d, da + 2 * j, db + 2 * j, f16_desc<T>(kWideM, n), k > it.s0 || j > 0);
                 }
-                mma_commit(smem_u32(sh.empty + a.s));
-                mma_commit(smem_u32(sh.tokens_empty + b.s));
+                mma_commit(smem_u32(sh.empty + as));
+                mma_commit(smem_u32(sh.tokens_empty + bs));
                 if (k == it.s1 - 1) mma_commit(smem_u32(sh.acc_full + acc.s));
-                a.next();
-                b.next();
             }
             acc.next();
         }
@@ -375,10 +396,10 @@ struct Wide {
         return true;
     }
 
-    // Spreaders: codes and scales of W. Windows of 16 scale bytes, four stages each, two windows
-    // ahead: they come from DRAM.
+    // Spreaders: codes and scales of W; a group of four warps takes every other stage. Scale bytes
+    // come in windows of 16, four stages each, two windows ahead, since they come from DRAM.
     static __device__ __forceinline__ bool spread(W& work, Shared& sh, uint32_t base) {
-        const int t = threadIdx.x - kWideEpilogue * 32, lane = t & 31, half = t / kWideHalf;
+        const int group = threadIdx.x / 128 - kWideEpilogue / 4, t = threadIdx.x % 128, lane = t & 31, half = t / kWideHalf;
         Ring<W::kStages> ring;
         Ring<kRaw> raw;
         WideItem it;
@@ -398,26 +419,28 @@ struct Wide {
                     window[0] = window[1], window[1] = window[2];
                     load(2, k + 8);
                 }
-                const bool first = k == it.s0 || k % 2 == 0;
-                const bool ready = ring.free(sh.empty) && (!first || mbar_wait(smem_u32(sh.raw_full + raw.s), raw.ph));
-                if (!__all_sync(0xFFFFFFFFu, ready)) return false;
-                // a warp takes eight rows, four blocks of 16 bytes each, at a time
-                const uint32_t from = base + kAtRaw + raw.s * kRawStage, to = base + ring.s * kStageA;
-                const int block = lane >> 3;
-                uint4 c[4];
+                // every warp waits for each raw stage, so that none arrives at its end a round early
+                if ((k == it.s0 || k % 2 == 0) && !mbar_wait_warp(smem_u32(sh.raw_full + raw.s), raw.ph)) return false;
+                if (ring.issued % kSpreadGroups == group) {
+                    if (!__all_sync(0xFFFFFFFFu, ring.free(sh.empty))) return false;
+                    // a warp takes eight rows, four blocks of 16 bytes each, at a time
+                    const uint32_t from = base + kAtRaw + raw.s * kRawStage, to = base + ring.s * kStageA;
+                    const int block = lane >> 3;
+                    uint4 c[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) c[u] = lds128(from + swizzled((t / 32 + u * 4) * 8 + (lane & 7), k % 2 * 4 + block));
+                    for (int u = 0; u < 4; ++u) c[u] = lds128(from + swizzled((t / 32 + u * 4) * 8 + (lane & 7), k % 2 * 4 + block));
+                    const uint4& w = window[0];
+                    sts32(base + kAtScalesA + ring.s * kScaleBlock + scale_place(t), k & 2 ? (k & 1 ? w.w : w.z) : (k & 1 ? w.y : w.x));
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int q = (t / 32 + u * 4) * 8 + (lane & 7);
-                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to + swizzled(q, 2 * block)), "r"(c[u].x), "r"(c[u].y) : "memory");
-                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to + swizzled(q, 2 * block + 1)), "r"(c[u].z), "r"(c[u].w) : "memory");
+                    for (int u = 0; u < 4; ++u) {
+                        const int q = (t / 32 + u * 4) * 8 + (lane & 7);
+                        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to + swizzled(q, 2 * block)), "r"(c[u].x), "r"(c[u].y) : "memory");
+                        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to + swizzled(q, 2 * block + 1)), "r"(c[u].z), "r"(c[u].w) : "memory");
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(sh.full + ring.s));
                 }
-                const uint4& w = window[0];
-                sts32(base + kAtScalesA + ring.s * kScaleBlock + scale_place(t), k & 2 ? (k & 1 ? w.w : w.z) : (k & 1 ? w.y : w.x));
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(sh.full + ring.s));
                 ring.next();
                 if (k % 2 == 1 || k + 1 == it.s1) {
                     if (lane == 0) mbar_arrive(smem_u32(sh.raw_empty + raw.s));
@@ -499,40 +522,52 @@ struct Wide {
         return true;
     }
 
-    // Prepared tokens: a warp brings a stage's rows by TMA, their scale words by plain loads.
+    // Prepared tokens: a warp brings a stage's rows, by TMA or (gathered) by asynchronous copies, and
+    // their scale words by plain loads.
     static __device__ __forceinline__ bool bring(W& work, Shared& sh, uint32_t base, const CUtensorMap* map_b) {
         const int lane = threadIdx.x & 31, group = threadIdx.x / 32 - kWideEpilogue - kSpreaders;
         Ring<W::kTokenStages> ring;
         WideItem it;
         for (int i = 0; work.item(i, it); ++i) {
-            const int n = columns(it.count);
+            const int n = columns(it.count), rows = it.count * W::kPieces;
             for (int k = it.s0; k < it.s1; ++k) {
                 if (ring.issued % kGroups == group) {
                     if (!__all_sync(0xFFFFFFFFu, ring.free(sh.tokens_empty))) {
-                        if (lane == 0) ring.drain(sh.tokens_full);
+                        if (!W::kGather && lane == 0) ring.drain(sh.tokens_full);
                         return false;
                     }
                     const uint32_t bar = smem_u32(sh.tokens_full + ring.s), b = base + kAtB + ring.s * kStageB;
+                    if constexpr (W::kGather) {  // eight lanes a row
+                        for (int r = lane / 8; r < rows; r += 4) {
+                            const int64_t from = int64_t(work.place(it, r / W::kPieces)) * W::kPieces + r % W::kPieces;
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(b + swizzled(r, lane & 7)),
+                                         "l"(work.pieces + from * work.pitch + k * kWideRowBytes + (lane & 7) * 16) : "memory");
+                        }
+                    }
                     if constexpr (kMx) {
 #pragma unroll
                         for (int u = 0; u < (kN + 31) / 32; ++u) {
                             const int r = lane + 32 * u;
-                            if (r >= it.count * W::kPieces) continue;
-                            const unsigned char* row = work.sb + int64_t(it.first * W::kPieces + r) * work.blocks;
+                            if (r >= rows) continue;
+                            const int64_t from = (W::kGather ? int64_t(work.place(it, r / W::kPieces)) : int64_t(it.first + r / W::kPieces)) * W::kPieces + r % W::kPieces;
+                            const unsigned char* row = work.sb + from * work.pitch_b;
                             uint32_t w = 0u;
-                            if ((work.blocks & 3) == 0) {
+                            if ((work.pitch_b & 3) == 0) {
                                 w = *reinterpret_cast<const uint32_t*>(row + k * 4);
                             } else {
 #pragma unroll
                                 for (int e = 0; e < 4; ++e)
-                                    if (k * 4 + e < work.blocks) w |= uint32_t(row[k * 4 + e]) << (8 * e);
+                                    if (k * 4 + e < work.pitch_b) w |= uint32_t(row[k * 4 + e]) << (8 * e);
                             }
                             sts32(base + kAtScalesB + ring.s * kBlocksB * kScaleBlock + scale_place(r), w);
                         }
+                        if (W::kGather) asm volatile("cp.async.wait_all;" ::: "memory");
                         fence_proxy_async_smem();
                         __syncwarp();
                     }
-                    if (elect_one()) {
+                    if constexpr (W::kGather) {
+                        if (lane == 0) mbar_arrive(bar);
+                    } else if (elect_one()) {
                         mbar_arrive_expect_tx(bar, n * kWideRowBytes);
                         for (int r = 0; r < n; r += 16)
                             tma_load_2d(b + r * kWideRowBytes, map_b, k * kValues, it.first * W::kPieces + r, bar);
