@@ -46,6 +46,7 @@ constexpr int kMmaM = 128;
 constexpr int kRowBytes = 128;     // of a row in a stage: 256 values, 8 scales
 constexpr int kWindow = 16;        // scale bytes of a row that a thread loads at once: two stages
 constexpr int kEpilogueWarps = 4, kScaleWarps = 4;
+constexpr int kTurnColumns = 64, kTurnPitch = kTurnColumns + 2;  // floats of a row in the epilogue
 constexpr int kThreads = (kEpilogueWarps + kScaleWarps + 2) * 32;
 
 struct MatmulParams {
@@ -65,13 +66,14 @@ struct MatmulParams {
 
 template <int N, int MT, bool TOKENS_M>
 struct MatmulShape {
-    static constexpr int kStages = TOKENS_M ? (MT == 2 ? 3 : 5) : (N <= 32 ? 5 : 4);
+    static constexpr int kStages = TOKENS_M ? (MT == 2 ? 3 : 4) : (N <= 32 ? 5 : 4);
     static constexpr int kPerSm = TOKENS_M || N > 64 ? 1 : 2;
     static constexpr int kRowsA = MT * kMmaM;
     static constexpr int kBytesA = kRowsA * kRowBytes, kBytesB = N * kRowBytes;
     static constexpr int kBlocksB = (N + kMmaM - 1) / kMmaM;   // 128-row blocks of scales of the N side
     static constexpr int kScales = 2 * (MT + kBlocksB) * kScaleBlock;
     static constexpr int kStage = kBytesA + kBytesB + kScales;
+    static_assert(!TOKENS_M || N % kTurnColumns == 0, "whole turns");
     static_assert(kStage % 1024 == 0, "stages keep the swizzle's alignment");
     static constexpr int kAccs = TOKENS_M ? 2 : 1;             // accumulators of N columns
     static constexpr int kScaleColumns = 2 * (MT + kBlocksB) * 4;
@@ -80,7 +82,8 @@ struct MatmulShape {
     static_assert(kUsed <= 512, "TMEM columns");
     static constexpr int kPartPitch = kMmaM + 1;               // floats of a token's column in the exchange
     static constexpr int kExchange = TOKENS_M ? 0 : N * kPartPitch * 4;
-    static constexpr size_t kSmem = size_t(kStages) * kStage + 1024;  // the exchange reuses the stages
+    static constexpr int kTurn = TOKENS_M ? kEpilogueWarps * 32 * kTurnPitch * 4 : 0;  // the epilogue's tiles
+    static constexpr size_t kSmem = size_t(kStages) * kStage + kTurn + 1024;  // the exchange reuses the stages
     static_assert(kExchange <= kStages * kStage, "exchange fits the stages");
     static_assert(kColumns * kPerSm <= 512, "CTAs of an SM share TMEM");
     static_assert((kSmem + 2048) * kPerSm <= kSmemPerSm, "CTAs of an SM share its shared memory");
@@ -278,51 +281,80 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
             for (int m = 0; m < MT; ++m) {
                 const int use = MT == 2 ? m : acc;
+                // the residual's values for 64 columns of this warp's tokens, on their way before the
+                // accumulator is waited for
+                uint32_t residual[32];
+                const int64_t token0 = a0 + m * kMmaM + warp * 32;
+                const int tokens = int(min(int64_t(32), P.tokens - token0));
+                auto load_residual = [&](int c) {
+                    if (!TOKENS_M || !P.residual) return;
+                    const int64_t row = b0 + c + 2 * lane;
+#pragma unroll
+                    for (int u = 0; u < 32; ++u) {
+                        const T* r = static_cast<const T*>(P.residual) + (token0 + u) * P.rows + row;
+                        residual[u] = 0u;
+                        if (u < tokens && row < P.rows) {
+                            if (row + 1 < P.rows && (reinterpret_cast<uintptr_t>(r) & 3) == 0) {
+                                residual[u] = *reinterpret_cast<const uint32_t*>(r);
+                            } else {
+                                residual[u] = *reinterpret_cast<const unsigned short*>(r);
+                                if (row + 1 < P.rows) residual[u] |= uint32_t(reinterpret_cast<const unsigned short*>(r)[1]) << 16;
+                            }
+                        }
+                    }
+                };
+                load_residual(0);
                 ok = mbar_wait_warp(smem_u32(acc_full + use), ph);
                 if (!ok) break;
                 fence_after();
                 const int in_tile = m * kMmaM + warp * 32 + lane;
                 if constexpr (TOKENS_M) {
-                    const int64_t token = a0 + in_tile;
-                    const bool wide = P.rows % 8 == 0 && (reinterpret_cast<uintptr_t>(P.out) & 15) == 0 &&
-                                      (reinterpret_cast<uintptr_t>(P.residual) & 15) == 0;
+                    // A lane holds a token's columns; through shared memory, so that a warp writes 64
+                    // neighbouring values of one token at a time (a lane storing its own token's 16
+                    // bytes took 40 % of the kernel, single values of ragged rows 80 %).
+                    float* turn = reinterpret_cast<float*>(raw + (base - smem_u32(raw)) + S::kStages * S::kStage) + warp * 32 * kTurnPitch;
 #pragma unroll 1
-                    for (int c = 0; c < N; c += 32) {
-                        uint32_t v[32];
+                    for (int c = 0; c < N; c += kTurnColumns) {
+                        if (c > 0) load_residual(c);
+                        __syncwarp();  // the last columns are read
+#pragma unroll
+                        for (int h = 0; h < kTurnColumns; h += 32) {
+                            uint32_t v[32];
+                            tmem_load32(tmem + quadrant + use * N + c + h, v);
+                            tmem_load_wait();
+#pragma unroll
+                            for (int j = 0; j < 32; j += 2)
+                                *reinterpret_cast<float2*>(turn + lane * kTurnPitch + h + j) =
+                                    make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+                        }
                         __syncwarp();
-                        tmem_load32(tmem + quadrant + use * N + c, v);
-                        tmem_load_wait();
-                        if (token >= P.tokens) continue;
-                        const int64_t row0 = b0 + c, at = token * P.rows + row0;
-                        T* out = static_cast<T*>(P.out) + at;
+                        const int64_t row = b0 + c + 2 * lane;  // this lane's two columns
+                        float2 bias = make_float2(0.f, 0.f);
+                        if (P.bias) {
+                            if (row < P.rows) bias.x = load_value<T>(P.bias, row);
+                            if (row + 1 < P.rows) bias.y = load_value<T>(P.bias, row + 1);
+                        }
 #pragma unroll
-                        for (int j = 0; j < 32; j += 8) {
-                            if (row0 + j >= P.rows) break;
-                            float f[8];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[j + e]);
-                            if (wide) {
-                                if (P.bias) {
-#pragma unroll
-                                    for (int e = 0; e < 8; ++e) f[e] += load_value<T>(P.bias, row0 + j + e);
-                                }
-                                if (P.residual) {
-                                    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const T*>(P.residual) + at + j);
-#pragma unroll
-                                    for (int e = 0; e < 8; ++e) f[e] += Num<T>::to_float(reinterpret_cast<const T*>(&q)[e]);
-                                }
-                                uint4 q;
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(&q)[e] = Num<T>::from_float(f[e]);
-                                *reinterpret_cast<uint4*>(out + j) = q;
+                        for (int u = 0; u < 32; ++u) {
+                            if (u >= tokens) break;
+                            float2 v = *reinterpret_cast<const float2*>(turn + u * kTurnPitch + 2 * lane);
+                            T two[2];
+                            if (P.residual) {
+                                *reinterpret_cast<uint32_t*>(two) = residual[u];
+                                v.x += bias.x + Num<T>::to_float(two[0]);
+                                v.y += bias.y + Num<T>::to_float(two[1]);
                             } else {
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    if (row0 + j + e >= P.rows) break;
-                                    if (P.bias) f[e] += load_value<T>(P.bias, row0 + j + e);
-                                    if (P.residual) f[e] += load_value<T>(P.residual, at + j + e);
-                                    out[j + e] = Num<T>::from_float(f[e]);
-                                }
+                                v.x += bias.x;
+                                v.y += bias.y;
+                            }
+                            two[0] = Num<T>::from_float(v.x);
+                            two[1] = Num<T>::from_float(v.y);
+                            T* o = static_cast<T*>(P.out) + (token0 + u) * P.rows + row;
+                            if (row + 1 < P.rows && (reinterpret_cast<uintptr_t>(o) & 3) == 0) {
+                                *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(two);
+                            } else {
+                                if (row < P.rows) o[0] = two[0];
+                                if (row + 1 < P.rows) o[1] = two[1];
                             }
                         }
                     }
