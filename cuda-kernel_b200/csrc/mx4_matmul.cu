@@ -45,8 +45,8 @@ namespace {
 constexpr int kMmaM = 128;
 constexpr int kRowBytes = 128;     // of a row in a stage: 256 values, 8 scales
 constexpr int kWindow = 16;        // scale bytes of a row that a thread loads at once: two stages
-constexpr int kEpilogueWarps = 4, kScaleWarps = 4;
-constexpr int kTurnColumns = 64, kTurnPitch = kTurnColumns + 2;  // floats of a row in the epilogue
+constexpr int kEpilogueWarps = 8, kScaleWarps = 4;  // epilogue: two warps a TMEM quadrant
+constexpr int kTurnColumns = 32, kTurnPitch = kTurnColumns + 2;  // floats of a row in the epilogue
 constexpr int kThreads = (kEpilogueWarps + kScaleWarps + 2) * 32;
 
 struct MatmulParams {
@@ -95,7 +95,7 @@ __device__ __forceinline__ float load_value(const void* p, int64_t i) {
 }
 
 template <typename T, int N, int MT, bool TOKENS_M>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, MatmulShape<N, MT, TOKENS_M>::kPerSm)
     matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const MatmulParams P) {
     using S = MatmulShape<N, MT, TOKENS_M>;
@@ -214,7 +214,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp >= kEpilogueWarps) {
         // ------------------------------------------------------- scales
         constexpr int kRows = S::kRowsA + N, kPer = (kRows + 127) / 128;
-        const int t = threadIdx.x - kEpilogueWarps * 32;
+        // A warp's lanes take rows 8 apart in four quarters of 128: their words lie side by side.
+        const int lt = threadIdx.x - kEpilogueWarps * 32, t = lt / 32 * 8 + (lt & 7) + (lt >> 3 & 3) * 32;
         int s = 0, issued = 0;
         uint32_t ph = 0;
         bool ok = true;
@@ -234,20 +235,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // blocks of the M side: [128 values][128 rows], then the N side's
                 dst[i] = (in_a ? q >> 7 : 2 * MT + (q >> 7)) * kScaleBlock + (in & 31) * 16 + (in >> 5) * 4;
             }
-            uint4 next[kPer];
-            auto load = [&](int k) {  // the window that holds stage k's scales
+            // two windows ahead: scales of long rows come from L2 or DRAM
+            uint4 window[3][kPer];
+            auto load = [&](int w, int k) {  // the window that holds stage k's scales
 #pragma unroll
                 for (int i = 0; i < kPer; ++i)
-                    next[i] = row[i] ? load_scales(row[i], k * 8 & ~(kWindow - 1), P.blocks) : make_uint4(0u, 0u, 0u, 0u);
+                    window[w][i] = row[i] && k < k1 ? load_scales(row[i], k * 8 & ~(kWindow - 1), P.blocks) : make_uint4(0u, 0u, 0u, 0u);
             };
-            load(k0);
-            uint4 now[kPer];
+            load(0, k0);
+            load(1, (k0 | 1) + 1);
+            load(2, (k0 | 1) + 3);
             for (int k = k0; k < k1; ++k) {
-                if (k == k0 || (k & 1) == 0) {
+                if (k > k0 && (k & 1) == 0) {
 #pragma unroll
-                    for (int i = 0; i < kPer; ++i) now[i] = next[i];
-                    const int then = (k | 1) + 1;
-                    if (then < k1) load(then);
+                    for (int i = 0; i < kPer; ++i) window[0][i] = window[1][i], window[1][i] = window[2][i];
+                    load(2, k + 4);
                 }
                 if (issued >= S::kStages && !mbar_wait(smem_u32(empty + s), ph ^ 1u)) {
                     ok = false;
@@ -259,8 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int r = t + 128 * i;
                     if (r < kRows) {
                         const uint32_t next_block = (r < S::kRowsA ? MT : S::kBlocksB) * kScaleBlock;
-                        sts32(sc + dst[i], k & 1 ? now[i].z : now[i].x);
-                        sts32(sc + dst[i] + next_block, k & 1 ? now[i].w : now[i].y);
+                        sts32(sc + dst[i], k & 1 ? window[0][i].z : window[0][i].x);
+                        sts32(sc + dst[i] + next_block, k & 1 ? window[0][i].w : window[0][i].y);
                     }
                 }
                 fence_proxy_async_smem();
@@ -275,86 +277,91 @@ __global__ void __launch_bounds__(kThreads, 1)
         int acc = 0;
         uint32_t ph = 0;
         bool ok = true;
-        const uint32_t quadrant = uint32_t(warp * 32) << 16;
+        const int quarter = warp % 4, share = warp / 4;  // this warp takes every other group of columns
+        const uint32_t quadrant = uint32_t(quarter * 32) << 16;
         for (int64_t tile = first; tile < P.tiles && ok; tile += step) {
             const int64_t a0 = tile % P.tiles_a * S::kRowsA, b0 = tile / P.tiles_a * N;
 #pragma unroll 1
             for (int m = 0; m < MT; ++m) {
                 const int use = MT == 2 ? m : acc;
-                // the residual's values for 64 columns of this warp's tokens, on their way before the
-                // accumulator is waited for
-                uint32_t residual[32];
-                const int64_t token0 = a0 + m * kMmaM + warp * 32;
+                // The residual's values for 32 columns of this warp's tokens (a lane: two columns of every
+                // other token), on their way before the accumulator is waited for, the next
+                // ones before these are written.
+                uint32_t residual[16], ahead[16];
+                const int64_t token0 = a0 + m * kMmaM + quarter * 32 + lane / 16;
                 const int tokens = int(min(int64_t(32), P.tokens - token0));
                 auto load_residual = [&](int c) {
                     if (!TOKENS_M || !P.residual) return;
-                    const int64_t row = b0 + c + 2 * lane;
+                    const int64_t row = b0 + c + lane % 16 * 2;
+                    const T* r = static_cast<const T*>(P.residual) + token0 * P.rows + row;
+                    const bool have0 = row < P.rows, have1 = row + 1 < P.rows;
 #pragma unroll
-                    for (int u = 0; u < 32; ++u) {
-                        const T* r = static_cast<const T*>(P.residual) + (token0 + u) * P.rows + row;
-                        residual[u] = 0u;
-                        if (u < tokens && row < P.rows) {
-                            if (row + 1 < P.rows && (reinterpret_cast<uintptr_t>(r) & 3) == 0) {
-                                residual[u] = *reinterpret_cast<const uint32_t*>(r);
+                    for (int u = 0; u < 16; ++u, r += 2 * P.rows) {
+                        ahead[u] = 0u;
+                        if (2 * u < tokens && have0) {
+                            if (have1 && (reinterpret_cast<uintptr_t>(r) & 3) == 0) {
+                                ahead[u] = *reinterpret_cast<const uint32_t*>(r);
                             } else {
-                                residual[u] = *reinterpret_cast<const unsigned short*>(r);
-                                if (row + 1 < P.rows) residual[u] |= uint32_t(reinterpret_cast<const unsigned short*>(r)[1]) << 16;
+                                ahead[u] = *reinterpret_cast<const unsigned short*>(r);
+                                if (have1) ahead[u] |= uint32_t(reinterpret_cast<const unsigned short*>(r)[1]) << 16;
                             }
                         }
                     }
                 };
-                load_residual(0);
+                load_residual(share * kTurnColumns);
                 ok = mbar_wait_warp(smem_u32(acc_full + use), ph);
                 if (!ok) break;
                 fence_after();
-                const int in_tile = m * kMmaM + warp * 32 + lane;
+                const int in_tile = m * kMmaM + quarter * 32 + lane;
                 if constexpr (TOKENS_M) {
-                    // A lane holds a token's columns; through shared memory, so that a warp writes 64
+                    // A lane holds a token's columns; through shared memory, so that half a warp writes 32
                     // neighbouring values of one token at a time (a lane storing its own token's 16
                     // bytes took 40 % of the kernel, single values of ragged rows 80 %).
                     float* turn = reinterpret_cast<float*>(raw + (base - smem_u32(raw)) + S::kStages * S::kStage) + warp * 32 * kTurnPitch;
 #pragma unroll 1
-                    for (int c = 0; c < N; c += kTurnColumns) {
-                        if (c > 0) load_residual(c);
-                        __syncwarp();  // the last columns are read
+                    for (int c = share * kTurnColumns; c < N; c += 2 * kTurnColumns) {
+                        if (P.residual) {
 #pragma unroll
-                        for (int h = 0; h < kTurnColumns; h += 32) {
-                            uint32_t v[32];
-                            tmem_load32(tmem + quadrant + use * N + c + h, v);
-                            tmem_load_wait();
-#pragma unroll
-                            for (int j = 0; j < 32; j += 2)
-                                *reinterpret_cast<float2*>(turn + lane * kTurnPitch + h + j) =
-                                    make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+                            for (int u = 0; u < 16; ++u) residual[u] = ahead[u];
+                            if (c + 2 * kTurnColumns < N) load_residual(c + 2 * kTurnColumns);
                         }
+                        uint32_t v[32];
+                        __syncwarp();  // the last columns are read
+                        tmem_load32(tmem + quadrant + use * N + c, v);
+                        tmem_load_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2)
+                            *reinterpret_cast<float2*>(turn + lane * kTurnPitch + j) =
+                                make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
                         __syncwarp();
-                        const int64_t row = b0 + c + 2 * lane;  // this lane's two columns
+                        const int64_t row = b0 + c + lane % 16 * 2;  // this lane's two columns
+                        const bool have0 = row < P.rows, have1 = row + 1 < P.rows;
                         float2 bias = make_float2(0.f, 0.f);
                         if (P.bias) {
-                            if (row < P.rows) bias.x = load_value<T>(P.bias, row);
-                            if (row + 1 < P.rows) bias.y = load_value<T>(P.bias, row + 1);
+                            if (have0) bias.x = load_value<T>(P.bias, row);
+                            if (have1) bias.y = load_value<T>(P.bias, row + 1);
                         }
+                        T* o = static_cast<T*>(P.out) + token0 * P.rows + row;
+                        const float* from = turn + lane / 16 * kTurnPitch + lane % 16 * 2;
 #pragma unroll
-                        for (int u = 0; u < 32; ++u) {
-                            if (u >= tokens) break;
-                            float2 v = *reinterpret_cast<const float2*>(turn + u * kTurnPitch + 2 * lane);
+                        for (int u = 0; u < 16; ++u, o += 2 * P.rows) {
+                            if (2 * u >= tokens) break;
+                            float2 f = *reinterpret_cast<const float2*>(from + 2 * u * kTurnPitch);
                             T two[2];
+                            f.x += bias.x;
+                            f.y += bias.y;
                             if (P.residual) {
                                 *reinterpret_cast<uint32_t*>(two) = residual[u];
-                                v.x += bias.x + Num<T>::to_float(two[0]);
-                                v.y += bias.y + Num<T>::to_float(two[1]);
-                            } else {
-                                v.x += bias.x;
-                                v.y += bias.y;
+                                f.x += Num<T>::to_float(two[0]);
+                                f.y += Num<T>::to_float(two[1]);
                             }
-                            two[0] = Num<T>::from_float(v.x);
-                            two[1] = Num<T>::from_float(v.y);
-                            T* o = static_cast<T*>(P.out) + (token0 + u) * P.rows + row;
-                            if (row + 1 < P.rows && (reinterpret_cast<uintptr_t>(o) & 3) == 0) {
+                            two[0] = Num<T>::from_float(f.x);
+                            two[1] = Num<T>::from_float(f.y);
+                            if (have1 && (reinterpret_cast<uintptr_t>(o) & 3) == 0) {
                                 *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(two);
                             } else {
-                                if (row < P.rows) o[0] = two[0];
-                                if (row + 1 < P.rows) o[1] = two[1];
+                                if (have0) o[0] = two[0];
+                                if (have1) o[1] = two[1];
                             }
                         }
                     }
@@ -362,8 +369,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // a column is a token, a lane a row of W: to shared memory, [token][row]
                     float* part = reinterpret_cast<float*>(raw + (base - smem_u32(raw)));
 #pragma unroll 1
-                    for (int c = 0; c < N; c += 16) {
+                    for (int c = share * 16; c < N; c += 32) {
                         uint32_t v[16];
+                        __syncwarp();
                         tmem_load16(tmem + quadrant + use * N + c, v);
                         tmem_load_wait();
 #pragma unroll

@@ -399,12 +399,14 @@ struct Wide {
     // Spreaders: codes and scales of W; a group of four warps takes every other stage. Scale bytes
     // come in windows of 16, four stages each, two windows ahead, since they come from DRAM.
     static __device__ __forceinline__ bool spread(W& work, Shared& sh, uint32_t base) {
-        const int group = threadIdx.x / 128 - kWideEpilogue / 4, t = threadIdx.x % 128, lane = t & 31, half = t / kWideHalf;
+        const int group = threadIdx.x / 128 - kWideEpilogue / 4, t = threadIdx.x % 128, lane = t & 31;
+        // the thread's row for scales: a warp's words lie side by side in their block
+        const int q0 = t / 32 * 8 + (t & 7) + (t >> 3 & 3) * 32, half = q0 / kWideHalf;
         Ring<W::kStages> ring;
         Ring<kRaw> raw;
         WideItem it;
         for (int i = 0; work.item(i, it); ++i) {
-            const int64_t r = (half ? it.row[1] : it.row[0]) + t % kWideHalf;
+            const int64_t r = (half ? it.row[1] : it.row[0]) + q0 % kWideHalf;
             const unsigned char* row =
                 r < work.rows_a && half < work.halves ? (half ? work.sa[1] : work.sa[0]) + r * work.blocks : nullptr;
             uint4 window[3];
@@ -430,7 +432,7 @@ struct Wide {
 #pragma unroll
                     for (int u = 0; u < 4; ++u) c[u] = lds128(from + swizzled((t / 32 + u * 4) * 8 + (lane & 7), k % 2 * 4 + block));
                     const uint4& w = window[0];
-                    sts32(base + kAtScalesA + ring.s * kScaleBlock + scale_place(t), k & 2 ? (k & 1 ? w.w : w.z) : (k & 1 ? w.y : w.x));
+                    sts32(base + kAtScalesA + ring.s * kScaleBlock + scale_place(q0), k & 2 ? (k & 1 ? w.w : w.z) : (k & 1 ? w.y : w.x));
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         const int q = (t / 32 + u * 4) * 8 + (lane & 7);
