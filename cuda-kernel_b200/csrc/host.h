@@ -30,6 +30,7 @@ int mx4_device_error(int clear, int* out);
 int mx4_matmul_device_error(int clear, int* out);
 int mx4_wide_device_error(int clear, int* out);
 int moe_wide_device_error(int clear, int* out);
+int mx4_deep_device_error(int clear, int* out);
 
 // Launches an attribute-carrying kernel; the returned error is the launch's own.
 template <typename... Args>

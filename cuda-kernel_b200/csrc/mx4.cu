@@ -414,6 +414,7 @@ int swb_mx4_project(int type, const void* codes, const void* scales, const void*
     P.half_out = half;
     P.x_aligned = cols % 8 == 0 && x_pitch % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
     auto s = static_cast<cudaStream_t>(stream);
+    if (project_deep_takes(P)) return project_deep(type, P, s);
     if (project_wide_takes(P)) return project_wide(type, P, s);
     return type == SWB_F16 ? dispatch_project<__half>(P, s) : dispatch_project<__nv_bfloat16>(P, s);
 }

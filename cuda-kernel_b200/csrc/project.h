@@ -25,5 +25,8 @@ struct ProjectParams {
 // The tensor-core kernel (mx4_wide.cu): takes codes whose rows are whole 64 bytes, on 32 bytes.
 bool project_wide_takes(const ProjectParams& P);
 int project_wide(int type, ProjectParams P, cudaStream_t stream);
+// For more tokens (mx4_deep.cu): takes tokens on 16 bytes.
+bool project_deep_takes(const ProjectParams& P);
+int project_deep(int type, const ProjectParams& P, cudaStream_t stream);
 
 }  // namespace swb

@@ -876,7 +876,7 @@ int swb_device_error(int clear, int* out) {
         if (e != cudaSuccess) return fail(SWB_E_CUDA, cudaGetErrorString(e));
     }
     for (auto other : {moe_device_error, mx4_device_error, mx4_matmul_device_error, mx4_wide_device_error,
-                       moe_wide_device_error}) {
+                       mx4_deep_device_error, moe_wide_device_error}) {
         int more = 0;
         if (int rc = other(clear, &more)) return rc;
         v |= more;

@@ -10,7 +10,9 @@ k is 16 or 32, so K values lose at most 1.125 K 2^-24 of sum|w x|, and the parts
 warps, bias and residual add at most 76 roundings more. Where a token is split into e4m3 pieces, a
 value within 13 binades of its block's largest is exact, and another is off by at most half the
 last piece's smallest step: 2^-10 of the piece's unit, which is 2^10 (three pieces, fp16) or
-2^5 (two, bf16) below the first's, where the largest is at least 2^7: 2^-27 or 2^-22 of it.
+2^5 (two, bf16) below the first's, where the largest is at least 2^7: 2^-27 or 2^-22 of it. Where
+fp16 weights are decoded against their row's largest scale, a value is exact or off by at most 2^-40
+of the row's largest, far below the first term for these inputs.
 So |out - exact| <= (1.125 K + 76) 2^-24 sum|w x| + d sum over blocks of max|x| sum|w| (+ |bias| +
 |residual| in the first sum) + half a step of the output type (eps/2 relative, or half of the
 smallest subnormal).
@@ -149,7 +151,7 @@ def check_product(got, x, w, bias, residual, dtype):
     (1, 1, 1), (1, 32, 128), (1, 33, 31), (2, 16, 32), (3, 65, 130), (8, 48, 1024), (9, 100, 257), (16, 31, 160),
     (17, 512, 96), (33, 40, 72), (64, 64, 544), (65, 17, 33), (130, 96, 1030), (1, 5632, 2048),
     (3, 200, 128), (16, 129, 384), (20, 300, 512), (33, 64, 256), (64, 260, 640), (100, 130, 1024), (513, 65, 128),
-    (5, 4100, 2048), (2, 128, 100), (12, 192, 4064)])
+    (5, 4100, 2048), (2, 128, 100), (12, 192, 4064), (48, 1000, 512), (200, 5000, 320), (700, 200, 1032)])
 def test_project(kind, tokens, rows, cols):
     dtype = TYPES[kind]
     codes, scales, w = packed((rows, cols), rows + cols, cols ** -0.5)
