@@ -10,8 +10,8 @@
 //          column by what is left. Exact for blocks within 2^37 of the row's largest scale; smaller
 //          ones round to multiples of 2^-24 of that range, at most 2^-40 of the row's largest value.
 //
-// Roles (18 warps): copies (TMA: 64 values of the tokens a stage, 256 of W's packed rows), eight
-// decoding warps in two groups, stage about, products, eight epilogue warps. Two accumulators,
+// Roles: copies (TMA: 64 values of the tokens a stage, 256 of W's packed rows), decoding
+// warps in groups, stage about, products, eight epilogue warps. Two accumulators,
 // so that a tile's epilogue runs beside the next tile's products.
 #include <algorithm>
 #include <cstring>
@@ -36,19 +36,22 @@ int mx4_deep_device_error(int clear, int* out) {
 
 namespace {
 
-constexpr int kDeepM = 128, kDeepEpilogue = 8, kDeepDecoders = 8;
-constexpr int kDeepThreads = (kDeepEpilogue + kDeepDecoders + 2) * 32;
+constexpr int kDeepM = 128, kDeepEpilogue = 8;  // rows; warps
 constexpr int kDeepTurn = 32, kDeepPitch = kDeepTurn + 2;  // columns of the epilogue's tiles
 constexpr int kDeepScales = 3;  // tiles whose row factors are kept: decoders run at most two ahead of the epilogue
 
 template <int N>
 struct DeepShape {
-    static constexpr int kStagesA = N == 192 ? 4 : 5, kStagesB = N == 192 ? 3 : 4, kRaw = N == 192 ? 2 : 4;
+    // A stage's decoding is a chain of about a microsecond: groups of warps take stages of their own.
+    static constexpr int kGroups = N == 192 ? 3 : 8, kGroupWarps = N == 192 ? 4 : 1, kDecoders = kGroups * kGroupWarps;
+    static constexpr int kThreads = (kDeepEpilogue + kDecoders + 2) * 32;
+    static constexpr int kStagesA = N == 192 ? 4 : 5, kStagesB = N == 192 ? 3 : 8, kRaw = N == 192 ? 2 : 4;
+    static_assert(kGroups <= kStagesB, "groups do not overtake the ring");
     static constexpr int kStageA = kDeepM * 128, kStageB = N * 128, kRawStage = N * 128;
     static constexpr uint32_t kAtB = kStagesA * kStageA, kAtRaw = kAtB + kStagesB * kStageB;
     static constexpr uint32_t kAtTurn = kAtRaw + kRaw * kRawStage;
     static constexpr uint32_t kAtFactors = kAtTurn + kDeepEpilogue * 32 * kDeepPitch * 4;
-    static constexpr size_t kSmem = kAtFactors + kDeepScales * N * 4 + 1024;
+    static constexpr size_t kSmem = kAtFactors + (kDeepScales + 1) * N * 4 + 1024;  // factors, and the current tile's largest scales
     static constexpr int kColumns = N == 192 ? 512 : 128;  // two accumulators
     static_assert(kSmem + 1024 <= kSmemPerCtaMax && 2 * N <= kColumns, "fits");
 };
@@ -94,10 +97,11 @@ __device__ __forceinline__ void deep_decode(const uint4& codes, uint32_t scale, 
 }
 
 template <typename T, int N>
-__global__ void __launch_bounds__(kDeepThreads, 1)
+__global__ void __launch_bounds__(DeepShape<N>::kThreads, 1)
     project_deep_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                         const ProjectParams P, int tiles_x, int stages) {
     using S = DeepShape<N>;
+    constexpr int kDeepDecoders = S::kDecoders;
     extern __shared__ unsigned char raw_smem[];
     __shared__ uint64_t a_full[S::kStagesA], a_empty[S::kStagesA], b_full[S::kStagesB], b_empty[S::kStagesB];
     __shared__ uint64_t raw_full[S::kRaw], raw_empty[S::kRaw], acc_full[2], acc_empty[2];
@@ -106,8 +110,8 @@ __global__ void __launch_bounds__(kDeepThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kStagesA; ++i) mbar_init(smem_u32(a_full + i), 1), mbar_init(smem_u32(a_empty + i), 1);
-        for (int i = 0; i < S::kStagesB; ++i) mbar_init(smem_u32(b_full + i), 4), mbar_init(smem_u32(b_empty + i), 1);
-        for (int i = 0; i < S::kRaw; ++i) mbar_init(smem_u32(raw_full + i), 1), mbar_init(smem_u32(raw_empty + i), kDeepDecoders);
+        for (int i = 0; i < S::kStagesB; ++i) mbar_init(smem_u32(b_full + i), S::kGroupWarps), mbar_init(smem_u32(b_empty + i), 1);
+        for (int i = 0; i < S::kRaw; ++i) mbar_init(smem_u32(raw_full + i), 1), mbar_init(smem_u32(raw_empty + i), 4 * S::kGroupWarps);
         for (int i = 0; i < 2; ++i) mbar_init(smem_u32(acc_full + i), 1), mbar_init(smem_u32(acc_empty + i), kDeepEpilogue);
         mbar_fence_init();
     }
@@ -182,83 +186,82 @@ __global__ void __launch_bounds__(kDeepThreads, 1)
         }
     } else if (warp >= kDeepEpilogue) {
         // ---------------------------------------------------- decoders
-        constexpr int kTasks = N * 2 / 128;  // blocks of a stage's 64 values that a thread decodes
-        const int group = (warp - kDeepEpilogue) / 4, t = (threadIdx.x - kDeepEpilogue * 32) % 128;
-        int b = 0, r = 0, slot = 0;
-        uint32_t pb = 0, pr = 0;
-        int64_t nb = 0;
+        // Group g takes the stages g, g + kGroups, ... of the sequence, and nothing else: passing
+        // over the others' stages one by one cost more than decoding its own.
+        constexpr int kGroupThreads = S::kGroupWarps * 32, kAll = S::kDecoders * 32;
+        constexpr int kTasks = N * 2 / kGroupThreads;  // blocks of a stage's 64 values that a thread decodes
+        const int thread = threadIdx.x - kDeepEpilogue * 32, group = thread / kGroupThreads, t = thread % kGroupThreads;
+        const int raws = (stages + 3) / 4;
+        uint32_t* tops = reinterpret_cast<uint32_t*>(factors) + kDeepScales * N;
+        int slot = 0, tiles = 0;
         bool ok = true;
-        for (int64_t tile = blockIdx.x; tile < P.items && ok; tile += gridDim.x) {
+        for (int64_t tile = blockIdx.x; tile < P.items && ok; tile += gridDim.x, ++tiles) {
             const int64_t w0 = tile / tiles_x * N;
-            const unsigned char* row[kTasks];
-            uint32_t top[kTasks];
-            uint4 window[kTasks], ahead[kTasks];
-#pragma unroll
-            for (int u = 0; u < kTasks; ++u) {
-                const int64_t q = w0 + (t + 128 * u) % N;
-                row[u] = q < P.rows ? P.s + q * blocks : nullptr;
-                top[u] = 0u;
-            }
-            if constexpr (std::is_same<T, __half>::value) {
-#pragma unroll
-                for (int u = 0; u < kTasks; ++u) {
+            if constexpr (std::is_same<T, __half>::value) {  // the rows' largest scales
+                named_barrier_sync(1, kAll);                 // the last tile's are read
+                for (int q = thread; q < N; q += kAll) {
                     uint32_t m = 0u;
-                    if (row[u]) {
+                    if (w0 + q < P.rows) {
 #pragma unroll 4
                         for (int i = 0; i < blocks; i += 16) {
-                            const uint4 v = load_scales(row[u], i, blocks);
+                            const uint4 v = load_scales(P.s + (w0 + q) * blocks, i, blocks);
                             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                             for (int e = 0; e < 4; ++e) m = __vmaxu4(m, w[e] & ~__vcmpeq4(w[e], 0xFFFFFFFFu));
                         }
                     }
-                    top[u] = max(max(m & 255u, m >> 8 & 255u), max(m >> 16 & 255u, m >> 24));
-                    if (group == 0 && t + 128 * u < N) factors[slot * N + t + 128 * u] = mx_scale(top[u]);
+                    m = max(max(m & 255u, m >> 8 & 255u), max(m >> 16 & 255u, m >> 24));
+                    tops[q] = m;
+                    factors[slot * N + q] = mx_scale(m);
                 }
+                named_barrier_sync(1, kAll);
             }
-            auto load = [&](int k, uint4 (&w)[kTasks]) {  // 16 scale bytes: stages k & ~7 to k | 7
+            const unsigned char* row[kTasks];
+            uint32_t top[kTasks], scale[kTasks];
 #pragma unroll
-                for (int u = 0; u < kTasks; ++u)
-                    w[u] = row[u] && k < stages ? load_scales(row[u], k / 8 * 16, blocks) : make_uint4(0u, 0u, 0u, 0u);
+            for (int u = 0; u < kTasks; ++u) {
+                const int q = (t + kGroupThreads * u) % N;
+                row[u] = w0 + q < P.rows ? P.s + (w0 + q) * blocks + (t + kGroupThreads * u) / N : nullptr;
+                top[u] = std::is_same<T, __half>::value ? tops[q] : 0u;
+            }
+            auto load = [&](int k) {
+#pragma unroll
+                for (int u = 0; u < kTasks; ++u) {
+                    const int byte = k * 2 + (t + kGroupThreads * u) / N;
+                    scale[u] = row[u] && byte < blocks ? row[u][k * 2] : 0u;
+                }
             };
-            load(0, window);
-            load(8, ahead);
-            for (int k = 0; k < stages; ++k) {
-                if (k > 0 && k % 8 == 0) {
+            const uint32_t q0 = uint32_t(tiles) * uint32_t(stages);  // of the sequence
+            int k = int((uint32_t(group) + uint32_t(S::kGroups) - q0 % S::kGroups) % S::kGroups);
+            if (k < stages) load(k);
+            for (; k < stages; k += S::kGroups) {
+                const uint32_t q = q0 + uint32_t(k), b = q % S::kStagesB, use = q / S::kStagesB;
+                const uint32_t rq = uint32_t(tiles) * uint32_t(raws) + uint32_t(k / 4), r = rq % S::kRaw;
+                ok = mbar_wait_warp(smem_u32(raw_full + r), rq / S::kRaw & 1u) &&
+                     (use == 0 || mbar_wait_warp(smem_u32(b_empty + b), (use & 1u) ^ 1u));
+                if (!ok) break;
+                const uint32_t from = base + S::kAtRaw + r * S::kRawStage, to = base + S::kAtB + b * S::kStageB;
+                uint32_t now[kTasks];
 #pragma unroll
-                    for (int u = 0; u < kTasks; ++u) window[u] = ahead[u];
-                    load(k + 8, ahead);
-                }
-                if (k % 4 == 0 && !mbar_wait_warp(smem_u32(raw_full + r), pr)) {
-                    ok = false;
-                    break;
-                }
-                if (nb % 2 == group) {
-                    ok = __all_sync(0xFFFFFFFFu, nb < S::kStagesB || mbar_wait(smem_u32(b_empty + b), pb ^ 1u));
-                    if (!ok) break;
-                    const uint32_t from = base + S::kAtRaw + r * S::kRawStage, to = base + S::kAtB + b * S::kStageB;
+                for (int u = 0; u < kTasks; ++u) now[u] = scale[u];
+                if (k + S::kGroups < stages) load(k + S::kGroups);
 #pragma unroll
-                    for (int u = 0; u < kTasks; ++u) {
-                        const int q = (t + 128 * u) % N, block = (t + 128 * u) / N, byte = (k * 2 + block) & 15;
-                        const uint4 codes = lds128(from + swizzled(q, k % 4 * 2 + block));
-                        const uint32_t word = byte & 8 ? (byte & 4 ? window[u].w : window[u].z) : (byte & 4 ? window[u].y : window[u].x);
-                        uint32_t w[16];
-                        deep_decode<T>(codes, word >> (byte % 4 * 8) & 255u, top[u], w);
+                for (int u = 0; u < kTasks; ++u) {
+                    const int row16 = (t + kGroupThreads * u) % N, block = (t + kGroupThreads * u) / N;
+                    const uint4 codes = lds128(from + swizzled(row16, k % 4 * 2 + block));
+                    uint32_t w[16];
+                    deep_decode<T>(codes, now[u], top[u], w);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + swizzled(q, block * 4 + i)), "r"(w[4 * i]),
-                                         "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3]) : "memory");
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(b_full + b));
+                    for (int i = 0; i < 4; ++i)
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + swizzled(row16, block * 4 + i)), "r"(w[4 * i]),
+                                     "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3]) : "memory");
                 }
-                ++nb;
-                if (++b == S::kStagesB) b = 0, pb ^= 1u;
-                if (k % 4 == 3 || k == stages - 1) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(raw_empty + r));
-                    if (++r == S::kRaw) r = 0, pr ^= 1u;
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(b_full + b));
+                    // a raw stage is free after its four; the last one's missing stages count here
+                    for (int n = k == stages - 1 ? 4 - k % 4 : 1; n > 0; --n) mbar_arrive(smem_u32(raw_empty + r));
                 }
             }
             if (++slot == kDeepScales) slot = 0;
@@ -358,7 +361,7 @@ int launch_deep(ProjectParams P, cudaStream_t stream) {
     const int tiles_x = int((P.tokens + kDeepM - 1) / kDeepM), stages = (P.cols + 63) / 64;
     P.tiles = (P.rows + N - 1) / N;
     P.items = int64_t(P.tiles) * tiles_x;
-    return launch_ex(kernel, unsigned(std::min<int64_t>(P.items, sms)), kDeepThreads, S::kSmem, stream, false, map_x, map_w, P,
+    return launch_ex(kernel, unsigned(std::min<int64_t>(P.items, sms)), S::kThreads, S::kSmem, stream, false, map_x, map_w, P,
                      tiles_x, stages);
 }
 
