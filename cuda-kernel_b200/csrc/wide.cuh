@@ -229,6 +229,20 @@ struct Wide {
         }
     };
 
+    // Groups of warps take the stages of the sequence (item after item) in turn, each its own only:
+    // passing over the others' stages one by one cost more than the work on its own. Stage q of
+    // the sequence is in slot q % STAGES for the (q / STAGES)-th time.
+    template <int STAGES>
+    static __device__ __forceinline__ bool slot_free(uint64_t* empty, uint32_t q) {
+        const uint32_t use = q / STAGES;
+        return use == 0 || mbar_wait(smem_u32(empty + q % STAGES), (use & 1u) ^ 1u);
+    }
+    // The first stage from s0 on of an item that starts at q0 of the sequence which is `group`'s.
+    template <int GROUPS>
+    static __device__ __forceinline__ int first_of(int group, uint32_t q0, int s0) {
+        return s0 + int((uint32_t(group) + GROUPS - q0 % GROUPS) % GROUPS);
+    }
+
     // Every thread of the CTA, before run(); the CTA synchronises in between.
     static __device__ __forceinline__ void init(Shared& s) {
         if (threadIdx.x == 0) {
@@ -247,7 +261,7 @@ struct Wide {
             }
             for (int i = 0; i < kRaw; ++i) {
                 mbar_init(smem_u32(s.raw_full + i), 1);
-                mbar_init(smem_u32(s.raw_empty + i), kSpreaders);
+                mbar_init(smem_u32(s.raw_empty + i), 8);  // two stages, four warps each
             }
             mbar_fence_init();
         }
@@ -396,72 +410,78 @@ struct Wide {
         return true;
     }
 
-    // Spreaders: codes and scales of W; a group of four warps takes every other stage. Scale bytes
-    // come in windows of 16, four stages each, two windows ahead, since they come from DRAM.
+    // Spreaders: codes and scales of W. Scale words are loaded four of the group's stages ahead, since
+    // they come from DRAM.
     static __device__ __forceinline__ bool spread(W& work, Shared& sh, uint32_t base) {
+        constexpr int kGroupsA = kSpreadGroups > 0 ? kSpreadGroups : 1;
         const int group = threadIdx.x / 128 - kWideEpilogue / 4, t = threadIdx.x % 128, lane = t & 31;
         // the thread's row for scales: a warp's words lie side by side in their block
-        const int q0 = t / 32 * 8 + (t & 7) + (t >> 3 & 3) * 32, half = q0 / kWideHalf;
-        Ring<W::kStages> ring;
-        Ring<kRaw> raw;
+        const int row_a = t / 32 * 8 + (t & 7) + (t >> 3 & 3) * 32, half = row_a / kWideHalf;
+        uint32_t q0 = 0, raw0 = 0;
         WideItem it;
         for (int i = 0; work.item(i, it); ++i) {
-            const int64_t r = (half ? it.row[1] : it.row[0]) + q0 % kWideHalf;
+            const int64_t r = (half ? it.row[1] : it.row[0]) + row_a % kWideHalf;
             const unsigned char* row =
                 r < work.rows_a && half < work.halves ? (half ? work.sa[1] : work.sa[0]) + r * work.blocks : nullptr;
-            uint4 window[3];
-            auto load = [&](int w, int k) {
-                window[w] = row && k < it.s1 ? load_scales(row, k / 4 * 16, work.blocks) : make_uint4(0u, 0u, 0u, 0u);
-            };
-            load(0, it.s0);
-            load(1, (it.s0 | 3) + 1);
-            load(2, (it.s0 | 3) + 5);
-            for (int k = it.s0; k < it.s1; ++k) {
-                if (k > it.s0 && k % 4 == 0) {
-                    window[0] = window[1], window[1] = window[2];
-                    load(2, k + 8);
-                }
-                // every warp waits for each raw stage, so that none arrives at its end a round early
-                if ((k == it.s0 || k % 2 == 0) && !mbar_wait_warp(smem_u32(sh.raw_full + raw.s), raw.ph)) return false;
-                if (ring.issued % kSpreadGroups == group) {
-                    if (!__all_sync(0xFFFFFFFFu, ring.free(sh.empty))) return false;
-                    // a warp takes eight rows, four blocks of 16 bytes each, at a time
-                    const uint32_t from = base + kAtRaw + raw.s * kRawStage, to = base + ring.s * kStageA;
-                    const int block = lane >> 3;
-                    uint4 c[4];
+            int k = first_of<kGroupsA>(group, q0, it.s0);
+            uint32_t word[5];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) c[u] = lds128(from + swizzled((t / 32 + u * 4) * 8 + (lane & 7), k % 2 * 4 + block));
-                    const uint4& w = window[0];
-                    sts32(base + kAtScalesA + ring.s * kScaleBlock + scale_place(q0), k & 2 ? (k & 1 ? w.w : w.z) : (k & 1 ? w.y : w.x));
+            for (int w = 0; w < 4; ++w) word[w] = scale_word(row, k + w * kGroupsA, it.s1, work.blocks);
+            for (; k < it.s1; k += kGroupsA) {
+                word[4] = scale_word(row, k + 4 * kGroupsA, it.s1, work.blocks);
+                const uint32_t q = q0 + uint32_t(k - it.s0), s = q % W::kStages;
+                const uint32_t raw = raw0 + uint32_t(k / 2 - it.s0 / 2), rs = raw % kRaw;
+                const bool ready = mbar_wait(smem_u32(sh.raw_full + rs), raw / kRaw & 1u) && slot_free<W::kStages>(sh.empty, q);
+                if (!__all_sync(0xFFFFFFFFu, ready)) return false;
+                // a warp takes eight rows, four blocks of 16 bytes each, at a time
+                const uint32_t from = base + kAtRaw + rs * kRawStage, to = base + s * kStageA;
+                const int block = lane >> 3;
+                uint4 c[4];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int q = (t / 32 + u * 4) * 8 + (lane & 7);
-                        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to + swizzled(q, 2 * block)), "r"(c[u].x), "r"(c[u].y) : "memory");
-                        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to + swizzled(q, 2 * block + 1)), "r"(c[u].z), "r"(c[u].w) : "memory");
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(sh.full + ring.s));
+                for (int u = 0; u < 4; ++u) c[u] = lds128(from + swizzled((t / 32 + u * 4) * 8 + (lane & 7), k % 2 * 4 + block));
+                sts32(base + kAtScalesA + s * kScaleBlock + scale_place(row_a), word[0]);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int n = (t / 32 + u * 4) * 8 + (lane & 7);
+                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to + swizzled(n, 2 * block)), "r"(c[u].x), "r"(c[u].y) : "memory");
+                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to + swizzled(n, 2 * block + 1)), "r"(c[u].z), "r"(c[u].w) : "memory");
                 }
-                ring.next();
-                if (k % 2 == 1 || k + 1 == it.s1) {
-                    if (lane == 0) mbar_arrive(smem_u32(sh.raw_empty + raw.s));
-                    raw.next();
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(sh.full + s));
+                    mbar_arrive(smem_u32(sh.raw_empty + rs));
+                    // a raw stage of which the item takes one half only
+                    if ((k == it.s0 && k % 2 == 1) || (k == it.s1 - 1 && k % 2 == 0)) mbar_arrive(smem_u32(sh.raw_empty + rs));
                 }
+#pragma unroll
+                for (int w = 0; w < 4; ++w) word[w] = word[w + 1];
             }
+            q0 += uint32_t(it.s1 - it.s0);
+            raw0 += uint32_t((it.s1 + 1) / 2 - it.s0 / 2);
         }
         return true;
     }
+    // The four scale bytes of stage k of a row, zero beyond it.
+    static __device__ __forceinline__ uint32_t scale_word(const unsigned char* row, int k, int end, int blocks) {
+        if (!row || k >= end) return 0u;
+        if ((blocks & 3) == 0 && (reinterpret_cast<uintptr_t>(row) & 3) == 0)
+            return __ldg(reinterpret_cast<const uint32_t*>(row) + k);
+        uint32_t w = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (k * 4 + e < blocks) w |= uint32_t(__ldg(row + k * 4 + e)) << (8 * e);
+        return w;
+    }
 
-    // Splitters: group g takes the stages g, g + kGroups, ... of the sequence.
+    // Splitters: tokens from their rows.
     static __device__ __forceinline__ bool split(W& work, Shared& sh, uint32_t base) {
         constexpr int kPer = kMx ? 16 : 8;                    // eight-value parts of a row in a stage
         constexpr int kStride = kGroupWarps * 32 / kPer;      // tokens taken at once
         constexpr int kTurns = (W::kTok + kStride - 1) / kStride, kBatch = kTurns < 4 ? kTurns : 4;
         const int warp = threadIdx.x / 32 - kWideEpilogue - kSpreaders, group = warp / kGroupWarps;
         const int t = threadIdx.x - (kWideEpilogue + kSpreaders + group * kGroupWarps) * 32, j = t % kPer, n0 = t / kPer;
-        Ring<W::kTokenStages> ring;
-        int turn = 0;  // of the group whose stage is next
+        uint32_t q0 = 0;
         WideItem it;
         uint4 x[kTurns];
         for (int i = 0; work.item(i, it); ++i) {
@@ -475,51 +495,47 @@ struct Wide {
                     x[u] = work.x_aligned ? load_piece<T, true>(row, at, work.cols) : load_piece<T, false>(row, at, work.cols);
                 }
             };
-            int mine = it.s0 + (group - turn + kGroups) % kGroups;  // this group's first stage of the item
-            load(mine);
-            for (int k = it.s0; k < it.s1; ++k) {
-                if (k == mine) {
-                    if (!__all_sync(0xFFFFFFFFu, ring.free(sh.tokens_empty))) return false;
-                    const uint32_t b = base + kAtB + ring.s * kStageB;
-                    const uint32_t sc = base + kAtScalesB + ring.s * kBlocksB * kScaleBlock;
+            int k = first_of<kGroups>(group, q0, it.s0);
+            load(k);
+            for (; k < it.s1; k += kGroups) {
+                const uint32_t q = q0 + uint32_t(k - it.s0), s = q % W::kTokenStages;
+                if (!__all_sync(0xFFFFFFFFu, slot_free<W::kTokenStages>(sh.tokens_empty, q))) return false;
+                const uint32_t b = base + kAtB + s * kStageB, sc = base + kAtScalesB + s * kBlocksB * kScaleBlock;
 #pragma unroll
-                    for (int u0 = 0; u0 < kTurns; u0 += kBatch) {
-                        if (u0 * kStride >= it.count) break;  // whole groups: the shuffles stay together
-                        if constexpr (!kMx) {
+                for (int u0 = 0; u0 < kTurns; u0 += kBatch) {
+                    if (u0 * kStride >= it.count) break;  // whole groups: the shuffles stay together
+                    if constexpr (!kMx) {
 #pragma unroll
-                            for (int u = u0; u < u0 + kBatch && u < kTurns; ++u) {
-                                const int n = n0 + u * kStride;
-                                if (n < it.count)
-                                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(b + swizzled(n, j)), "r"(x[u].x), "r"(x[u].y), "r"(x[u].z), "r"(x[u].w) : "memory");
-                            }
-                        } else {
-                            uint2 piece[kBatch][W::kPieces];
-                            uint32_t scale[kBatch];
+                        for (int u = u0; u < u0 + kBatch && u < kTurns; ++u) {
+                            const int n = n0 + u * kStride;
+                            if (n < it.count)
+                                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(b + swizzled(n, j)), "r"(x[u].x), "r"(x[u].y), "r"(x[u].z), "r"(x[u].w) : "memory");
+                        }
+                    } else {
+                        uint2 piece[kBatch][W::kPieces];
+                        uint32_t scale[kBatch];
 #pragma unroll
-                            for (int u = 0; u < kBatch; ++u)
-                                scale[u] = split_token<W::kPieces>(x[u0 + u < kTurns ? u0 + u : kTurns - 1], piece[u], T());
+                        for (int u = 0; u < kBatch; ++u)
+                            scale[u] = split_token<W::kPieces>(x[u0 + u < kTurns ? u0 + u : kTurns - 1], piece[u], T());
 #pragma unroll
-                            for (int u = 0; u < kBatch; ++u) {
-                                const int n = n0 + (u0 + u) * kStride;
-                                if (n >= it.count) continue;
+                        for (int u = 0; u < kBatch; ++u) {
+                            const int n = n0 + (u0 + u) * kStride;
+                            if (n >= it.count) continue;
 #pragma unroll
-                                for (int p = 0; p < W::kPieces; ++p) {
-                                    const int r = n * W::kPieces + p;
-                                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(b + swizzled(r, j / 2) + (j & 1) * 8), "r"(piece[u][p].x), "r"(piece[u][p].y) : "memory");
-                                    if ((j & 3) == 0) sts8(sc + scale_place(r) + j / 4, scale[u] - 5u * p);
-                                }
+                            for (int p = 0; p < W::kPieces; ++p) {
+                                const int r = n * W::kPieces + p;
+                                asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(b + swizzled(r, j / 2) + (j & 1) * 8), "r"(piece[u][p].x), "r"(piece[u][p].y) : "memory");
+                                if ((j & 3) == 0) sts8(sc + scale_place(r) + j / 4, scale[u] - 5u * p);
                             }
                         }
                     }
-                    mine += kGroups;
-                    load(mine);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(sh.tokens_full + ring.s));
                 }
-                ring.next();
+                load(k + kGroups);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(sh.tokens_full + s));
             }
-            turn = (turn + it.s1 - it.s0) % kGroups;
+            q0 += uint32_t(it.s1 - it.s0);
         }
         return true;
     }
@@ -528,55 +544,48 @@ struct Wide {
     // their scale words by plain loads.
     static __device__ __forceinline__ bool bring(W& work, Shared& sh, uint32_t base, const CUtensorMap* map_b) {
         const int lane = threadIdx.x & 31, group = threadIdx.x / 32 - kWideEpilogue - kSpreaders;
-        Ring<W::kTokenStages> ring;
+        uint32_t q0 = 0;
         WideItem it;
         for (int i = 0; work.item(i, it); ++i) {
             const int n = columns(it.count), rows = it.count * W::kPieces;
-            for (int k = it.s0; k < it.s1; ++k) {
-                if (ring.issued % kGroups == group) {
-                    if (!__all_sync(0xFFFFFFFFu, ring.free(sh.tokens_empty))) {
-                        if (!W::kGather && lane == 0) ring.drain(sh.tokens_full);
-                        return false;
-                    }
-                    const uint32_t bar = smem_u32(sh.tokens_full + ring.s), b = base + kAtB + ring.s * kStageB;
-                    if constexpr (W::kGather) {  // eight lanes a row
-                        for (int r = lane / 8; r < rows; r += 4) {
-                            const int64_t from = int64_t(work.place(it, r / W::kPieces)) * W::kPieces + r % W::kPieces;
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(b + swizzled(r, lane & 7)),
-                                         "l"(work.pieces + from * work.pitch + k * kWideRowBytes + (lane & 7) * 16) : "memory");
-                        }
-                    }
-                    if constexpr (kMx) {
-#pragma unroll
-                        for (int u = 0; u < (kN + 31) / 32; ++u) {
-                            const int r = lane + 32 * u;
-                            if (r >= rows) continue;
-                            const int64_t from = (W::kGather ? int64_t(work.place(it, r / W::kPieces)) : int64_t(it.first + r / W::kPieces)) * W::kPieces + r % W::kPieces;
-                            const unsigned char* row = work.sb + from * work.pitch_b;
-                            uint32_t w = 0u;
-                            if ((work.pitch_b & 3) == 0) {
-                                w = *reinterpret_cast<const uint32_t*>(row + k * 4);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    if (k * 4 + e < work.pitch_b) w |= uint32_t(row[k * 4 + e]) << (8 * e);
-                            }
-                            sts32(base + kAtScalesB + ring.s * kBlocksB * kScaleBlock + scale_place(r), w);
-                        }
-                        if (W::kGather) asm volatile("cp.async.wait_all;" ::: "memory");
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
-                    if constexpr (W::kGather) {
-                        if (lane == 0) mbar_arrive(bar);
-                    } else if (elect_one()) {
-                        mbar_arrive_expect_tx(bar, n * kWideRowBytes);
-                        for (int r = 0; r < n; r += 16)
-                            tma_load_2d(b + r * kWideRowBytes, map_b, k * kValues, it.first * W::kPieces + r, bar);
-                    }
+            for (int k = first_of<kGroups>(group, q0, it.s0); k < it.s1; k += kGroups) {
+                const uint32_t q = q0 + uint32_t(k - it.s0), s = q % W::kTokenStages;
+                const uint32_t bar = smem_u32(sh.tokens_full + s), b = base + kAtB + s * kStageB;
+                if (!__all_sync(0xFFFFFFFFu, slot_free<W::kTokenStages>(sh.tokens_empty, q))) {
+                    // this warp's copies have landed where its earlier stages were read; the last ones may not
+                    if (!W::kGather && lane == 0 && q >= kGroups)
+                        mbar_wait(smem_u32(sh.tokens_full + (q - kGroups) % W::kTokenStages), (q - kGroups) / W::kTokenStages & 1u);
+                    return false;
                 }
-                ring.next();
+                if constexpr (W::kGather) {  // eight lanes a row
+                    for (int r = lane / 8; r < rows; r += 4) {
+                        const int64_t from = int64_t(work.place(it, r / W::kPieces)) * W::kPieces + r % W::kPieces;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(b + swizzled(r, lane & 7)),
+                                     "l"(work.pieces + from * work.pitch + k * kWideRowBytes + (lane & 7) * 16) : "memory");
+                    }
+                } else if (elect_one()) {
+                    mbar_expect_tx(bar, n * kWideRowBytes);
+                    for (int r = 0; r < n; r += 16)
+                        tma_load_2d(b + r * kWideRowBytes, map_b, k * kValues, it.first * W::kPieces + r, bar);
+                }
+                if constexpr (kMx) {
+                    uint32_t word[(kN + 31) / 32];
+#pragma unroll
+                    for (int u = 0; u < (kN + 31) / 32; ++u) {
+                        const int r = lane + 32 * u;
+                        const int64_t from = r >= rows ? -1 : (W::kGather ? int64_t(work.place(it, r / W::kPieces)) : int64_t(it.first + r / W::kPieces)) * W::kPieces + r % W::kPieces;
+                        word[u] = scale_word(from < 0 ? nullptr : work.sb + from * work.pitch_b, k, it.s1, work.pitch_b);
+                    }
+#pragma unroll
+                    for (int u = 0; u < (kN + 31) / 32; ++u)
+                        if (lane + 32 * u < rows) sts32(base + kAtScalesB + s * kBlocksB * kScaleBlock + scale_place(lane + 32 * u), word[u]);
+                    if (W::kGather) asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_proxy_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar);
             }
+            q0 += uint32_t(it.s1 - it.s0);
         }
         return true;
     }
