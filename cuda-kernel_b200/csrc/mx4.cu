@@ -32,6 +32,7 @@ struct Elem<float> {
 struct RowMap {
     int64_t rows, cols, blocks, total;  // total = rows * blocks
     int64_t pitch;                      // elements from row to row of the unpacked side
+    bool flat;                          // rows of whole blocks without gaps: block id starts at value 32 id
 };
 
 // Block id -> (row, block of the row); 32-bit division where the ids allow it.
@@ -59,16 +60,36 @@ __device__ __forceinline__ float inverse_scale(uint32_t byte) {
     return byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
 }
 
+// Where a quad lane's eight values lie, or -1 beyond the row. (The division of locate is a fifth of
+// the kernels' instructions, and they are close to bound by those.)
+__device__ __forceinline__ int64_t values_at(const RowMap& m, int64_t id, int q) {
+    if (m.flat) return id * kMxBlock + q * 8;
+    int64_t row, block;
+    locate(m, id, row, block);
+    const int64_t k = block * kMxBlock + q * 8;
+    return k < m.cols ? row * m.pitch + k : -1;
+}
+
+// Eight values, and the bits of the largest magnitude as fp32.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+__device__ __forceinline__ uint32_t load8(const T* p, float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {
         const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        uint32_t top = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        return top;
     } else {
         const uint4 a = *reinterpret_cast<const uint4*>(p);
         const T* e = reinterpret_cast<const T*>(&a);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = Elem<T>::load(e[i]);
+        // magnitudes of 16-bit values order like integers, two at a time
+        const uint32_t m = 0x7FFF7FFFu;
+        const uint32_t t = __vmaxu2(__vmaxu2(a.x & m, a.y & m), __vmaxu2(a.z & m, a.w & m));
+        const unsigned short one = static_cast<unsigned short>(max(t & 0xFFFFu, t >> 16));
+        return __float_as_uint(Elem<T>::load(*reinterpret_cast<const T*>(&one)));
     }
 }
 template <typename T>
@@ -103,16 +124,12 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = 0.f;
-            int64_t row = 0, block = 0;
             const bool have = id < m.total;
-            if (have) {
-                locate(m, id, row, block);
-                const int64_t k = block * kMxBlock + q * 8;
-                if (k < m.cols) load8(x + row * m.pitch + k, v);
-            }
             uint32_t top = 0u;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+            if (have) {
+                const int64_t at = values_at(m, id, q);
+                if (at >= 0) top = load8(x + at, v);
+            }
             top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
             top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
             const uint32_t byte = scale_byte(top);
@@ -153,10 +170,8 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const unsigned char* __
         const int64_t step = int64_t(gridDim.x) * (blockDim.x / 4);
         const int q = lane & 3;
         for (int64_t id = int64_t(blockIdx.x) * (blockDim.x / 4) + threadIdx.x / 4; id < m.total; id += step) {
-            int64_t row, block;
-            locate(m, id, row, block);
-            const int64_t k = block * kMxBlock + q * 8;
-            if (k >= m.cols) continue;
+            const int64_t at = values_at(m, id, q);
+            if (at < 0) continue;
             const float s = mx_scale(scales[id]);
             uint32_t p[4];
             mx_decode_f16(reinterpret_cast<const uint32_t*>(codes)[id * 4 + q], p);
@@ -167,7 +182,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const unsigned char* __
                 v[2 * i] = f.x * s;
                 v[2 * i + 1] = f.y * s;
             }
-            store8(out + row * m.pitch + k, v);
+            store8(out + at, v);
         }
     } else {
         const int64_t step = int64_t(gridDim.x) * (blockDim.x / 32);
@@ -225,6 +240,7 @@ int convert(int type, const void* from, void* to, int64_t pitch, const void* cod
     m.blocks = mx_blocks(cols);
     m.total = rows * m.blocks;
     m.pitch = pitch;
+    m.flat = cols % kMxBlock == 0 && (pitch == cols || rows == 1);
     const size_t bytes = (size_t(rows - 1) * pitch + cols) * elem_size(type);
     if (overlaps(side, bytes, codes, size_t(m.total) * kMxBlockBytes) || overlaps(side, bytes, scales, size_t(m.total)))
         return fail(SWB_E_OVERLAP_INPUT);

@@ -52,27 +52,27 @@ def moe_out(x: torch.Tensor, router: torch.Tensor, gate: torch.Tensor, up: torch
     _check(four_bit == (up_scales is not None) == (down_scales is not None),
            "scales belong to all three matrices or to none")
     if four_bit:
-        for codes, scales, shape in ((gate, gate_scales, (experts, inter, hidden)),
-                                     (up, up_scales, (experts, inter, hidden)),
-                                     (down, down_scales, (experts, hidden, inter))):
-            _check_packed(codes, scales, shape, device)
+        _check_packed(gate, gate_scales, (experts, inter), hidden, device)
+        _check_packed(up, up_scales, (experts, inter), hidden, device)
+        _check_packed(down, down_scales, (experts, hidden), inter, device)
         typed = (router, y)
     else:
         _check(gate.shape == (experts, inter, hidden) and up.shape == gate.shape
                and down.shape == (experts, hidden, inter), "incompatible weights")
         typed = (router, y, gate, up, down)
     for t in typed:
-        _check(t.dtype == dtype and t.device == device and t.is_contiguous(),
-               "router, weights and y must be contiguous, of x's type and on its device")
-    for t in (x, *typed):
-        _check(not t.requires_grad, "inference only: disable gradients")
+        if t.dtype != dtype or t.device != device or not t.is_contiguous():
+            raise RuntimeError("router, weights and y must be contiguous, of x's type and on its device")
+        if t.requires_grad:
+            raise RuntimeError("inference only: disable gradients")
+    _check(not x.requires_grad, "inference only: disable gradients")
     _check(y.shape == x.shape, "y must have x's shape")
     _check(workspace.device == device and workspace.dtype == torch.uint8 and workspace.is_contiguous(),
            "workspace must come from moe_workspace on x's device")
-    for t, kind, name in ((ids, torch.int32, "ids"), (weights, torch.float32, "weights")):
-        if t is not None:
-            _check(t.dtype == kind and t.device == device and t.is_contiguous()
-                   and tuple(t.shape) == (tokens, topk), f"{name} must be contiguous [tokens, topk]")
+    for t, kind in ((ids, torch.int32), (weights, torch.float32)):
+        if t is not None and (t.dtype != kind or t.device != device or not t.is_contiguous()
+                              or t.shape != (tokens, topk)):
+            raise RuntimeError("ids (int32) and weights (fp32) must be contiguous [tokens, topk]")
     flags = (_lib.SWB_MOE_MX4 if four_bit else 0) | (_lib.SWB_MOE_RENORMALIZE if renormalize else 0)
     _call(device, _lib.lib().swb_moe, _TYPES[dtype], flags, x.data_ptr(), pitch, router.data_ptr(), gate.data_ptr(),
           up.data_ptr(), down.data_ptr(), gate_scales.data_ptr() if four_bit else None,

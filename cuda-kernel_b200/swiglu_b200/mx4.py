@@ -27,9 +27,15 @@ def blocks(cols: int) -> int:
     return -(-cols // BLOCK)
 
 
+# The current stream's handle by device index; the public torch.cuda.current_stream builds a
+# Stream object each time, 2 of a small call's 10 microseconds.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _call(device: torch.device, fn, *args) -> None:
-    if device.index == torch.cuda.current_device():
-        status = fn(*args, _stream(device))
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(index) if _raw_stream else _stream(device))
     else:
         with torch.cuda.device(device):
             status = fn(*args, _stream(device))
@@ -40,22 +46,24 @@ def _call(device: torch.device, fn, *args) -> None:
 def _rows(t: torch.Tensor, name: str) -> tuple[int, int, int]:
     """(rows, cols, pitch) of a tensor whose rows are contiguous and evenly spaced."""
     cols = t.size(-1)
-    rows = t.numel() // cols if cols else 0
     if t.is_contiguous():
-        return rows, cols, cols
-    _check(t.dim() == 2 and (cols <= 1 or t.stride(1) == 1) and t.stride(0) >= cols,
-           f"{name} must be contiguous, or a matrix with contiguous rows")
-    return rows, cols, t.stride(0)
+        return (t.numel() // cols if cols else 0), cols, cols
+    if not (t.dim() == 2 and (cols <= 1 or t.stride(1) == 1) and t.stride(0) >= cols):
+        raise RuntimeError(f"{name} must be contiguous, or a matrix with contiguous rows")
+    return t.size(0), cols, t.stride(0)
 
 
-def _check_packed(codes: torch.Tensor, scales: torch.Tensor, shape, device: torch.device) -> None:
-    """codes and scales of a matrix of ``shape`` (its last size: columns)."""
-    lead, n = tuple(shape[:-1]), blocks(shape[-1])
-    _check(codes.dtype == torch.uint8 and scales.dtype == torch.uint8, "codes and scales must be uint8")
-    _check(codes.is_contiguous() and scales.is_contiguous(), "codes and scales must be contiguous")
-    _check(codes.device == device and scales.device == device, "buffers must share a device")
-    _check(tuple(codes.shape) == (*lead, n * 16) and tuple(scales.shape) == (*lead, n),
-           "codes and scales do not fit the matrix")
+def _check_packed(codes: torch.Tensor, scales: torch.Tensor, lead: tuple, cols: int, device: torch.device) -> None:
+    """codes and scales of a matrix of shape (*lead, cols)."""
+    n = -(-cols // BLOCK)
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise RuntimeError("codes and scales must be uint8")
+    if not (codes.is_contiguous() and scales.is_contiguous()):
+        raise RuntimeError("codes and scales must be contiguous")
+    if codes.device != device or scales.device != device:
+        raise RuntimeError("buffers must share a device")
+    if codes.shape != (*lead, n * 16) or scales.shape != (*lead, n):
+        raise RuntimeError("codes and scales do not fit the matrix")
 
 
 def mx4_empty(*shape: int, device=None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -75,7 +83,7 @@ def mx4_quantize_out(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor)
     _check(x.is_cuda and x.dtype in _TYPES and x.dim() >= 1, "x must be a CUDA FP16, BF16 or FP32 tensor")
     _check(not x.requires_grad, "inference only: disable gradients")
     rows, cols, pitch = _rows(x, "x")
-    _check_packed(codes, scales, x.shape, x.device)
+    _check_packed(codes, scales, x.shape[:-1], cols, x.device)
     _call(x.device, _lib.lib().swb_mx4_quantize, _TYPES[x.dtype], x.data_ptr(), pitch, codes.data_ptr(),
           scales.data_ptr(), rows, cols)
 
@@ -93,7 +101,7 @@ def mx4_dequantize_out(codes: torch.Tensor, scales: torch.Tensor, out: torch.Ten
     rounds what its range does not hold."""
     _check(out.is_cuda and out.dtype in _TYPES and out.dim() >= 1, "out must be a CUDA FP16, BF16 or FP32 tensor")
     rows, cols, pitch = _rows(out, "out")
-    _check_packed(codes, scales, out.shape, out.device)
+    _check_packed(codes, scales, out.shape[:-1], cols, out.device)
     _call(out.device, _lib.lib().swb_mx4_dequantize, _TYPES[out.dtype], codes.data_ptr(), scales.data_ptr(),
           out.data_ptr(), pitch, rows, cols)
 
@@ -109,12 +117,14 @@ def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, cols: int | None =
 
 
 def _product_arguments(out, like, tokens, rows, bias, residual):
-    _check(tuple(out.shape) == (tokens, rows) and out.is_contiguous(), "out must be contiguous [tokens, rows]")
-    for t, shape, name in ((bias, (rows,), "bias"), (residual, (tokens, rows), "residual")):
+    if out.shape != (tokens, rows) or not out.is_contiguous():
+        raise RuntimeError("out must be contiguous [tokens, rows]")
+    for t, shape in ((bias, (rows,)), (residual, (tokens, rows))):
         if t is not None:
-            _check(t.dtype == like and t.device == out.device and t.is_contiguous() and tuple(t.shape) == shape,
-                   f"{name} does not fit the product")
-            _check(not t.requires_grad, "inference only: disable gradients")
+            if t.dtype != like or t.device != out.device or not t.is_contiguous() or t.shape != shape:
+                raise RuntimeError("bias must be [rows], residual [tokens, rows], contiguous and of the tokens' type")
+            if t.requires_grad:
+                raise RuntimeError("inference only: disable gradients")
 
 
 def mx4_project_out(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor,
@@ -132,7 +142,7 @@ def mx4_project_out(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, 
     tokens, rows = x.size(0), codes.size(0)
     cols, pitch = x.size(1), x.stride(0) if tokens > 1 else x.size(1)
     _check((cols <= 1 or x.stride(1) == 1) and pitch >= cols, "x must have contiguous rows")
-    _check_packed(codes, scales, (rows, cols), x.device)
+    _check_packed(codes, scales, (rows,), cols, x.device)
     _product_arguments(out, x.dtype, tokens, rows, bias, residual)
     flags = (_lib.SWB_RESIDUAL if residual is not None else 0) | \
             (_lib.SWB_HALF_OUT if out.dtype == x.dtype else 0)
@@ -162,8 +172,8 @@ def mx4_matmul_out(x_codes: torch.Tensor, x_scales: torch.Tensor, codes: torch.T
     _check(out.is_cuda and out.dtype in (torch.float16, torch.bfloat16), "out must be a CUDA FP16 or BF16 matrix")
     _check(x_codes.dim() == 2 and codes.dim() == 2 and x_scales.dim() == 2, "codes must be matrices")
     tokens, rows, cols = x_codes.size(0), codes.size(0), x_scales.size(1) * BLOCK
-    _check_packed(x_codes, x_scales, (tokens, cols), out.device)
-    _check_packed(codes, scales, (rows, cols), out.device)
+    _check_packed(x_codes, x_scales, (tokens,), cols, out.device)
+    _check_packed(codes, scales, (rows,), cols, out.device)
     _product_arguments(out, out.dtype, tokens, rows, bias, residual)
     _call(out.device, _lib.lib().swb_mx4_matmul, _TYPES[out.dtype], x_codes.data_ptr(), x_scales.data_ptr(),
           codes.data_ptr(), scales.data_ptr(), None if bias is None else bias.data_ptr(),
