@@ -54,12 +54,14 @@ int launch_moe(MoeParams P, cudaStream_t stream) {
     return launch_ex(kernel, unsigned(sms), S::Pipe::kThreads, S::kSmem, stream, true, maps, P);
 }
 
-template <typename T, bool MX>
-int dispatch_moe(const MoeParams& P, cudaStream_t stream) {
+template <typename T>
+int dispatch_moe(bool mx, const MoeParams& P, cudaStream_t stream) {
+    // four-bit experts come here with up to eight tokens only (moe_wide_takes)
+    if (mx) return launch_moe<T, true, 1>(P, stream);
     // an expert can be given every token; beyond 32 in groups of 32
-    if (P.tokens <= 8) return launch_moe<T, MX, 1>(P, stream);
-    if (P.tokens <= 16) return launch_moe<T, MX, 2>(P, stream);
-    return launch_moe<T, MX, 4>(P, stream);
+    if (P.tokens <= 8) return launch_moe<T, false, 1>(P, stream);
+    if (P.tokens <= 16) return launch_moe<T, false, 2>(P, stream);
+    return launch_moe<T, false, 4>(P, stream);
 }
 
 }  // namespace
@@ -147,14 +149,14 @@ int swb_moe(int type, unsigned flags, const void* x, int64_t x_pitch, const void
     P.inter = inter;
     P.experts = experts;
     P.topk = topk;
+    P.group = kMoeGroup;
     P.h_pitch = moe_h_pitch(inter);
     P.renormalize = (flags & SWB_MOE_RENORMALIZE) != 0;
     P.x_aligned = hidden % 8 == 0 && x_pitch % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
     P.router_aligned = hidden % 8 == 0 && reinterpret_cast<uintptr_t>(router) % 16 == 0;
     auto s = static_cast<cudaStream_t>(stream);
     if (moe_wide_takes(P, mx)) return moe_wide(type, mx, P, s);
-    if (type == SWB_F16) return mx ? dispatch_moe<__half, true>(P, s) : dispatch_moe<__half, false>(P, s);
-    return mx ? dispatch_moe<__nv_bfloat16, true>(P, s) : dispatch_moe<__nv_bfloat16, false>(P, s);
+    return type == SWB_F16 ? dispatch_moe<__half>(mx, P, s) : dispatch_moe<__nv_bfloat16>(mx, P, s);
 }
 
 }  // extern "C"

@@ -40,14 +40,14 @@ struct WideMaps {
 
 // SPLIT: tokens are split into pieces at each use; else once, ahead of the items, into the
 // workspace, which holds the pieces of kMoePieceDim values a token.
-template <typename T_, bool MX, bool SPLIT>
+template <typename T_, bool MX, bool SPLIT, int TOK>
 struct GateWork {
     using T = T_;
     static constexpr bool kMx = MX, kLoad = SPLIT || !MX, kGather = MX && !SPLIT;
     static constexpr int kPieces = MX ? (std::is_same<T, __half>::value ? 3 : 2) : 1;
-    static constexpr int kTok = kMoeGroup, kAccs = 2, kPerSm = 1;
-    static constexpr int kStages = MX ? 3 : 8, kRaw = 4, kTokenStages = MX ? 5 : 6;
-    static constexpr int kSpreadGroups = 2, kSplitters = MX ? 5 : 6, kGroupWarps = 1;
+    static constexpr int kTok = TOK, kAccs = 2, kPerSm = 1;
+    static constexpr int kStages = MX ? 3 : 8, kRaw = 4, kTokenStages = MX ? (TOK == 16 ? 10 : 5) : 6;
+    static constexpr int kSpreadGroups = 2, kSplitters = kTokenStages, kGroupWarps = 1;
 
     const unsigned char* sa[2];
     const unsigned char *sb, *pieces;
@@ -122,14 +122,14 @@ struct GateWork {
     }
 };
 
-template <typename T_, bool MX>
+template <typename T_, bool MX, int TOK>
 struct DownWork {
     using T = T_;
     static constexpr bool kMx = MX, kLoad = false, kGather = false;
     static constexpr int kPieces = h_pieces(MX);
-    static constexpr int kTok = kMoeGroup, kAccs = 2, kPerSm = 1;
-    static constexpr int kStages = MX ? 3 : 7, kRaw = 4, kTokenStages = MX ? 4 : 6;
-    static constexpr int kSpreadGroups = 2, kSplitters = 4, kGroupWarps = 1;
+    static constexpr int kTok = TOK, kAccs = 2, kPerSm = 1;
+    static constexpr int kStages = MX ? 3 : 7, kRaw = 4, kTokenStages = MX ? (TOK == 16 ? 8 : 4) : 6;
+    static constexpr int kSpreadGroups = 2, kSplitters = MX ? kTokenStages : 4, kGroupWarps = 1;
 
     const unsigned char* sa[2];
     const unsigned char *sb, *pieces;
@@ -189,28 +189,28 @@ __device__ void split_tokens(const MoeParams& P) {
     }
 }
 
-template <typename T, bool MX, bool SPLIT>
+template <typename T, bool MX, bool SPLIT, int TOK>
 struct GateShape {
-    using Pipe = Wide<GateWork<T, MX, SPLIT>>;
+    using Pipe = Wide<GateWork<T, MX, SPLIT, TOK>>;
     static constexpr size_t kPart = Pipe::kRing;
-    static constexpr size_t kRoute = (kPart + kMoeGroup * kWidePartPitch * 4 + 15) / 16 * 16;
+    static constexpr size_t kRoute = (kPart + TOK * kWidePartPitch * 4 + 15) / 16 * 16;
     static constexpr size_t kSmem = kRoute + sizeof(MoeRoute) + 1024;
     static_assert(kSmem + 2048 <= kSmemPerCtaMax, "shared memory");
 };
-template <typename T, bool MX>
+template <typename T, bool MX, int TOK>
 struct DownShape {
-    using Pipe = Wide<DownWork<T, MX>>;
+    using Pipe = Wide<DownWork<T, MX, TOK>>;
     static constexpr size_t kTotal = Pipe::kRing;
     static constexpr size_t kRoute = kTotal + kMoeMaxTokens * kWideM * 4;
     static constexpr size_t kSmem = kRoute + sizeof(MoeRoute) + 1024;
     static_assert(kSmem + 1024 <= kSmemPerCtaMax, "shared memory");
 };
 
-template <typename T, bool MX, bool SPLIT>
-__global__ void __launch_bounds__(Wide<GateWork<T, MX, SPLIT>>::kThreads, 1)
+template <typename T, bool MX, bool SPLIT, int TOK>
+__global__ void __launch_bounds__(Wide<GateWork<T, MX, SPLIT, TOK>>::kThreads, 1)
     moe_gate_kernel(const __grid_constant__ WideMaps maps, const __grid_constant__ MoeParams P) {
-    using S = GateShape<T, MX, SPLIT>;
-    using Work = GateWork<T, MX, SPLIT>;
+    using S = GateShape<T, MX, SPLIT, TOK>;
+    using Work = GateWork<T, MX, SPLIT, TOK>;
     constexpr int kWideThreads = S::Pipe::kThreads;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ typename S::Pipe::Shared sh;
@@ -255,12 +255,12 @@ __global__ void __launch_bounds__(Wide<GateWork<T, MX, SPLIT>>::kThreads, 1)
     S::Pipe::finish(sh);
 }
 
-template <typename T, bool MX>
-__global__ void __launch_bounds__(Wide<DownWork<T, MX>>::kThreads, 1)
+template <typename T, bool MX, int TOK>
+__global__ void __launch_bounds__(Wide<DownWork<T, MX, TOK>>::kThreads, 1)
     moe_down_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_h,
                     const __grid_constant__ MoeParams P, int splits, int halves) {
-    using S = DownShape<T, MX>;
-    using Work = DownWork<T, MX>;
+    using S = DownShape<T, MX, TOK>;
+    using Work = DownWork<T, MX, TOK>;
     constexpr int kWideThreads = S::Pipe::kThreads;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ typename S::Pipe::Shared sh;
@@ -319,15 +319,15 @@ __global__ void __launch_bounds__(Wide<DownWork<T, MX>>::kThreads, 1)
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-template <typename T, bool MX, bool SPLIT>
+template <typename T, bool MX, bool SPLIT, int TOK>
 int launch_moe_wide(const MoeParams& P, cudaStream_t stream) {
     static std::atomic<uint64_t> gate_set{0}, down_set{0};
     const int sms = sm_count();
     if (sms <= 0) return check_launch();
-    using G = GateShape<T, MX, SPLIT>;
-    using D = DownShape<T, MX>;
-    auto gate = moe_gate_kernel<T, MX, SPLIT>;
-    auto down = moe_down_kernel<T, MX>;
+    using G = GateShape<T, MX, SPLIT, TOK>;
+    using D = DownShape<T, MX, TOK>;
+    auto gate = moe_gate_kernel<T, MX, SPLIT, TOK>;
+    auto down = moe_down_kernel<T, MX, TOK>;
     if (int rc = allow_smem(gate, gate_set, G::kSmem)) return rc;
     if (int rc = allow_smem(down, down_set, D::kSmem)) return rc;
     WideMaps maps;
@@ -380,14 +380,26 @@ bool moe_wide_takes(const MoeParams& P, bool mx) {
            wide_rows(P.w[2], P.inter, mx);
 }
 
-int moe_wide(int type, bool mx, const MoeParams& P, cudaStream_t stream) {
-    const bool half = type == SWB_F16;
-    if (!mx) return half ? launch_moe_wide<__half, false, false>(P, stream) : launch_moe_wide<__nv_bfloat16, false, false>(P, stream);
+namespace {
+template <typename T>
+int dispatch_moe_wide(bool mx, MoeParams P, cudaStream_t stream) {
+    if (!mx) return launch_moe_wide<T, false, false, kMoeGroup>(P, stream);
     // longer tokens than the workspace's pieces are split at each use: every item of an expert repeats
     // the conversions (four-bit experts of 14336 x 4096, 32 tokens: 330 us of gate against 190)
-    if (P.hidden > kMoePieceDim)
-        return half ? launch_moe_wide<__half, true, true>(P, stream) : launch_moe_wide<__nv_bfloat16, true, true>(P, stream);
-    return half ? launch_moe_wide<__half, true, false>(P, stream) : launch_moe_wide<__nv_bfloat16, true, false>(P, stream);
+    const bool split = P.hidden > kMoePieceDim;
+    // Four-bit items of 16 tokens leave shared memory for twice the stages of tokens: 247 us against
+    // 273 (32 tokens, 2 of 8 experts of 14336 x 4096). An expert with more tokens is then read twice:
+    // 118 us against 101 (64 tokens, 2 of 8 experts of 5632 x 2048, 16 each on average).
+    if (P.tokens * P.topk <= 8 * P.experts) {
+        P.group = kMoeFewGroup;
+        return split ? launch_moe_wide<T, true, true, kMoeFewGroup>(P, stream) : launch_moe_wide<T, true, false, kMoeFewGroup>(P, stream);
+    }
+    return split ? launch_moe_wide<T, true, true, kMoeGroup>(P, stream) : launch_moe_wide<T, true, false, kMoeGroup>(P, stream);
+}
+}  // namespace
+
+int moe_wide(int type, bool mx, const MoeParams& P, cudaStream_t stream) {
+    return type == SWB_F16 ? dispatch_moe_wide<__half>(mx, P, stream) : dispatch_moe_wide<__nv_bfloat16>(mx, P, stream);
 }
 
 }  // namespace swb

@@ -105,6 +105,68 @@ def test_all_tokens_to_one_expert_and_ties():
     check(d, v, 1, True, got)
 
 
+def test_four_bit_experts_with_more_tokens_than_an_item():
+    """Few tokens an expert on average, but every token at the same two experts."""
+    d, v = layer(11, 64, 16, 96, 70, torch.bfloat16, True)
+    d["router"].zero_()
+    check(d, v, 2, True, call(d, 2))
+    d, v = layer(12, 19, 12, 160, 33, torch.float16, True)
+    d["router"].zero_()
+    check(d, v, 1, False, call(d, 1, False))
+
+
+@pytest.mark.parametrize("hidden", [8192, 8200])
+@pytest.mark.parametrize("tokens,experts", [(12, 3), (10, 12)])
+def test_long_four_bit_tokens(hidden, tokens, experts):
+    """Up to the length whose pieces the workspace holds, and beyond it."""
+    for dtype in (torch.float16, torch.bfloat16):
+        d, v = layer(hidden, tokens, experts, hidden, 40, dtype, True)
+        check(d, v, 2, True, call(d, 2))
+
+
+def test_misaligned_four_bit_layer():
+    """Scales and tokens off a word, a short last block, for few and for more tokens."""
+    for tokens in (3, 13):
+        d, v = layer(13, tokens, 4, 104, 72, torch.float16, True)
+        for name in ("gate_scales", "up_scales", "down_scales", "router", "x"):
+            room = torch.zeros(d[name].numel() + 1, dtype=d[name].dtype, device="cuda")
+            room[1:] = d[name].flatten()
+            d[name] = room[1:].view_as(d[name])
+        check(d, v, 2, True, call(d, 2))
+
+
+def test_few_and_more_tokens_share_a_workspace_and_graphs():
+    """One workspace for both sizes of batch in turn; two captured graphs with a workspace each,
+    replayed on two streams at once."""
+    sets = [layer(30 + t, t, 8, 128, 96, torch.float16, q)[0] for t, q in ((4, True), (24, True), (24, False))]
+    ws = S.moe_workspace(24, 8, 2, 96)
+    first = [call(d, 2, workspace=ws) for d in sets]
+    for _ in range(2):
+        for d, want in zip(sets, first):
+            assert all(torch.equal(a, b) for a, b in zip(call(d, 2, workspace=ws), want))
+    graphs, outs = [], []
+    for _ in range(2):
+        own = S.moe_workspace(24, 8, 2, 96)
+        y = [torch.zeros_like(d["x"]) for d in sets]
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            for d, t in zip(sets, y):
+                S.moe_out(d["x"], d["router"], d["gate"], d["up"], d["down"], t, own, 2,
+                          **{k: d[k] for k in d if k.endswith("_scales")})
+        graphs.append((g, own))
+        outs.append(y)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for stream, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                g.replay()
+    torch.cuda.synchronize()
+    for y in outs:
+        assert all(torch.equal(t, want[0]) for t, want in zip(y, first))
+    assert binding.device_error() == 0
+
+
 @pytest.mark.parametrize("tokens,hidden,four_bit", [(4, 64, False), (4, 64, True), (12, 128, False), (12, 128, True)])
 def test_non_finite_tokens(tokens, hidden, four_bit):
     """A NaN or infinite value makes its token NaN or infinite and leaves the others as they are."""
