@@ -26,7 +26,6 @@ bool overlaps(const void* a, size_t abytes, const void* b, size_t bbytes);
 
 // Device error words of the other translation units (each holds its own).
 int moe_device_error(int clear, int* out);
-int mx4_device_error(int clear, int* out);
 int mx4_matmul_device_error(int clear, int* out);
 int mx4_wide_device_error(int clear, int* out);
 int moe_wide_device_error(int clear, int* out);

@@ -2,7 +2,6 @@
 // weight matrix with 16-bit tokens (declarations: include/swiglu_b200.h).
 #include <algorithm>
 #include <cstring>
-#include <type_traits>
 
 #include "host.h"
 #include "project.h"
@@ -255,126 +254,7 @@ int convert(int type, const void* from, void* to, int64_t pitch, const void* cod
     }
 }
 
-// ---------------------------------------------------------------- product
-template <typename T, int NT>
-struct ProjectShape {
-    using Pipe = Stream<T, true, NT>;
-    static constexpr int kStages = Pipe::stages(0);
-    static constexpr size_t kSmem = Pipe::bytes(kStages);
-};
-
-template <typename T, int NT>
-__global__ void __launch_bounds__(Stream<T, true, NT>::kThreads, 1)
-    project_kernel(const __grid_constant__ WeightMaps maps, const ProjectParams P) {
-    using Shape = ProjectShape<T, NT>;
-    using Pipe = typename Shape::Pipe;
-    extern __shared__ __align__(1024) unsigned char smem[];
-    constexpr int kConsumers = Pipe::kConsumers;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const auto l = Pipe::layout(smem_u32(smem), Shape::kStages);
-    if (threadIdx.x == 0) Pipe::init(l);
-    __syncthreads();
-
-    const int64_t first = int64_t(blockIdx.x) * P.items / gridDim.x;
-    const int64_t last = int64_t(blockIdx.x + 1) * P.items / gridDim.x;
-    const WeightView one = weight_view<true>(P.w, P.s, P.rows, P.cols, P.fast ? &maps : nullptr, P.deep);
-    const WeightView v[2] = {one, one};
-    typename Pipe::Place place;
-    auto tiles = [&](int64_t item) {
-        Tiles<2> t;
-        for (int m = 0; m < 2; ++m) {
-            t.row[m] = item % P.tiles * 32 + m * kTileRows;
-            t.rows[m] = int(min(int64_t(kTileRows), max(int64_t(0), P.rows - t.row[m])));
-        }
-        return t;
-    };
-    if (warp == kConsumers) {
-        const uint64_t policy = P.items > P.tiles ? l2_normal_policy() : l2_evict_first_policy();
-        for (int64_t i = first; i < last && place.ok; ++i) Pipe::template produce<2>(l, place, tiles(i), v, policy);
-        Pipe::drain(l, place);
-    } else if (warp < kConsumers) {
-        auto items = [&](auto fast) {
-            typename Pipe::template Tokens<2, false> tokens;
-            auto turn_to = [&](int64_t i) {
-                const int64_t t0 = i / P.tiles * (NT * 8);
-                tokens.count = i < last ? int(min(int64_t(NT * 8), P.tokens - t0)) : 0;
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    tokens.x[n] = static_cast<const T*>(P.x) + (t0 + min(n * 8 + (lane >> 2), max(tokens.count - 1, 0))) * P.x_pitch;
-            };
-            turn_to(first);
-            tokens.template load<decltype(fast)::value>(0, 0, P.cols);
-            for (int64_t i = first; i < last && place.ok; ++i)
-                Pipe::template consume<2, false, decltype(fast)::value>(l, place, tiles(i), v, tokens, P.cols,
-                                                                        [&](auto&) { turn_to(i + 1); });
-        };
-        if (P.fast)
-            items(std::true_type{});
-        else
-            items(std::false_type{});
-    } else {
-        const int thread = threadIdx.x - (kConsumers + 1) * 32;
-        for (int64_t i = first; i < last && Pipe::acquire(l, place); ++i) {
-            const int64_t t0 = i / P.tiles * (NT * 8);
-            const int count = int(min(int64_t(NT * 8), P.tokens - t0)), row0 = int(i % P.tiles) * 32;
-            for (int e = thread; e < count * 32; e += kEpilogueThreads) {
-                const int t = e >> 5, row = row0 + (e & 31);
-                if (row >= P.rows) continue;
-                float a = Pipe::template sum<2>(l, place, (e & 31) >> 4, t, e & 15);
-                if (P.bias) a += Num<T>::to_float(static_cast<const T*>(P.bias)[row]);
-                const int64_t at = (t0 + t) * P.rows + row;
-                if (P.residual) a += Num<T>::to_float(static_cast<const T*>(P.residual)[at]);
-                if (P.half_out)
-                    static_cast<T*>(P.out)[at] = Num<T>::from_float(a);
-                else
-                    static_cast<float*>(P.out)[at] = a;
-            }
-            Pipe::release(l, place);
-        }
-    }
-}
-
-template <typename T, int NT>
-int launch_project(ProjectParams P, cudaStream_t stream) {
-    using Shape = ProjectShape<T, NT>;
-    static std::atomic<uint64_t> smem_set{0};
-    const int sms = sm_count();
-    if (sms <= 0) return check_launch();
-    auto kernel = project_kernel<T, NT>;
-    static_assert(Shape::kStages >= 3, "a ring");
-    if (int rc = allow_smem(kernel, smem_set, Shape::kSmem)) return rc;
-    WeightMaps maps;
-    const int64_t blocks = mx_blocks(P.cols);
-    if (int rc = make_weight_maps(&maps, P.w, P.s, P.rows, blocks * kMxBlockBytes, blocks, &P.fast, &P.deep)) return rc;
-    // one way of reading for the copies and the consumers
-    P.fast = P.fast && P.x_aligned;
-    P.tiles = (P.rows + 31) / 32;
-    P.items = int64_t(P.tiles) * ((P.tokens + NT * 8 - 1) / (NT * 8));
-    const unsigned grid = unsigned(std::min<int64_t>(P.items, sms));
-    return launch_ex(kernel, grid, Shape::Pipe::kThreads, Shape::kSmem, stream, false, maps, P);
-}
-
-template <typename T>
-int dispatch_project(const ProjectParams& P, cudaStream_t stream) {
-    if (P.tokens <= 8) return launch_project<T, 1>(P, stream);
-    if (P.tokens <= 16) return launch_project<T, 2>(P, stream);
-    return launch_project<T, 4>(P, stream);
-}
-
 }  // namespace
-
-int mx4_device_error(int clear, int* out) {
-    int v = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(&v, g_device_error, sizeof v);
-    if (e == cudaSuccess && clear) {
-        const int zero = 0;
-        e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof zero);
-    }
-    if (e != cudaSuccess) return fail(SWB_E_CUDA, cudaGetErrorString(e));
-    *out = v;
-    return SWB_OK;
-}
-
 }  // namespace swb
 
 using namespace swb;
@@ -430,9 +310,7 @@ int swb_mx4_project(int type, const void* codes, const void* scales, const void*
     P.half_out = half;
     P.x_aligned = cols % 8 == 0 && x_pitch % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
     auto s = static_cast<cudaStream_t>(stream);
-    if (project_deep_takes(P)) return project_deep(type, P, s);
-    if (project_wide_takes(P)) return project_wide(type, P, s);
-    return type == SWB_F16 ? dispatch_project<__half>(P, s) : dispatch_project<__nv_bfloat16>(P, s);
+    return project_deep_takes(P) ? project_deep(type, P, s) : project_wide(type, P, s);
 }
 
 }  // extern "C"

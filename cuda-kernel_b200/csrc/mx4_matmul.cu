@@ -7,10 +7,10 @@
 // blocks' power-of-two scales itself, so codes go from global memory to the tensor
 // core untouched: TMA brings 256 values (128 bytes) of every row of both tiles into a
 // 128-byte swizzled stage; four warps bring the scale bytes of the same rows into
-// the 32 x 16-byte blocks that tcgen05.cp spreads over TMEM; one thread issues the
-// copies and products; four warps drain the accumulators.
+// the 32 x 16-byte blocks that tcgen05.cp spreads over TMEM; a thread each issues the
+// copies and the products; eight warps drain the accumulators.
 //
-// Long batches (tokens on the M side, MT x 128 of them by N = 192 rows of W): two
+// Long batches (tokens on the M side, 128 of them by N = 192 rows of W): two
 // accumulators of 192 columns and the stages' scales fill TMEM. Without sharing a
 // tile between CTAs the bytes that L2 hands out bound this kernel (0.5 B per value at
 // 4x the rate of 16-bit products), hence the large tile.
@@ -64,19 +64,18 @@ struct MatmulParams {
     int splits;               // CTAs of a cluster that share a tile's K
 };
 
-template <int N, int MT, bool TOKENS_M>
+template <int N, bool TOKENS_M>
 struct MatmulShape {
-    static constexpr int kStages = TOKENS_M ? (MT == 2 ? 3 : 4) : (N <= 32 ? 5 : 4);
+    static constexpr int kStages = TOKENS_M || N > 32 ? 4 : 5;
     static constexpr int kPerSm = TOKENS_M || N > 64 ? 1 : 2;
-    static constexpr int kRowsA = MT * kMmaM;
-    static constexpr int kBytesA = kRowsA * kRowBytes, kBytesB = N * kRowBytes;
+    static constexpr int kBytesA = kMmaM * kRowBytes, kBytesB = N * kRowBytes;
     static constexpr int kBlocksB = (N + kMmaM - 1) / kMmaM;   // 128-row blocks of scales of the N side
-    static constexpr int kScales = 2 * (MT + kBlocksB) * kScaleBlock;
+    static constexpr int kScales = 2 * (1 + kBlocksB) * kScaleBlock;
     static constexpr int kStage = kBytesA + kBytesB + kScales;
     static_assert(!TOKENS_M || N % kTurnColumns == 0, "whole turns");
     static_assert(kStage % 1024 == 0, "stages keep the swizzle's alignment");
     static constexpr int kAccs = TOKENS_M ? 2 : 1;             // accumulators of N columns
-    static constexpr int kScaleColumns = 2 * (MT + kBlocksB) * 4;
+    static constexpr int kScaleColumns = 2 * (1 + kBlocksB) * 4;
     static constexpr int kUsed = kAccs * N + kStages * kScaleColumns;
     static constexpr int kColumns = kUsed <= 32 ? 32 : kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
     static_assert(kUsed <= 512, "TMEM columns");
@@ -94,11 +93,11 @@ __device__ __forceinline__ float load_value(const void* p, int64_t i) {
     return Num<T>::to_float(static_cast<const T*>(p)[i]);
 }
 
-template <typename T, int N, int MT, bool TOKENS_M>
-__global__ void __launch_bounds__(kThreads, MatmulShape<N, MT, TOKENS_M>::kPerSm)
+template <typename T, int N, bool TOKENS_M>
+__global__ void __launch_bounds__(kThreads, MatmulShape<N, TOKENS_M>::kPerSm)
     matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const MatmulParams P) {
-    using S = MatmulShape<N, MT, TOKENS_M>;
+    using S = MatmulShape<N, TOKENS_M>;
     extern __shared__ unsigned char raw[];
     __shared__ uint64_t full[S::kStages], scaled[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2];
     __shared__ uint32_t s_tmem;
@@ -146,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, MatmulShape<N, MT, TOKENS_M>::kPerSm
                     }
                     const uint32_t bar = smem_u32(full + s), at = base + s * S::kStage;
                     mbar_arrive_expect_tx(bar, S::kBytesA + S::kBytesB);
-                    tma_load_2d(at, &map_a, k * (kRowBytes / 4), a * S::kRowsA, bar);
+                    tma_load_2d(at, &map_a, k * (kRowBytes / 4), a * kMmaM, bar);
                     tma_load_2d(at + S::kBytesA, &map_b, k * (kRowBytes / 4), b * N, bar);
                     ++issued;
                     if (++s == S::kStages) s = 0, ph ^= 1u;
@@ -176,35 +175,24 @@ __global__ void __launch_bounds__(kThreads, MatmulShape<N, MT, TOKENS_M>::kPerSm
                     const uint32_t at = base + s * S::kStage, sc = at + S::kBytesA + S::kBytesB;
                     const uint32_t col = scale_columns + s * S::kScaleColumns;
 #pragma unroll
-                    for (int i = 0; i < 2 * (MT + S::kBlocksB); ++i)
+                    for (int i = 0; i < 2 * (1 + S::kBlocksB); ++i)
                         scale_copy(col + 4 * i, scale_desc(sc + i * kScaleBlock));
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        const int use = MT == 2 ? m : acc;
-                        // the accumulator's last tile has been read
-                        if (k == k0 && done >= (MT == 2 ? 1 : S::kAccs)) {
-                            ok = mbar_wait(smem_u32(acc_empty + use), aph ^ 1u);
-                            if (!ok) break;
-                            fence_after();
-                        }
-                        const uint64_t da = operand_desc(at + m * kMmaM * kRowBytes), db = operand_desc(at + S::kBytesA);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)  // 64 values a step; scales: blocks of 128 values, then rows
-                            mma_mxf4(tmem + use * N, da + 2 * i, db + 2 * i, mxf4_desc(kMmaM, N, (i & 1) * 2),
-                                     col + ((i >> 1) * MT + m) * 4, col + (2 * MT + (i >> 1) * S::kBlocksB) * 4,
-                                     k > k0 || i > 0);
+                    // the accumulator's last tile has been read
+                    if (k == k0 && done >= S::kAccs) {
+                        ok = mbar_wait(smem_u32(acc_empty + acc), aph ^ 1u);
+                        if (!ok) break;
+                        fence_after();
                     }
-                    if (!ok) break;
+                    const uint64_t da = operand_desc(at), db = operand_desc(at + S::kBytesA);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)  // 64 values a step; scales: blocks of 128 values, then rows
+                        mma_mxf4(tmem + acc * N, da + 2 * i, db + 2 * i, mxf4_desc(kMmaM, N, (i & 1) * 2),
+                                 col + (i >> 1) * 4, col + (2 + (i >> 1) * S::kBlocksB) * 4, k > k0 || i > 0);
                     mma_commit(smem_u32(empty + s));
-                    if (k == k1 - 1) {
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) mma_commit(smem_u32(acc_full + (MT == 2 ? m : acc)));
-                    }
+                    if (k == k1 - 1) mma_commit(smem_u32(acc_full + acc));
                     if (++s == S::kStages) s = 0, ph ^= 1u;
                 }
-                if (MT == 2 || S::kAccs == 1) {
-                    aph ^= 1u;
-                } else if (++acc == S::kAccs) {
+                if (++acc == S::kAccs) {
                     acc = 0;
                     aph ^= 1u;
                 }
@@ -213,27 +201,27 @@ __global__ void __launch_bounds__(kThreads, MatmulShape<N, MT, TOKENS_M>::kPerSm
         }
     } else if (warp >= kEpilogueWarps) {
         // ------------------------------------------------------- scales
-        constexpr int kRows = S::kRowsA + N, kPer = (kRows + 127) / 128;
+        constexpr int kRows = kMmaM + N, kPer = (kRows + 127) / 128;
         // A warp's lanes take rows 8 apart in four quarters of 128: their words lie side by side.
         const int lt = threadIdx.x - kEpilogueWarps * 32, t = lt / 32 * 8 + (lt & 7) + (lt >> 3 & 3) * 32;
         int s = 0, issued = 0;
         uint32_t ph = 0;
         bool ok = true;
         for (int64_t tile = first; tile < P.tiles && ok; tile += step) {
-            const int64_t a0 = tile % P.tiles_a * S::kRowsA, b0 = tile / P.tiles_a * N;
+            const int64_t a0 = tile % P.tiles_a * kMmaM, b0 = tile / P.tiles_a * N;
             const unsigned char* row[kPer];
             uint32_t dst[kPer];
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int r = t + 128 * i;
                 row[i] = nullptr;
-                const bool in_a = r < S::kRowsA;
-                const int q = in_a ? r : r - S::kRowsA, in = q & 127;
+                const bool in_a = r < kMmaM;
+                const int q = in_a ? r : r - kMmaM, in = q & 127;
                 const int64_t global = in_a ? a0 + q : b0 + q;
                 if (r < kRows && global < (in_a ? P.rows_a : P.rows_b))
                     row[i] = (in_a ? P.sa : P.sb) + global * P.blocks;
                 // blocks of the M side: [128 values][128 rows], then the N side's
-                dst[i] = (in_a ? q >> 7 : 2 * MT + (q >> 7)) * kScaleBlock + (in & 31) * 16 + (in >> 5) * 4;
+                dst[i] = (in_a ? q >> 7 : 2 + (q >> 7)) * kScaleBlock + (in & 31) * 16 + (in >> 5) * 4;
             }
             // two windows ahead: scales of long rows come from L2 or DRAM
             uint4 window[3][kPer];
@@ -260,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, MatmulShape<N, MT, TOKENS_M>::kPerSm
                 for (int i = 0; i < kPer; ++i) {
                     const int r = t + 128 * i;
                     if (r < kRows) {
-                        const uint32_t next_block = (r < S::kRowsA ? MT : S::kBlocksB) * kScaleBlock;
+                        const uint32_t next_block = (r < kMmaM ? 1 : S::kBlocksB) * kScaleBlock;
                         sts32(sc + dst[i], k & 1 ? window[0][i].z : window[0][i].x);
                         sts32(sc + dst[i] + next_block, k & 1 ? window[0][i].w : window[0][i].y);
                     }
@@ -280,110 +268,104 @@ __global__ void __launch_bounds__(kThreads, MatmulShape<N, MT, TOKENS_M>::kPerSm
         const int quarter = warp % 4, share = warp / 4;  // this warp takes every other group of columns
         const uint32_t quadrant = uint32_t(quarter * 32) << 16;
         for (int64_t tile = first; tile < P.tiles && ok; tile += step) {
-            const int64_t a0 = tile % P.tiles_a * S::kRowsA, b0 = tile / P.tiles_a * N;
-#pragma unroll 1
-            for (int m = 0; m < MT; ++m) {
-                const int use = MT == 2 ? m : acc;
-                // The residual's values for 32 columns of this warp's tokens (a lane: two columns of every
-                // other token), on their way before the accumulator is waited for, the next
-                // ones before these are written.
-                uint32_t residual[16], ahead[16];
-                const int64_t token0 = a0 + m * kMmaM + quarter * 32 + lane / 16;
-                const int tokens = int(min(int64_t(32), P.tokens - token0));
-                auto load_residual = [&](int c) {
-                    if (!TOKENS_M || !P.residual) return;
-                    const int64_t row = b0 + c + lane % 16 * 2;
-                    const T* r = static_cast<const T*>(P.residual) + token0 * P.rows + row;
-                    const bool have0 = row < P.rows, have1 = row + 1 < P.rows;
+            const int64_t a0 = tile % P.tiles_a * kMmaM, b0 = tile / P.tiles_a * N;
+            // The residual's values for 32 columns of this warp's tokens (a lane: two columns of every
+            // other token), on their way before the accumulator is waited for, the next
+            // ones before these are written.
+            uint32_t residual[16], ahead[16];
+            const int64_t token0 = a0 + quarter * 32 + lane / 16;
+            const int tokens = int(min(int64_t(32), P.tokens - token0));
+            auto load_residual = [&](int c) {
+                if (!TOKENS_M || !P.residual) return;
+                const int64_t row = b0 + c + lane % 16 * 2;
+                const T* r = static_cast<const T*>(P.residual) + token0 * P.rows + row;
+                const bool have0 = row < P.rows, have1 = row + 1 < P.rows;
 #pragma unroll
-                    for (int u = 0; u < 16; ++u, r += 2 * P.rows) {
-                        ahead[u] = 0u;
-                        if (2 * u < tokens && have0) {
-                            if (have1 && (reinterpret_cast<uintptr_t>(r) & 3) == 0) {
-                                ahead[u] = *reinterpret_cast<const uint32_t*>(r);
-                            } else {
-                                ahead[u] = *reinterpret_cast<const unsigned short*>(r);
-                                if (have1) ahead[u] |= uint32_t(reinterpret_cast<const unsigned short*>(r)[1]) << 16;
-                            }
+                for (int u = 0; u < 16; ++u, r += 2 * P.rows) {
+                    ahead[u] = 0u;
+                    if (2 * u < tokens && have0) {
+                        if (have1 && (reinterpret_cast<uintptr_t>(r) & 3) == 0) {
+                            ahead[u] = *reinterpret_cast<const uint32_t*>(r);
+                        } else {
+                            ahead[u] = *reinterpret_cast<const unsigned short*>(r);
+                            if (have1) ahead[u] |= uint32_t(reinterpret_cast<const unsigned short*>(r)[1]) << 16;
                         }
-                    }
-                };
-                load_residual(share * kTurnColumns);
-                ok = mbar_wait_warp(smem_u32(acc_full + use), ph);
-                if (!ok) break;
-                fence_after();
-                const int in_tile = m * kMmaM + quarter * 32 + lane;
-                if constexpr (TOKENS_M) {
-                    // A lane holds a token's columns; through shared memory, so that half a warp writes 32
-                    // neighbouring values of one token at a time (a lane storing its own token's 16
-                    // bytes took 40 % of the kernel, single values of ragged rows 80 %).
-                    float* turn = reinterpret_cast<float*>(raw + (base - smem_u32(raw)) + S::kStages * S::kStage) + warp * 32 * kTurnPitch;
-#pragma unroll 1
-                    for (int c = share * kTurnColumns; c < N; c += 2 * kTurnColumns) {
-                        if (P.residual) {
-#pragma unroll
-                            for (int u = 0; u < 16; ++u) residual[u] = ahead[u];
-                            if (c + 2 * kTurnColumns < N) load_residual(c + 2 * kTurnColumns);
-                        }
-                        uint32_t v[32];
-                        __syncwarp();  // the last columns are read
-                        tmem_load32(tmem + quadrant + use * N + c, v);
-                        tmem_load_wait();
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2)
-                            *reinterpret_cast<float2*>(turn + lane * kTurnPitch + j) =
-                                make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
-                        __syncwarp();
-                        const int64_t row = b0 + c + lane % 16 * 2;  // this lane's two columns
-                        const bool have0 = row < P.rows, have1 = row + 1 < P.rows;
-                        float2 bias = make_float2(0.f, 0.f);
-                        if (P.bias) {
-                            if (have0) bias.x = load_value<T>(P.bias, row);
-                            if (have1) bias.y = load_value<T>(P.bias, row + 1);
-                        }
-                        T* o = static_cast<T*>(P.out) + token0 * P.rows + row;
-                        const float* from = turn + lane / 16 * kTurnPitch + lane % 16 * 2;
-#pragma unroll
-                        for (int u = 0; u < 16; ++u, o += 2 * P.rows) {
-                            if (2 * u >= tokens) break;
-                            float2 f = *reinterpret_cast<const float2*>(from + 2 * u * kTurnPitch);
-                            T two[2];
-                            f.x += bias.x;
-                            f.y += bias.y;
-                            if (P.residual) {
-                                *reinterpret_cast<uint32_t*>(two) = residual[u];
-                                f.x += Num<T>::to_float(two[0]);
-                                f.y += Num<T>::to_float(two[1]);
-                            }
-                            two[0] = Num<T>::from_float(f.x);
-                            two[1] = Num<T>::from_float(f.y);
-                            if (have1 && (reinterpret_cast<uintptr_t>(o) & 3) == 0) {
-                                *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(two);
-                            } else {
-                                if (have0) o[0] = two[0];
-                                if (have1) o[1] = two[1];
-                            }
-                        }
-                    }
-                } else {
-                    // a column is a token, a lane a row of W: to shared memory, [token][row]
-                    float* part = reinterpret_cast<float*>(raw + (base - smem_u32(raw)));
-#pragma unroll 1
-                    for (int c = share * 16; c < N; c += 32) {
-                        uint32_t v[16];
-                        __syncwarp();
-                        tmem_load16(tmem + quadrant + use * N + c, v);
-                        tmem_load_wait();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) part[(c + j) * S::kPartPitch + in_tile] = __uint_as_float(v[j]);
                     }
                 }
-                fence_before();
-                mbar_arrive(smem_u32(acc_empty + use));
+            };
+            load_residual(share * kTurnColumns);
+            ok = mbar_wait_warp(smem_u32(acc_full + acc), ph);
+            if (!ok) break;
+            fence_after();
+            const int in_tile = quarter * 32 + lane;
+            if constexpr (TOKENS_M) {
+                // A lane holds a token's columns; through shared memory, so that half a warp writes 32
+                // neighbouring values of one token at a time (a lane storing its own token's 16
+                // bytes took 40 % of the kernel, single values of ragged rows 80 %).
+                float* turn = reinterpret_cast<float*>(raw + (base - smem_u32(raw)) + S::kStages * S::kStage) + warp * 32 * kTurnPitch;
+#pragma unroll 1
+                for (int c = share * kTurnColumns; c < N; c += 2 * kTurnColumns) {
+                    if (P.residual) {
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) residual[u] = ahead[u];
+                        if (c + 2 * kTurnColumns < N) load_residual(c + 2 * kTurnColumns);
+                    }
+                    uint32_t v[32];
+                    __syncwarp();  // the last columns are read
+                    tmem_load32(tmem + quadrant + acc * N + c, v);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2)
+                        *reinterpret_cast<float2*>(turn + lane * kTurnPitch + j) =
+                            make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+                    __syncwarp();
+                    const int64_t row = b0 + c + lane % 16 * 2;  // this lane's two columns
+                    const bool have0 = row < P.rows, have1 = row + 1 < P.rows;
+                    float2 bias = make_float2(0.f, 0.f);
+                    if (P.bias) {
+                        if (have0) bias.x = load_value<T>(P.bias, row);
+                        if (have1) bias.y = load_value<T>(P.bias, row + 1);
+                    }
+                    T* o = static_cast<T*>(P.out) + token0 * P.rows + row;
+                    const float* from = turn + lane / 16 * kTurnPitch + lane % 16 * 2;
+#pragma unroll
+                    for (int u = 0; u < 16; ++u, o += 2 * P.rows) {
+                        if (2 * u >= tokens) break;
+                        float2 f = *reinterpret_cast<const float2*>(from + 2 * u * kTurnPitch);
+                        T two[2];
+                        f.x += bias.x;
+                        f.y += bias.y;
+                        if (P.residual) {
+                            *reinterpret_cast<uint32_t*>(two) = residual[u];
+                            f.x += Num<T>::to_float(two[0]);
+                            f.y += Num<T>::to_float(two[1]);
+                        }
+                        two[0] = Num<T>::from_float(f.x);
+                        two[1] = Num<T>::from_float(f.y);
+                        if (have1 && (reinterpret_cast<uintptr_t>(o) & 3) == 0) {
+                            *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(two);
+                        } else {
+                            if (have0) o[0] = two[0];
+                            if (have1) o[1] = two[1];
+                        }
+                    }
+                }
+            } else {
+                // a column is a token, a lane a row of W: to shared memory, [token][row]
+                float* part = reinterpret_cast<float*>(raw + (base - smem_u32(raw)));
+#pragma unroll 1
+                for (int c = share * 16; c < N; c += 32) {
+                    uint32_t v[16];
+                    __syncwarp();
+                    tmem_load16(tmem + quadrant + acc * N + c, v);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) part[(c + j) * S::kPartPitch + in_tile] = __uint_as_float(v[j]);
+                }
             }
-            if (MT == 2 || S::kAccs == 1) {
-                ph ^= 1u;
-            } else if (++acc == S::kAccs) {
+            fence_before();
+            mbar_arrive(smem_u32(acc_empty + acc));
+            if (++acc == S::kAccs) {
                 acc = 0;
                 ph ^= 1u;
             }
@@ -401,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, MatmulShape<N, MT, TOKENS_M>::kPerSm
         // The cluster's parts, added in rank order; each CTA takes its share of the tile's outputs.
         // A CTA that failed writes nothing, and its peers keep what they could add.
         asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-        const int64_t w0 = first % P.tiles_a * S::kRowsA, t0 = first / P.tiles_a * N;
+        const int64_t w0 = first % P.tiles_a * kMmaM, t0 = first / P.tiles_a * N;
         const int count = int(min(int64_t(N), P.tokens - t0)) * kMmaM;
         if (!s_failed) {
             for (int i = rank * kThreads + threadIdx.x; i < count; i += P.splits * kThreads) {
@@ -433,24 +415,24 @@ struct Side {
     int64_t rows;
 };
 
-template <typename T, int N, int MT, bool TOKENS_M>
+template <typename T, int N, bool TOKENS_M>
 int launch_matmul(const Side& x, const Side& w, MatmulParams P, cudaStream_t stream) {
-    using S = MatmulShape<N, MT, TOKENS_M>;
+    using S = MatmulShape<N, TOKENS_M>;
     static std::atomic<uint64_t> smem_set{0};
     const int sms = sm_count();
     if (sms <= 0) return check_launch();
-    auto kernel = matmul_kernel<T, N, MT, TOKENS_M>;
+    auto kernel = matmul_kernel<T, N, TOKENS_M>;
     if (int rc = allow_smem(kernel, smem_set, S::kSmem)) return rc;
     const Side& a = TOKENS_M ? x : w;
     const Side& b = TOKENS_M ? w : x;
     CUtensorMap map_a, map_b;
-    if (int rc = make_map(&map_a, a.codes, a.rows, int64_t(P.blocks) * kMxBlockBytes, kRowBytes, S::kRowsA)) return rc;
+    if (int rc = make_map(&map_a, a.codes, a.rows, int64_t(P.blocks) * kMxBlockBytes, kRowBytes, kMmaM)) return rc;
     if (int rc = make_map(&map_b, b.codes, b.rows, int64_t(P.blocks) * kMxBlockBytes, kRowBytes, N)) return rc;
     P.sa = a.scales;
     P.sb = b.scales;
     P.rows_a = a.rows;
     P.rows_b = b.rows;
-    P.tiles_a = int((a.rows + S::kRowsA - 1) / S::kRowsA);
+    P.tiles_a = int((a.rows + kMmaM - 1) / kMmaM);
     P.tiles_b = int((b.rows + N - 1) / N);
     P.tiles = int64_t(P.tiles_a) * P.tiles_b;
     P.stages_k = (P.blocks + 7) / 8;
@@ -485,11 +467,11 @@ int launch_matmul(const Side& x, const Side& w, MatmulParams P, cudaStream_t str
 
 template <typename T>
 int dispatch_matmul(const Side& x, const Side& w, const MatmulParams& P, cudaStream_t stream) {
-    if (P.tokens <= 16) return launch_matmul<T, 16, 1, false>(x, w, P, stream);
-    if (P.tokens <= 32) return launch_matmul<T, 32, 1, false>(x, w, P, stream);
-    if (P.tokens <= 64) return launch_matmul<T, 64, 1, false>(x, w, P, stream);
-    if (P.tokens <= 128) return launch_matmul<T, 128, 1, false>(x, w, P, stream);
-    return launch_matmul<T, 192, 1, true>(x, w, P, stream);
+    if (P.tokens <= 16) return launch_matmul<T, 16, false>(x, w, P, stream);
+    if (P.tokens <= 32) return launch_matmul<T, 32, false>(x, w, P, stream);
+    if (P.tokens <= 64) return launch_matmul<T, 64, false>(x, w, P, stream);
+    if (P.tokens <= 128) return launch_matmul<T, 128, false>(x, w, P, stream);
+    return launch_matmul<T, 192, true>(x, w, P, stream);
 }
 
 }  // namespace

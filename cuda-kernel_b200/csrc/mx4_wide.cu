@@ -180,8 +180,6 @@ int dispatch_wide(const ProjectParams& P, cudaStream_t stream) {
 
 }  // namespace
 
-bool project_wide_takes(const ProjectParams&) { return true; }
-
 int project_wide(int type, ProjectParams P, cudaStream_t stream) {
     return type == SWB_F16 ? dispatch_wide<__half>(P, stream) : dispatch_wide<__nv_bfloat16>(P, stream);
 }

@@ -18,14 +18,13 @@ struct ProjectParams {
     int rows, cols;
     int tiles;       // of rows
     int64_t items;   // tiles x groups of tokens
-    bool x_aligned, fast, deep;  // 16-byte pieces of x; make_weight_maps
+    bool x_aligned;  // 16-byte pieces of x
     bool half_out;
 };
 
-// The tensor-core kernel (mx4_wide.cu): takes codes whose rows are whole 64 bytes, on 32 bytes.
-bool project_wide_takes(const ProjectParams& P);
+// Few tokens, split into e4m3 pieces (mx4_wide.cu).
 int project_wide(int type, ProjectParams P, cudaStream_t stream);
-// For more tokens (mx4_deep.cu): takes tokens on 16 bytes.
+// More tokens, W decoded into 16-bit tiles (mx4_deep.cu): takes tokens on 16 bytes.
 bool project_deep_takes(const ProjectParams& P);
 int project_deep(int type, const ProjectParams& P, cudaStream_t stream);
 

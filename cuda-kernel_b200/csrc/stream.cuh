@@ -189,7 +189,7 @@ constexpr int kRingTarget = 160 * 1024;
 template <typename T, bool MX, int NT>
 struct Stream {
     // Decoding four-bit codes for few tokens keeps the schedulers busy only with four warps each.
-    static constexpr int kConsumers = MX && NT <= 2 ? 16 : 8;
+    static constexpr int kConsumers = MX ? 16 : 8;
     static constexpr int kThreads = (kConsumers + 4) * 32;  // consumers, producer, epilogue
     // A stage: 2 tiles of 16 rows by 1 KB, or one tile by 2 KB. With maps: 128 bytes of 16 rows
     // after another (kBox), swizzled by the copy; scales 64 bytes of 16 rows after another.

@@ -875,7 +875,7 @@ int swb_device_error(int clear, int* out) {
         e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof zero);
         if (e != cudaSuccess) return fail(SWB_E_CUDA, cudaGetErrorString(e));
     }
-    for (auto other : {moe_device_error, mx4_device_error, mx4_matmul_device_error, mx4_wide_device_error,
+    for (auto other : {moe_device_error, mx4_matmul_device_error, mx4_wide_device_error,
                        mx4_deep_device_error, moe_wide_device_error}) {
         int more = 0;
         if (int rc = other(clear, &more)) return rc;
