@@ -7,8 +7,9 @@
 //
 //   bf16   code times scale is exact
 //   fp16   code times 2^(scale - largest scale of the row + 13); the epilogue multiplies a row's
-//          column by what is left. Exact for blocks within 2^37 of the row's largest scale; smaller
-//          ones round to multiples of 2^-24 of that range, at most 2^-40 of the row's largest value.
+//          column by what is left. Exact for blocks whose scale is within 2^36 of the row's
+//          largest; a smaller value is off by at most 6 2^-38 of that scale (fp16's subnormals
+//          end there), 2^-37 of the largest value of a row that was rounded from 16 bits.
 //
 // Roles: copies (TMA: 64 values of the tokens a stage, 256 of W's packed rows), decoding
 // warps in groups, stage about, products, eight epilogue warps. Two accumulators,
@@ -195,8 +196,12 @@ __global__ void __launch_bounds__(DeepShape<N>::kThreads, 1)
         uint32_t* tops = reinterpret_cast<uint32_t*>(factors) + kDeepScales * N;
         int slot = 0, tiles = 0;
         bool ok = true;
-        for (int64_t tile = blockIdx.x; tile < P.items && ok; tile += gridDim.x, ++tiles) {
+        for (int64_t tile = blockIdx.x; tile < P.items; tile += gridDim.x, ++tiles) {
             const int64_t w0 = tile / tiles_x * N;
+            if (!ok) {  // a group that gave up still comes to the others' barriers
+                if constexpr (std::is_same<T, __half>::value) named_barrier_sync(1, kAll), named_barrier_sync(1, kAll);
+                continue;
+            }
             if constexpr (std::is_same<T, __half>::value) {  // the rows' largest scales
                 named_barrier_sync(1, kAll);                 // the last tile's are read
                 for (int q = thread; q < N; q += kAll) {

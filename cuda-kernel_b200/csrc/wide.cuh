@@ -12,10 +12,11 @@
 // Roles of a CTA, through two rings of stages of 128 bytes of every row (one for the weights, one
 // for the tokens):
 //   copies     one thread, TMA: two halves of 64 rows of W (gate and up rows, or neighbours)
-//   spreaders  (four-bit) one or two groups of four warps, stage about. Codes arrive packed in a ring of their own, 16 KB a stage, the
-//              bytes in flight, and are spread to the eight bytes of every sixteen that the product
-//              reads; their scales go into the 32 x 16-byte blocks that tcgen05.cp spreads over
-//              TMEM. (The copy engine can spread codes too, at about the same rate.)
+//   spreaders  (four-bit) one or two groups of four warps, stage about. Codes arrive packed in a
+//              ring of their own, 16 KB a stage, the bytes in flight, and are spread to the eight
+//              bytes of every sixteen that the product reads; their scales go into the 32 x 16-byte
+//              blocks that tcgen05.cp spreads over TMEM. (The copy engine can spread codes too, at
+//              about the same rate.)
 //   splitters  tokens from their rows, gathered and split into pieces, or copied where they lie
 //              prepared. A stage's chain of conversions takes 0.5 to 1 us whatever its size, so
 //              groups of warps each take stages of their own: that chain, done by all warps
@@ -163,8 +164,9 @@ struct WideItem {
 //   types      T; kMx; kPieces; kTok (tokens of an item, a multiple of 16); kLoad (tokens by the
 //              splitters; else rows `first * kPieces` on of a tensor map, or with kGather rows
 //              place(it, n) * kPieces on of `pieces`, `pitch` bytes apart, and for four-bit
-//              weights scales `sb`, `pitch_b` apart); kAccs; kStages and kTokenStages (of the rings); kRaw (stages of packed
-//              codes); kSpreadGroups; kSplitters (warps) in groups of kGroupWarps; kPerSm
+//              weights scales `sb`, `pitch_b` apart); kAccs; kStages and kTokenStages (of the
+//              rings); kRaw (stages of packed codes); kSpreadGroups; kSplitters (warps) in groups
+//              of kGroupWarps; kPerSm
 //   item(i, it) -> false past the last one;  token(it, n): row of token n (kLoad)
 //   halves: 1 or 2 of 64 rows;  scales of W: sa[2], blocks, rows_a;  x_aligned, cols
 //   begin(it) / value(it, n, row, v) / end(it): epilogue threads, by their row
@@ -182,7 +184,8 @@ struct Wide {
     static constexpr int kColumns = kUsed <= 32 ? 32 : kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
     static constexpr int kValues = kMx ? 128 : 64;   // of a row in a stage
     static constexpr int kRawStage = kMx ? kWideM * 128 : 0, kRaw = kMx ? W::kRaw : 0;
-    static constexpr int kSpreadGroups = kMx ? W::kSpreadGroups : 0, kSpreaders = 4 * kSpreadGroups, kSplitters = W::kSplitters, kGroupWarps = W::kGroupWarps;
+    static constexpr int kSpreadGroups = kMx ? W::kSpreadGroups : 0, kSpreaders = 4 * kSpreadGroups;
+    static constexpr int kSplitters = W::kSplitters, kGroupWarps = W::kGroupWarps;
     static constexpr int kGroups = kSplitters / kGroupWarps;
     static constexpr int kWarps = kWideEpilogue + kSpreaders + kSplitters + 2, kThreads = kWarps * 32;
     static_assert(kUsed <= 512 && kColumns * W::kPerSm <= 512, "TMEM columns");
@@ -380,12 +383,14 @@ struct Wide {
         const uint32_t quadrant = sh.tmem + (uint32_t(warp * 32) << 16);
         Ring<W::kAccs> acc;
         WideItem it;
+        bool ok = true;
         for (int i = 0; work.item(i, it); ++i) {
-            if (!mbar_wait_warp(smem_u32(sh.acc_full + acc.s), acc.ph)) return false;
+            // a warp that gives up still comes to the others' barriers
+            ok = ok && mbar_wait_warp(smem_u32(sh.acc_full + acc.s), acc.ph);
             fence_after();
             work.begin(it);
 #pragma unroll 1
-            for (int c = 0; c < it.count; c += 16) {  // 16 tokens, kPieces columns each
+            for (int c = 0; c < it.count && ok; c += 16) {  // 16 tokens, kPieces columns each
                 float v[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) v[j] = 0.f;
@@ -403,11 +408,11 @@ struct Wide {
                     if (c + j < it.count) work.value(it, c + j, warp * 32 + lane, v[j]);
             }
             fence_before();
-            mbar_arrive(smem_u32(sh.acc_empty + acc.s));
+            if (ok) mbar_arrive(smem_u32(sh.acc_empty + acc.s));
             work.end(it);
             acc.next();
         }
-        return true;
+        return ok;
     }
 
     // Spreaders: codes and scales of W. Scale words are loaded four of the group's stages ahead, since

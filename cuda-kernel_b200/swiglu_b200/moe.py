@@ -1,11 +1,12 @@
-"""The SwiGLU layer as a mixture of experts, for up to 64 tokens, in one kernel (swb_moe).
+"""The SwiGLU layer as a mixture of experts, for up to 64 tokens (swb_moe).
 
     logits = router x,  experts = the topk largest,  w = softmax
     y_t = sum_j w_tj down_e (SiLU(gate_e x_t) * (up_e x_t))
 
 Ties go to the lowest index and a NaN logit counts as the largest. ``renormalize``: the
 softmax runs over the selected logits, so that a token's weights sum to one; else over all
-logits. Like ``swiglu_out`` the call adds no bias and no residual, writes buffers the caller
+logits. In fp16 the product of the activations must lie within that type's range, or y is not
+finite. Like ``swiglu_out`` the call adds no bias and no residual, writes buffers the caller
 owns, launches on the current CUDA stream and allocates nothing.
 """
 from __future__ import annotations

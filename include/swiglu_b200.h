@@ -309,7 +309,13 @@ SWB_API int swb_mx4_dequantize(int type, const void* codes, const void* scales, 
  * W [rows, cols]; x [tokens, cols] of `type` (SWB_F16 or SWB_BF16), x_pitch elements from
  * token to token; bias [rows] or NULL and residual [tokens, rows] (read with SWB_RESIDUAL)
  * of `type`; out [tokens, rows] fp32, or `type` with SWB_HALF_OUT (then residual may be
- * out itself). Sums in fp32 over the exact values of W. tokens == 0: nothing to do. */
+ * out itself). Sums in fp32. Up to 16 tokens, or where x's rows do not lie on 16 bytes, W's
+ * values are exact and a token's are held to 2^-27 (SWB_BF16: 2^-22) of the largest of their
+ * block of 32; else tokens are exact, and W's values too but, with SWB_F16, those 2^36 below
+ * their row's largest scale (off by at most 6 2^-38 of it) and, with SWB_BF16, those of scales 253 and 254
+ * beyond bf16's range (infinite; swb_mx4_quantize writes no scale above 252). A token that
+ * holds a NaN or an infinity gives NaN or infinity, and leaves the others as they are.
+ * tokens == 0: nothing to do. */
 SWB_API int swb_mx4_project(int type, const void* codes, const void* scales, const void* x, int64_t x_pitch,
                             const void* bias, const void* residual, void* out, int64_t tokens, int64_t rows,
                             int64_t cols, unsigned flags, void* stream);
@@ -335,9 +341,13 @@ SWB_API int swb_mx4_matmul(int type, const void* x_codes, const void* x_scales, 
  * of gate, up [experts, inter, hidden] and down [experts, hidden, inter]; with SWB_MOE_MX4
  * these three are four-bit codes (16-byte aligned) and *_scales their scales, else
  * *_scales are ignored. The router's sums are held in 64 bits, the others in fp32; the
- * product of the activations is rounded to `type` once. ids [tokens, topk] int32 and
+ * product of the activations goes on as two values of `type` (rounded, and what the rounding
+ * left) or, with SWB_MOE_MX4 and more than eight tokens, as three 8-bit values; with SWB_F16 it
+ * must lie within fp16's range, or y is not finite. A token that holds a NaN or an infinity
+ * makes its y NaN or infinite, and leaves the others as they are. ids [tokens, topk] int32 and
  * weights [tokens, topk] fp32 receive the selection; either may be NULL.
- * One cooperative kernel. workspace: swb_moe_workspace_bytes of 256-byte aligned device
+ * One cooperative kernel, for more than eight tokens a second one after it, which fill the GPU.
+ * workspace: swb_moe_workspace_bytes of 256-byte aligned device
  * memory, zeroed once when allocated, then reused by every call on one stream (calls that
  * may overlap on the GPU need a workspace each). After a device error (swb_device_error)
  * zero it again. swb_moe_workspace_bytes is 0 for sizes beyond the limits. */

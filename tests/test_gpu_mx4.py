@@ -11,8 +11,8 @@ warps, bias and residual add at most 76 roundings more. Where a token is split i
 value within 13 binades of its block's largest is exact, and another is off by at most half the
 last piece's smallest step: 2^-10 of the piece's unit, which is 2^10 (three pieces, fp16) or
 2^5 (two, bf16) below the first's, where the largest is at least 2^7: 2^-27 or 2^-22 of it. Where
-fp16 weights are decoded against their row's largest scale, a value is exact or off by at most 2^-40
-of the row's largest, far below the first term for these inputs.
+fp16 weights are decoded against their row's largest scale, values are exact within 2^36 of it, as
+they are for these inputs but where a test says otherwise.
 So |out - exact| <= (1.125 K + 76) 2^-24 sum|w x| + d sum over blocks of max|x| sum|w| (+ |bias| +
 |residual| in the first sum) + half a step of the output type (eps/2 relative, or half of the
 smallest subnormal).
@@ -219,6 +219,57 @@ def test_project_far_binades():
         for out in (torch.float32, torch.bfloat16):
             check_product(S.mx4_project(x, codes, scales, dtype=out if out == torch.float32 or dtype == out else None), x, w,
                           None, None, torch.float32 if out == torch.float32 else dtype)
+
+
+@pytest.mark.parametrize("tokens", [17, 40, 70, 150])
+def test_project_misaligned_tokens(tokens):
+    """More tokens in rows that do not start on 16 bytes, and rows of ragged length."""
+    for dtype in (torch.float16, torch.bfloat16):
+        codes, scales, w = packed((140, 256), 5, 0.1)
+        wide = sample((tokens, 300), dtype, 6)
+        buf = torch.full((tokens + 2, 140), 9.0, dtype=torch.float32, device="cuda")
+        S.mx4_project_out(wide[:, 3:259], codes, scales, buf[1:-1])
+        check_product(buf[1:-1], wide[:, 3:259], w, None, None, torch.float32)
+        assert (buf[0] == 9).all() and (buf[-1] == 9).all()
+        codes, scales, w = packed((33, 101), 5, 0.1)
+        x = sample((tokens, 101), dtype, 7)
+        check_product(S.mx4_project(x, codes, scales), x, w, None, None, dtype)
+
+
+@pytest.mark.parametrize("rows", [48, 192 * 120])
+def test_project_special_values_more_tokens(rows):
+    """Extreme scales and non-finite tokens where W is decoded into 16-bit tiles.
+
+    fp16: a value below 2^-36 of its row's largest scale s is off by at most 6 2^-38 s, so the
+    product by at most that times sum|x|. bf16 holds every value of scales up to 252."""
+    cols, tokens = 128, 20
+    codes = torch.randint(0, 256, (rows, cols // 2), dtype=torch.uint8, generator=torch.Generator().manual_seed(1))
+    scales = torch.full((rows, 4), 127, dtype=torch.uint8)
+    scales[0] = 0
+    scales[1, 2] = 255
+    scales[2] = 200
+    scales[3, 1] = 0
+    scales[4] = torch.tensor([127, 91, 90, 85])
+    scales[5] = torch.tensor([252, 127, 0, 240])
+    scales[6] = 255
+    w = R.values(codes.numpy(), scales.numpy(), cols)
+    keep = [i for i in range(min(rows, 300)) if i not in (1, 6)]
+    largest = np.where(scales.numpy() == 255, 0, scales.numpy()).max(1)[keep].astype(np.int64) - 127
+    for dtype in (torch.float16, torch.bfloat16):
+        x = sample((tokens, cols), dtype, 2, 2.0 ** -6)
+        got = np64(S.mx4_project(x, codes.cuda(), scales.cuda(), dtype=torch.float32))
+        assert np.isnan(got[:, [1, 6]]).all()
+        want = np64(x) @ w[keep].T
+        bound = project_bound(np64(x), w[keep], 0, dtype) + cols * 2.0 ** -149
+        if dtype == torch.float16:
+            bound = bound + 6 * 2.0 ** -38 * np.exp2(largest)[None] * np.abs(np64(x)).sum(1)[:, None]
+        assert (np.abs(got[:, keep] - want) <= bound + half_step(np.abs(want) + bound, torch.float32)).all()
+        clean = S.mx4_project(x, codes.cuda(), scales.cuda(), dtype=torch.float32)
+        x[2, 5], x[3, 7] = float("inf"), float("nan")
+        bad = S.mx4_project(x, codes.cuda(), scales.cuda(), dtype=torch.float32)
+        rest = [i for i in range(tokens) if i not in (2, 3)]
+        assert torch.equal(bad[rest].nan_to_num(), clean[rest].nan_to_num())
+        assert torch.isnan(bad[3]).all() and not torch.isfinite(bad[2]).any()
 
 
 def test_project_refusals():
