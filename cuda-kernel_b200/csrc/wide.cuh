@@ -1,12 +1,13 @@
 // Products of a weight matrix with tokens on the fifth-generation tensor cores, for weights
-// that are streamed once: 128 rows of W are the M side, the tokens the N side, so that the
-// weights go from global memory to the tensor core without passing a register.
+// that are streamed once: 128 rows of W are the M side, the tokens the N side, so that
+// 16-bit weights go from global memory to the tensor core without passing a register.
 //
 // 16-bit weights: tcgen05.mma kind::f16. Four-bit weights: kind::mxf8f6f4, whose operands may
-// differ in type: the codes and their power-of-two scales are the M side as they are; a token is the sum of `pieces` e4m3 values, each block of 32 with
-// a scale of its own, five binades apart, rounded from what the piece before left. Three pieces
-// hold 15 bits below a block's largest value (all of an fp16 value within 13 binades of it, and
-// 2^-27 of the largest beyond), two hold 9 (bf16). A piece is a column of its own; the epilogue
+// differ in type: the codes and their power-of-two scales are the M side as they are; a token is
+// the sum of `pieces` e4m3 values, each block of 32 with a scale of its own, five binades apart,
+// rounded from what the piece before left. Three pieces hold an fp16 value exactly within 13
+// binades of its block's largest, and to 2^-27 of the largest below; two hold a bf16 value to
+// 2^-22 of it. A piece is a column of its own; the epilogue
 // adds a token's columns. Every product is exact and the sums are the tensor core's fp32.
 //
 // Roles of a CTA, through two rings of stages of 128 bytes of every row (one for the weights, one
