@@ -42,7 +42,6 @@ namespace {
 
 constexpr int kDeepM = 128, kDeepEpilogue = 8;  // rows; warps
 constexpr int kDeepTurn = 32, kDeepPitch = kDeepTurn + 2;  // columns of the epilogue's tiles
-constexpr int kDeepScales = 3;  // tiles whose row factors are kept: decoders run at most two ahead of the epilogue
 
 template <int N>
 struct DeepShape {
@@ -51,11 +50,15 @@ struct DeepShape {
     static constexpr int kThreads = (kDeepEpilogue + kDecoders + 2) * 32;
     static constexpr int kStagesA = N == 192 ? 4 : 5, kStagesB = N == 192 ? 3 : 8, kRaw = N == 192 ? 2 : 4;
     static_assert(kGroups <= kStagesB, "groups do not overtake the ring");
+    // Tiles whose row factors are kept. Decoders that begin tile t have filled the ring with stages before
+    // it, of which the products have finished all but the last kStagesB, tile t - 1 - kStagesB at least
+    // (one stage a tile); those began when the epilogue had read two tiles before.
+    static constexpr int kFactors = kStagesB + 3;
     static constexpr int kStageA = kDeepM * 128, kStageB = N * 128, kRawStage = N * 128;
     static constexpr uint32_t kAtB = kStagesA * kStageA, kAtRaw = kAtB + kStagesB * kStageB;
     static constexpr uint32_t kAtTurn = kAtRaw + kRaw * kRawStage;
     static constexpr uint32_t kAtFactors = kAtTurn + kDeepEpilogue * 32 * kDeepPitch * 4;
-    static constexpr size_t kSmem = kAtFactors + (kDeepScales + 1) * N * 4 + 1024;  // factors, and the current tile's largest scales
+    static constexpr size_t kSmem = kAtFactors + (kFactors + 1) * N * 4 + 1024;  // factors, and the current tile's largest scales
     static constexpr int kColumns = N == 192 ? 512 : 128;  // two accumulators
     static_assert(kSmem + 1024 <= kSmemPerCtaMax && 2 * N <= kColumns, "fits");
 };
@@ -196,7 +199,7 @@ __global__ void __launch_bounds__(DeepShape<N>::kThreads, 1)
         constexpr int kTasks = N * 2 / kGroupThreads;  // blocks of a stage's 64 values that a thread decodes
         const int thread = threadIdx.x - kDeepEpilogue * 32, group = thread / kGroupThreads, t = thread % kGroupThreads;
         const int raws = (stages + 3) / 4;
-        uint32_t* tops = reinterpret_cast<uint32_t*>(factors) + kDeepScales * N;
+        uint32_t* tops = reinterpret_cast<uint32_t*>(factors) + S::kFactors * N;
         int slot = 0, tiles = 0;
         bool ok = true;
         for (int64_t tile = blockIdx.x; tile < P.items; tile += gridDim.x, ++tiles) {
@@ -272,7 +275,7 @@ __global__ void __launch_bounds__(DeepShape<N>::kThreads, 1)
                     for (int n = k == stages - 1 ? 4 - k % 4 : 1; n > 0; --n) mbar_arrive(smem_u32(raw_empty + r));
                 }
             }
-            if (++slot == kDeepScales) slot = 0;
+            if (++slot == S::kFactors) slot = 0;
         }
     } else {
         // ---------------------------------------------------- epilogue
@@ -343,7 +346,7 @@ __global__ void __launch_bounds__(DeepShape<N>::kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(acc_empty + acc));
             if (++acc == 2) acc = 0, pacc ^= 1u;
-            if (++slot == kDeepScales) slot = 0;
+            if (++slot == S::kFactors) slot = 0;
         }
     }
     __syncwarp();

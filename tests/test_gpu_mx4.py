@@ -272,6 +272,23 @@ def test_project_special_values_more_tokens(rows):
         assert torch.isnan(bad[3]).all() and not torch.isfinite(bad[2]).any()
 
 
+@pytest.mark.parametrize("cols", [32, 64, 100, 128, 192, 200])
+def test_project_short_rows_many_tiles(cols):
+    """Many tiles of few stages, rows of very different scales: decoding runs far ahead of the epilogue."""
+    rows, tokens = 192 * 60, 2000
+    rng = np.random.RandomState(cols)
+    codes = rng.randint(0, 256, (rows, -(-cols // 32) * 16)).astype(np.uint8)
+    if cols % 32:
+        codes[:, cols // 2:] = 0
+    scales = np.repeat(rng.randint(97, 157, (rows, 1)), -(-cols // 32), axis=1).astype(np.uint8)
+    w = R.values(codes, scales, cols)
+    for dtype in (torch.float16, torch.bfloat16):
+        x = sample((tokens, cols), dtype, 1)
+        for _ in range(3):
+            got = S.mx4_project(x, torch.from_numpy(codes).cuda(), torch.from_numpy(scales).cuda(), dtype=torch.float32)
+            check_product(got, x, w, None, None, torch.float32)
+
+
 def test_project_refusals():
     codes, scales, _ = packed((8, 64), 1)
     x = sample((2, 64), torch.float16, 1)
