@@ -22,6 +22,11 @@ int fail(int status, const char* detail = nullptr);
 int check_launch();
 // SMs of the current device, -1 on a CUDA error.
 int sm_count();
+// Whether every address is a multiple of `bytes` (null is).
+template <typename... P>
+bool aligned(size_t bytes, P... p) {
+    return ((reinterpret_cast<uintptr_t>(p) | ... | uintptr_t(0)) & (bytes - 1)) == 0;
+}
 bool overlaps(const void* a, size_t abytes, const void* b, size_t bbytes);
 
 // Device error words of the other translation units (each holds its own).

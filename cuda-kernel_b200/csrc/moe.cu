@@ -95,10 +95,10 @@ int swb_moe(int type, unsigned flags, const void* x, int64_t x_pitch, const void
     if (!y) return fail(SWB_E_HALF_OUTPUT);
     const MoeWorkspace w = moe_workspace(tokens, experts, topk, inter);
     if (!workspace || workspace_bytes < w.total) return fail(SWB_E_WORKSPACE, "swb_moe workspace too small");
-    if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(SWB_E_ALIGNMENT, "workspace must be 256-byte aligned");
-    const uintptr_t bases[3] = {reinterpret_cast<uintptr_t>(gate), reinterpret_cast<uintptr_t>(up),
-                                reinterpret_cast<uintptr_t>(down)};
-    if (mx && ((bases[0] | bases[1] | bases[2]) % 16)) return fail(SWB_E_ALIGNMENT, "codes must be 16-byte aligned");
+    if (!aligned(256, workspace)) return fail(SWB_E_ALIGNMENT, "workspace must be 256-byte aligned");
+    if (!aligned(mx ? 16 : 2, gate, up, down))
+        return fail(SWB_E_ALIGNMENT, mx ? "codes must be 16-byte aligned" : "values off their type's size");
+    if (!aligned(2, x, router, y) || !aligned(4, ids, weights)) return fail(SWB_E_ALIGNMENT, "values off their type's size");
     // what the call writes may not overlap what it reads, nor each other
     const size_t n = size_t(experts) * hidden * inter;
     const size_t gate_blocks = size_t(experts) * inter * mx_blocks(hidden);

@@ -235,6 +235,7 @@ int convert(int type, const void* from, void* to, int64_t pitch, const void* cod
     if (rows == 0 || cols == 0) return SWB_OK;
     const void* side = BACK ? to : from;
     if (!side || !codes || !scales) return fail(SWB_E_INPUT);
+    if (!aligned(elem_size(type), side)) return fail(SWB_E_ALIGNMENT, "values off their type's size");
     RowMap m;
     m.rows = rows;
     m.cols = cols;
@@ -286,7 +287,9 @@ int swb_mx4_project(int type, const void* codes, const void* scales, const void*
     const bool half = (flags & SWB_HALF_OUT) != 0;
     if (!out) return fail(half ? SWB_E_HALF_OUTPUT : SWB_E_FLOAT_OUTPUT);
     if ((flags & SWB_RESIDUAL) && !residual) return fail(SWB_E_RESIDUAL);
-    if (reinterpret_cast<uintptr_t>(codes) % 16) return fail(SWB_E_ALIGNMENT, "codes must be 16-byte aligned");
+    if (!aligned(16, codes)) return fail(SWB_E_ALIGNMENT, "codes must be 16-byte aligned");
+    if (!aligned(2, x, bias, (flags & SWB_RESIDUAL) ? residual : nullptr) || !aligned(half ? 2 : 4, out))
+        return fail(SWB_E_ALIGNMENT, "values off their type's size");
     const size_t out_bytes = size_t(tokens) * rows * (half ? 2 : 4);
     const size_t blocks = size_t(rows) * mx_blocks(cols);
     if (overlaps(out, out_bytes, codes, blocks * kMxBlockBytes) || overlaps(out, out_bytes, scales, blocks) ||

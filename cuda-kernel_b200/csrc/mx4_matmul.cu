@@ -492,8 +492,9 @@ extern "C" int swb_mx4_matmul(int type, const void* x_codes, const void* x_scale
     if (!x_codes || !x_scales || !w_codes || !w_scales) return fail(SWB_E_INPUT);
     if (!out) return fail(SWB_E_HALF_OUTPUT);
     if ((flags & SWB_RESIDUAL) && !residual) return fail(SWB_E_RESIDUAL);
-    if ((reinterpret_cast<uintptr_t>(x_codes) | reinterpret_cast<uintptr_t>(w_codes)) % 16)
-        return fail(SWB_E_ALIGNMENT, "codes must be 16-byte aligned");
+    if (!aligned(16, x_codes, w_codes)) return fail(SWB_E_ALIGNMENT, "codes must be 16-byte aligned");
+    if (!aligned(2, out, bias, (flags & SWB_RESIDUAL) ? residual : nullptr))
+        return fail(SWB_E_ALIGNMENT, "values off their type's size");
     const int64_t blocks = mx_blocks(cols);
     const size_t out_bytes = size_t(tokens) * rows * 2;
     if (overlaps(out, out_bytes, x_codes, size_t(tokens) * blocks * kMxBlockBytes) ||

@@ -285,7 +285,8 @@ SWB_API int swb_residual_epilogue(float* y, const void* bias, const void* x, int
  * [rows, ceil(cols/32)] bytes, both contiguous: each block of 32 values along a row is
  * 16 bytes of e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives; value 2i in the
  * low half of byte i) times 2^(scale - 127); scale 255 makes the block NaN. A ragged last
- * block is filled up with zero codes. */
+ * block is filled up with zero codes. Values lie on multiples of their type's size
+ * (SWB_E_ALIGNMENT else). */
 #define SWB_F16 0
 #define SWB_BF16 1
 #define SWB_F32 2

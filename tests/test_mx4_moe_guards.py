@@ -132,6 +132,26 @@ def test_moe_guards():
     assert call(ids=ids, wt=ids + 8) == _lib.SWB_E_OVERLAP_OUTPUT and call(y=ws + 64) == _lib.SWB_E_OVERLAP_OUTPUT
 
 
+def test_values_off_their_size_are_refused():
+    """Addresses that no value of the type can have, which a kernel could not read."""
+    P, E = _lib.SWB_RESIDUAL, _lib.SWB_E_ALIGNMENT
+    x, c, s, o, b, r = (F + k * (1 << 30) for k in range(6))
+    for kind, off in ((0, 1), (1, 1), (2, 2)):
+        assert L().swb_mx4_quantize(kind, x + off, 64, c, s, 2, 64, None) == E
+        assert L().swb_mx4_dequantize(kind, c, s, o + off, 64, 2, 64, None) == E
+    for a in ((x + 1, b, r, o), (x, b + 1, r, o), (x, b, r + 1, o), (x, b, r, o + 2)):
+        assert L().swb_mx4_project(0, c, s, a[0], 64, a[1], a[2], a[3], 2, 32, 64, P, None) == E
+    assert L().swb_mx4_project(0, c, s, x, 64, b, r, o + 1, 2, 32, 64, P | _lib.SWB_HALF_OUT, None) == E
+    for a in ((b + 1, r, o), (b, r + 1, o), (b, r, o + 1)):
+        assert L().swb_mx4_matmul(0, x, x + (1 << 29), c, s, *a, 2, 32, 64, P, None) == E
+    q = [F + k * (1 << 30) for k in range(8)]
+    for i in range(8):  # x, router, gate, up, down, y, ids, weights
+        v = list(q)
+        v[i] += 2 if i > 5 else 1
+        assert L().swb_moe(0, 0, v[0], 64, *v[1:5], None, None, None, *v[5:8], 2, 64, 96, 4, 2, F + (1 << 35), 1 << 20,
+                           None) == E, i
+
+
 def test_moe_workspace_sizes():
     w = L().swb_moe_workspace_bytes
     assert w(0, 8, 2, 64) > 0 and w(64, 256, 16, 100000) > 64 * 16 * 100000 * 2
