@@ -204,12 +204,15 @@ __global__ void __launch_bounds__(DeepShape<N>::kThreads, 1)
         bool ok = true;
         for (int64_t tile = blockIdx.x; tile < P.items; tile += gridDim.x, ++tiles) {
             const int64_t w0 = tile / tiles_x * N;
+            // The groups begin a tile together: a group that went on past stages of others could come to a
+            // raw stage two rounds ahead of what has landed, where the barrier's parity says that it has.
+            // (Within a tile the ring of decoded stages holds them close enough.)
+            named_barrier_sync(1, kAll);
             if (!ok) {  // a group that gave up still comes to the others' barriers
-                if constexpr (std::is_same<T, __half>::value) named_barrier_sync(1, kAll), named_barrier_sync(1, kAll);
+                if constexpr (std::is_same<T, __half>::value) named_barrier_sync(1, kAll);
                 continue;
             }
-            if constexpr (std::is_same<T, __half>::value) {  // the rows' largest scales
-                named_barrier_sync(1, kAll);                 // the last tile's are read
+            if constexpr (std::is_same<T, __half>::value) {  // the rows' largest scales; the last tile's are read
                 for (int q = thread; q < N; q += kAll) {
                     uint32_t m = 0u;
                     if (w0 + q < P.rows) {
