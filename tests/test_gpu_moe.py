@@ -115,6 +115,20 @@ def test_four_bit_experts_with_more_tokens_than_an_item():
     check(d, v, 1, False, call(d, 1, False))
 
 
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("tokens,experts,topk,hidden,inter", [
+    (64, 64, 8, 64, 2000), (64, 6, 6, 40, 3000), (9, 100, 1, 32, 1500), (50, 30, 5, 2500, 32), (7, 20, 3, 64, 2500),
+    (12, 24, 2, 3100, 8)])
+def test_many_short_items(four_bit, tokens, experts, topk, hidden, inter):
+    """Many items of a stage or two on each SM: every ring goes round item after item."""
+    for dtype in (torch.float16, torch.bfloat16):
+        d, v = layer(tokens, tokens, experts, hidden, inter, dtype, four_bit)
+        first = call(d, topk)
+        check(d, v, topk, True, first)
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(call(d, topk), first))
+
+
 @pytest.mark.parametrize("hidden", [8192, 8200])
 @pytest.mark.parametrize("tokens,experts", [(12, 3), (10, 12)])
 def test_long_four_bit_tokens(hidden, tokens, experts):

@@ -357,6 +357,33 @@ def test_matmul(kind, tokens, rows, cols):
     assert binding.device_error() == 0
 
 
+@pytest.mark.parametrize("cols", [32, 256, 300, 600])
+def test_matmul_short_rows_many_tiles(cols):
+    """Many tiles of one to three stages, rows of very different scales on both sides."""
+    rows, tokens = 192 * 60, 2000
+    rng = np.random.RandomState(cols)
+    n = -(-cols // 32)
+    sides = []
+    for count in (tokens, rows):
+        codes = rng.randint(0, 256, (count, n * 16)).astype(np.uint8)
+        codes[:, cols // 2:] = 0
+        scales = np.repeat(rng.randint(112, 142, (count, 1)), n, axis=1).astype(np.uint8)
+        sides.append((codes, scales, R.values(codes, scales, cols)))
+    (xc, xs, x), (wc, ws, w) = sides
+    dev = [torch.from_numpy(t).cuda() for t in (xc, xs, wc, ws)]
+    for _ in range(2):
+        check_matmul(S.mx4_matmul(*dev, dtype=torch.bfloat16), x, w, None, None, torch.bfloat16)
+
+
+@pytest.mark.parametrize("tokens", [1, 8, 16])
+def test_few_tokens_many_short_rows(tokens):
+    """Many CTAs of one stage each."""
+    codes, scales, w = packed((40000, 72), 3, 0.1)
+    for dtype in (torch.float16, torch.bfloat16):
+        x = sample((tokens, 72), dtype, 4)
+        check_product(S.mx4_project(x, codes, scales), x, w, None, None, dtype)
+
+
 @pytest.mark.parametrize("tokens", [5, 200])
 def test_matmul_special_scales(tokens):
     """NaN scales on either side reach exactly their rows and tokens; extreme scales multiply out;
