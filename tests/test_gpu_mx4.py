@@ -447,3 +447,29 @@ def test_matmul_refusals():
         with pytest.raises(RuntimeError):
             bad()
     assert S.mx4_matmul(xc[:0], xs[:0], codes, scales).shape == (0, 8)
+
+
+def test_offsets_beyond_32_bits():
+    """Codes of more than 4 GB and values of more than 8 billion: the last rows are right."""
+    rows, cols = 140000, 65536
+    g = torch.Generator(device="cuda").manual_seed(1)
+    codes = torch.randint(0, 256, (rows, cols // 2), dtype=torch.uint8, device="cuda", generator=g)
+    scales = torch.randint(120, 124, (rows, cols // 32), dtype=torch.uint8, device="cuda", generator=g)
+    tail = [0, rows - 3, rows - 2, rows - 1]
+    c, s = codes[tail].contiguous(), scales[tail].contiguous()
+    w = R.values(c.cpu().numpy(), s.cpu().numpy(), cols)
+    for tokens in (1, 17):
+        for dtype in (torch.float16, torch.bfloat16):
+            x = sample((tokens, cols), dtype, tokens, 2.0 ** -6)
+            got = S.mx4_project(x, codes, scales, dtype=torch.float32)[:, tail]
+            check_product(got, x, w, None, None, torch.float32)
+    for tokens in (3, 130):
+        xc, xs, x = packed((tokens, cols), tokens, 2.0 ** -6)
+        check_matmul(S.mx4_matmul(xc, xs, codes, scales, dtype=torch.bfloat16)[:, tail], x, w, None, None, torch.bfloat16)
+    values = S.mx4_dequantize(codes, scales, dtype=torch.bfloat16)
+    assert torch.equal(values[tail].cpu().double(), torch.from_numpy(w))
+    S.mx4_quantize_out(values, codes, scales)
+    again = S.mx4_quantize(values[tail].contiguous())
+    assert torch.equal(codes[tail], again[0]) and torch.equal(scales[tail], again[1])
+    del codes, scales, values
+    torch.cuda.empty_cache()
