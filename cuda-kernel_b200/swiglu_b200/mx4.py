@@ -73,6 +73,13 @@ def mx4_empty(*shape: int, device=None) -> tuple[torch.Tensor, torch.Tensor]:
             torch.empty((*shape[:-1], n), dtype=torch.uint8, device=device or "cuda"))
 
 
+def _values(x: torch.Tensor) -> tuple[int, int, int]:
+    """(rows, cols, pitch) of a tensor to round."""
+    _check(x.is_cuda and x.dtype in _TYPES and x.dim() >= 1, "x must be a CUDA FP16, BF16 or FP32 tensor")
+    _check(not x.requires_grad, "inference only: disable gradients")
+    return _rows(x, "x")
+
+
 def mx4_quantize_out(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
     """Rounds fp16, bf16 or fp32 ``x`` [..., cols] to ``codes`` and ``scales`` (swb_mx4_quantize).
 
@@ -80,19 +87,18 @@ def mx4_quantize_out(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor)
     nearest code, ties to the even one, larger ones to 6. A block that holds a NaN or an
     infinity becomes NaN as a whole. A matrix may have spaced rows (``x.stride(0) > cols``).
     """
-    _check(x.is_cuda and x.dtype in _TYPES and x.dim() >= 1, "x must be a CUDA FP16, BF16 or FP32 tensor")
-    _check(not x.requires_grad, "inference only: disable gradients")
-    rows, cols, pitch = _rows(x, "x")
+    rows, cols, pitch = _values(x)
     _check_packed(codes, scales, x.shape[:-1], cols, x.device)
     _call(x.device, _lib.lib().swb_mx4_quantize, _TYPES[x.dtype], x.data_ptr(), pitch, codes.data_ptr(),
           scales.data_ptr(), rows, cols)
 
 
 def mx4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """Allocating wrapper of ``mx4_quantize_out``: (codes, scales)."""
-    _check(x.is_cuda and x.dim() >= 1, "x must be a CUDA FP16, BF16 or FP32 tensor")
+    """Allocating form of ``mx4_quantize_out``: (codes, scales)."""
+    rows, cols, pitch = _values(x)
     codes, scales = mx4_empty(*x.shape, device=x.device)
-    mx4_quantize_out(x, codes, scales)
+    _call(x.device, _lib.lib().swb_mx4_quantize, _TYPES[x.dtype], x.data_ptr(), pitch, codes.data_ptr(),
+          scales.data_ptr(), rows, cols)
     return codes, scales
 
 
