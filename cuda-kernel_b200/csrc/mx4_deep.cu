@@ -267,8 +267,7 @@ __global__ void __launch_bounds__(DeepShape<N>::kThreads, 1)
                     deep_decode<T>(codes, now[u], top[u], w);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + swizzled(row16, block * 4 + i)), "r"(w[4 * i]),
-                                     "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3]) : "memory");
+                        sts128(to + swizzled(row16, block * 4 + i), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -302,7 +301,8 @@ __global__ void __launch_bounds__(DeepShape<N>::kThreads, 1)
                 tmem_load_wait();
 #pragma unroll
                 for (int j = 0; j < 32; j += 2)
-                    *reinterpret_cast<float2*>(turn + lane * kDeepPitch + j) = make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+                    *reinterpret_cast<float2*>(turn + lane * kDeepPitch + j) =
+                        make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
                 __syncwarp();
                 float2 bias = make_float2(0.f, 0.f), f = make_float2(1.f, 1.f);
                 if constexpr (std::is_same<T, __half>::value) {
@@ -381,15 +381,18 @@ int launch_deep(ProjectParams P, cudaStream_t stream) {
 
 template <typename T>
 int dispatch_deep(const ProjectParams& P, cudaStream_t stream) {
-    // 192 rows a tile where that still gives every SM one, else 64
-    const int64_t tiles = int64_t((P.rows + 191) / 192) * ((P.tokens + kDeepM - 1) / kDeepM);
-    if (tiles * 4 >= 3 * sm_count()) return launch_deep<T, 192>(P, stream);
+    // 64 rows a tile while every SM gets one at most, else 192: 44.7 us against 51.2 with 224 tiles of 64
+    // (64 tokens by 14336 x 4096), 21.8 against 24.6 with 264 (384 tokens by 5632 x 2048).
+    const int64_t tiles = int64_t((P.rows + 63) / 64) * ((P.tokens + kDeepM - 1) / kDeepM);
+    if (tiles > sm_count()) return launch_deep<T, 192>(P, stream);
     return launch_deep<T, 64>(P, stream);
 }
 
 }  // namespace
 
-bool project_deep_takes(const ProjectParams& P) { return P.tokens > 16 && P.x_aligned; }
+// Up to 32 tokens their pieces cost less than decoding W (14336 x 4096: 32 tokens 39.4 us against 44.6, 24
+// tokens 32.0 against 43.7), from 33 on more (64 tokens: 76.6 against 44.7).
+bool project_deep_takes(const ProjectParams& P) { return P.tokens > 32 && P.x_aligned; }
 
 int project_deep(int type, const ProjectParams& P, cudaStream_t stream) {
     return type == SWB_F16 ? dispatch_deep<__half>(P, stream) : dispatch_deep<__nv_bfloat16>(P, stream);

@@ -471,7 +471,9 @@ int dispatch_matmul(const Side& x, const Side& w, const MatmulParams& P, cudaStr
     if (P.tokens <= 16) return launch_matmul<T, 16, false>(x, w, P, stream);
     if (P.tokens <= 32) return launch_matmul<T, 32, false>(x, w, P, stream);
     if (P.tokens <= 64) return launch_matmul<T, 64, false>(x, w, P, stream);
-    if (P.tokens <= 128) return launch_matmul<T, 128, false>(x, w, P, stream);
+    // 65 to 128 tokens: a tile of tokens by 192 rows where that gives half the SMs one (14336 x 4096, 128
+    // tokens: 16.2 us against 20.1, 100 tokens: 15.7 against 18.2; 64 tokens: 15.1 against 14.2)
+    if (P.tokens <= 128 && (P.rows + 191) / 192 * 2 < sm_count()) return launch_matmul<T, 128, false>(x, w, P, stream);
     return launch_matmul<T, 192, true>(x, w, P, stream);
 }
 

@@ -449,8 +449,8 @@ struct Wide {
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const int n = (t / 32 + u * 4) * 8 + (lane & 7);
-                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to + swizzled(n, 2 * block)), "r"(c[u].x), "r"(c[u].y) : "memory");
-                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to + swizzled(n, 2 * block + 1)), "r"(c[u].z), "r"(c[u].w) : "memory");
+                    sts64(to + swizzled(n, 2 * block), c[u].x, c[u].y);
+                    sts64(to + swizzled(n, 2 * block + 1), c[u].z, c[u].w);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -514,8 +514,7 @@ struct Wide {
 #pragma unroll
                         for (int u = u0; u < u0 + kBatch && u < kTurns; ++u) {
                             const int n = n0 + u * kStride;
-                            if (n < it.count)
-                                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(b + swizzled(n, j)), "r"(x[u].x), "r"(x[u].y), "r"(x[u].z), "r"(x[u].w) : "memory");
+                            if (n < it.count) sts128(b + swizzled(n, j), x[u].x, x[u].y, x[u].z, x[u].w);
                         }
                     } else {
                         uint2 piece[kBatch][W::kPieces];
@@ -530,7 +529,7 @@ struct Wide {
 #pragma unroll
                             for (int p = 0; p < W::kPieces; ++p) {
                                 const int r = n * W::kPieces + p;
-                                asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(b + swizzled(r, j / 2) + (j & 1) * 8), "r"(piece[u][p].x), "r"(piece[u][p].y) : "memory");
+                                sts64(b + swizzled(r, j / 2) + (j & 1) * 8, piece[u][p].x, piece[u][p].y);
                                 if ((j & 3) == 0) sts8(sc + scale_place(r) + j / 4, scale[u] - 5u * p);
                             }
                         }
@@ -575,16 +574,21 @@ struct Wide {
                         tma_load_2d(b + r * kWideRowBytes, map_b, k * kValues, it.first * W::kPieces + r, bar);
                 }
                 if constexpr (kMx) {
+                    const uint32_t sc = base + kAtScalesB + s * kBlocksB * kScaleBlock;
                     uint32_t word[(kN + 31) / 32];
 #pragma unroll
                     for (int u = 0; u < (kN + 31) / 32; ++u) {
                         const int r = lane + 32 * u;
-                        const int64_t from = r >= rows ? -1 : (W::kGather ? int64_t(work.place(it, r / W::kPieces)) : int64_t(it.first + r / W::kPieces)) * W::kPieces + r % W::kPieces;
-                        word[u] = scale_word(from < 0 ? nullptr : work.sb + from * work.pitch_b, k, it.s1, work.pitch_b);
+                        const unsigned char* row = nullptr;
+                        if (r < rows) {
+                            const int n = r / W::kPieces, token = W::kGather ? work.place(it, n) : it.first + n;
+                            row = work.sb + (int64_t(token) * W::kPieces + r % W::kPieces) * work.pitch_b;
+                        }
+                        word[u] = scale_word(row, k, it.s1, work.pitch_b);
                     }
 #pragma unroll
                     for (int u = 0; u < (kN + 31) / 32; ++u)
-                        if (lane + 32 * u < rows) sts32(base + kAtScalesB + s * kBlocksB * kScaleBlock + scale_place(lane + 32 * u), word[u]);
+                        if (lane + 32 * u < rows) sts32(sc + scale_place(lane + 32 * u), word[u]);
                     if (W::kGather) asm volatile("cp.async.wait_all;" ::: "memory");
                     fence_proxy_async_smem();
                 }

@@ -310,7 +310,7 @@ SWB_API int swb_mx4_dequantize(int type, const void* codes, const void* scales, 
  * W [rows, cols]; x [tokens, cols] of `type` (SWB_F16 or SWB_BF16), x_pitch elements from
  * token to token; bias [rows] or NULL and residual [tokens, rows] (read with SWB_RESIDUAL)
  * of `type`; out [tokens, rows] fp32, or `type` with SWB_HALF_OUT (then residual may be
- * out itself). Sums in fp32. Up to 16 tokens, or where x's rows do not lie on 16 bytes, W's
+ * out itself). Sums in fp32. Up to 32 tokens, or where x's rows do not lie on 16 bytes, W's
  * values are exact and a token's are held to 2^-27 (SWB_BF16: 2^-22) of the largest of their
  * block of 32; else tokens are exact, and W's values too but, with SWB_F16, those 2^36 below
  * their row's largest scale (off by at most 6 2^-38 of it) and, with SWB_BF16, those of scales 253 and 254

@@ -237,12 +237,13 @@ def test_project_misaligned_tokens(tokens):
 
 
 @pytest.mark.parametrize("rows", [48, 192 * 120])
-def test_project_special_values_more_tokens(rows):
+@pytest.mark.parametrize("tokens", [20, 40])
+def test_project_special_values_more_tokens(rows, tokens):
     """Extreme scales and non-finite tokens where W is decoded into 16-bit tiles.
 
     fp16: a value below 2^-36 of its row's largest scale s is off by at most 6 2^-38 s, so the
     product by at most that times sum|x|. bf16 holds every value of scales up to 252."""
-    cols, tokens = 128, 20
+    cols = 128
     codes = torch.randint(0, 256, (rows, cols // 2), dtype=torch.uint8, generator=torch.Generator().manual_seed(1))
     scales = torch.full((rows, 4), 127, dtype=torch.uint8)
     scales[0] = 0
@@ -340,7 +341,7 @@ def check_matmul(got, x, w, bias, residual, dtype):
 @pytest.mark.parametrize("kind", ["fp16", "bf16"])
 @pytest.mark.parametrize("tokens,rows,cols", [
     (1, 1, 1), (1, 128, 256), (2, 33, 31), (7, 129, 130), (16, 256, 512), (17, 100, 1030), (40, 300, 160),
-    (64, 128, 2048), (65, 200, 96), (128, 130, 640), (129, 192, 256), (200, 385, 1030), (300, 1000, 544),
+    (64, 128, 2048), (65, 200, 96), (100, 15000, 288), (128, 14300, 70), (128, 130, 640), (129, 192, 256), (200, 385, 1030), (300, 1000, 544),
     (16, 96, 6000), (520, 40, 33)])
 def test_matmul(kind, tokens, rows, cols):
     dtype = TYPES[kind]
@@ -458,7 +459,7 @@ def test_offsets_beyond_32_bits():
     tail = [0, rows - 3, rows - 2, rows - 1]
     c, s = codes[tail].contiguous(), scales[tail].contiguous()
     w = R.values(c.cpu().numpy(), s.cpu().numpy(), cols)
-    for tokens in (1, 17):
+    for tokens in (1, 17, 40):
         for dtype in (torch.float16, torch.bfloat16):
             x = sample((tokens, cols), dtype, tokens, 2.0 ** -6)
             got = S.mx4_project(x, codes, scales, dtype=torch.float32)[:, tail]
