@@ -432,9 +432,9 @@ struct Wide {
             int k = first_of<kGroupsA>(group, q0, it.s0);
             uint32_t word[5];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) word[w] = scale_word(row, k + w * kGroupsA, it.s1, work.blocks);
+            for (int w = 0; w < 4; ++w) word[w] = scale_word<false>(row, k + w * kGroupsA, it.s1, work.blocks);
             for (; k < it.s1; k += kGroupsA) {
-                word[4] = scale_word(row, k + 4 * kGroupsA, it.s1, work.blocks);
+                word[4] = scale_word<false>(row, k + 4 * kGroupsA, it.s1, work.blocks);
                 const uint32_t q = q0 + uint32_t(k - it.s0), s = q % W::kStages;
                 const uint32_t raw = raw0 + uint32_t(k / 2 - it.s0 / 2), rs = raw % kRaw;
                 const bool ready = mbar_wait(smem_u32(sh.raw_full + rs), raw / kRaw & 1u) && slot_free<W::kStages>(sh.empty, q);
@@ -468,15 +468,20 @@ struct Wide {
         }
         return true;
     }
-    // The four scale bytes of stage k of a row, zero beyond it.
+    // The four scale bytes of stage k of a row, zero beyond it. The non-coherent load is for W's, which
+    // nothing writes while the kernel runs. A token's (WRITTEN) come from the workspace, where other
+    // CTAs of this launch, or the launch before while this one is already resident, put them.
+    template <bool WRITTEN>
     static __device__ __forceinline__ uint32_t scale_word(const unsigned char* row, int k, int end, int blocks) {
         if (!row || k >= end) return 0u;
-        if ((blocks & 3) == 0 && (reinterpret_cast<uintptr_t>(row) & 3) == 0)
-            return __ldg(reinterpret_cast<const uint32_t*>(row) + k);
+        if ((blocks & 3) == 0 && (reinterpret_cast<uintptr_t>(row) & 3) == 0) {
+            const uint32_t* p = reinterpret_cast<const uint32_t*>(row) + k;
+            return WRITTEN ? __ldcg(p) : __ldg(p);
+        }
         uint32_t w = 0u;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (k * 4 + e < blocks) w |= uint32_t(__ldg(row + k * 4 + e)) << (8 * e);
+            if (k * 4 + e < blocks) w |= uint32_t(WRITTEN ? __ldcg(row + k * 4 + e) : __ldg(row + k * 4 + e)) << (8 * e);
         return w;
     }
 
@@ -584,7 +589,7 @@ struct Wide {
                             const int n = r / W::kPieces, token = W::kGather ? work.place(it, n) : it.first + n;
                             row = work.sb + (int64_t(token) * W::kPieces + r % W::kPieces) * work.pitch_b;
                         }
-                        word[u] = scale_word(row, k, it.s1, work.pitch_b);
+                        word[u] = scale_word<true>(row, k, it.s1, work.pitch_b);
                     }
 #pragma unroll
                     for (int u = 0; u < (kN + 31) / 32; ++u)
