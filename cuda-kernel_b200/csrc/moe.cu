@@ -26,7 +26,7 @@ namespace {
 static_assert(SWB_MOE_MAX_TOKENS == kMoeMaxTokens && SWB_MOE_MAX_EXPERTS == kMoeMaxExperts &&
                   SWB_MOE_MAX_TOPK == kMoeMaxTopk,
               "the header's limits");
-static_assert(1 + (kMoeMaxTokens + kRouteTokens - 1) / kRouteTokens <= 64, "sync words fit before the logits");
+static_assert(1 + (kMoeMaxTokens + kRouteTokens - 1) / kRouteTokens <= kSyncTurn && kSyncTurn < 64, "sync words fit");
 
 template <typename T, bool MX, int NT>
 int launch_moe(MoeParams P, cudaStream_t stream) {
@@ -138,6 +138,7 @@ int swb_moe(int type, unsigned flags, const void* x, int64_t x_pitch, const void
     P.ids = ids;
     P.weights = weights;
     P.sync = reinterpret_cast<uint32_t*>(base);
+    P.tops = reinterpret_cast<uint32_t*>(base + w.tops);
     P.logits = reinterpret_cast<double*>(base + w.logits);
     P.picks = reinterpret_cast<int*>(base + w.picks);
     P.shares = reinterpret_cast<float*>(base + w.shares);

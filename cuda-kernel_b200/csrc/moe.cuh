@@ -14,11 +14,12 @@
 //           and sums in 64 bits, so that the selection does not depend on the order of
 //           a sum. The CTA that completes a group of four tokens selects their experts.
 //   gate    items (expert, 16 rows of Wg and Wu) spread over the CTAs; h goes to the
-//           workspace with an expert's tokens side by side, as two values of the layer's
-//           type (h rounded, and what the rounding left), so that y keeps h's fp32 bits.
+//           workspace in fp32 with an expert's tokens side by side, for fp16 layers also the largest
+//           magnitude of each row.
 //   down    a CTA owns 16 rows of y at a time and takes every expert's product for
 //           them in expert order, so y needs no atomics and repeats bit for bit. Its
-//           weights are on their way while the grid waits for h.
+//           weights are on their way while the grid waits for h. h is multiplied as two values of
+//           the layer's type (split_pairs): 2^-22 of it is lost with fp16, 2^-16 with bf16.
 //
 // An expert with more than 32 tokens is taken in groups of 32, each group of a tile right
 // after the other, so that the second finds the weights in L2.
@@ -39,6 +40,11 @@ constexpr int kMoeMaxExperts = 256;
 constexpr int kMoeMaxTopk = 16;
 constexpr int kMoeGroup = 32, kMoeFewGroup = 16;  // most tokens of an item; where experts get few (moe_wide.cu)
 constexpr int kMoeMaxGroups = kMoeMaxExperts + kMoeMaxTokens * kMoeMaxTopk / kMoeFewGroup;
+constexpr int kMoeMaxRows = kMoeMaxTokens * kMoeMaxTopk;  // of h
+// The largest magnitudes start a call at zero. moe_kernel may have no barrier before the first of
+// them, so its calls use two sets in turn (sync word kSyncTurn: which) and clear the other; the third
+// is moe_wide.cu's, cleared before its router's barrier.
+constexpr int kSyncTurn = 63, kTopsWide = 2;
 constexpr int kRouteExperts = 4, kRouteTokens = 4;  // of a router unit
 constexpr int kRouteWarps = 8, kRouteThreads = kRouteWarps * 32;  // that compute logits
 
@@ -54,11 +60,12 @@ struct MoeParams {
     void* y;
     int* ids;        // [tokens, topk] or null
     float* weights;  // [tokens, topk] or null
-    uint32_t* sync;  // [0] grid barrier, [1 + group] finished router units of a group of tokens
+    uint32_t* sync;  // [0] grid barrier, [1 + group] finished router units of a group of tokens, [kSyncTurn]
+    uint32_t* tops;  // [3][kMoeMaxRows]: the largest magnitude of each row of h (fp16 layers)
     double* logits;  // [tokens, experts]
     int* picks;      // [tokens, topk]
     float* shares;   // [tokens, topk]
-    void* h;         // [2][tokens * topk, h_pitch]: rounded, then what is left
+    void* h;         // [tokens * topk, h_pitch] fp32 (moe_wide.cu: or what its second kernel's copies bring)
     void* pieces;    // tokens split into e4m3 values (moe_wide.cu)
     int64_t x_pitch;
     int tokens, hidden, inter, experts, topk, h_pitch;
@@ -70,13 +77,14 @@ struct MoeParams {
 
 // Offsets of the workspace's parts.
 struct MoeWorkspace {
-    size_t logits, picks, shares, h, pieces, total;
+    size_t tops, logits, picks, shares, h, pieces, total;
 };
 constexpr int kMoePieceDim = 8192;  // values of a token whose pieces the workspace holds
 __host__ __device__ inline int moe_h_pitch(int inter) { return (inter + kTileRows - 1) / kTileRows * kTileRows; }
 __host__ __device__ inline MoeWorkspace moe_workspace(int tokens, int experts, int topk, int inter) {
     MoeWorkspace m;
-    m.logits = 256;  // the sync words before it
+    m.tops = 256;  // the sync words before it; these two stand where every size of call finds them
+    m.logits = m.tops + 3 * kMoeMaxRows * 4;
     m.picks = m.logits + size_t(tokens) * experts * 8;
     m.shares = m.picks + size_t(tokens) * topk * 4;
     m.h = (m.shares + size_t(tokens) * topk * 4 + 255) / 256 * 256;
@@ -90,7 +98,10 @@ __host__ __device__ inline MoeWorkspace moe_workspace(int tokens, int experts, i
 struct MoeRoute {
     unsigned long long taken[kMoeMaxExperts];          // an expert's tokens, a bit each
     float share[kMoeMaxTokens * kMoeMaxTopk];          // of each row of h: its expert's weight
-    float shares[kMoeMaxTokens * kMoeMaxTopk];         // [token, place]: the same
+    union {
+        float shares[kMoeMaxTokens * kMoeMaxTopk];     // [token, place]: the same, until the lists are made
+        float unit[kMoeMaxTokens * kMoeMaxTopk];       // of each row of h (row_unit), once h is complete
+    };
     int pick[kMoeMaxTokens * kMoeMaxTopk];             // [token, place]: the expert
     int groups;
     short row[kMoeMaxExperts];                         // an expert's first row of h
@@ -386,6 +397,12 @@ __global__ void __launch_bounds__(Stream<T, MX, NT>::kThreads, 1)
     const int G = gridDim.x, b = blockIdx.x;
     const auto l = Pipe::layout(smem_u32(smem), S::kStages);
     if (threadIdx.x == kThreads - 1) Pipe::init(l);
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    // read before this CTA comes to a barrier, after which CTA 0 turns it
+    const uint32_t turn = kHalf ? *reinterpret_cast<volatile uint32_t*>(P.sync + kSyncTurn) & 1u : 0u;
+    uint32_t* tops = P.tops + turn * kMoeMaxRows;
+    if (kHalf && b == G - 1)
+        for (int i = threadIdx.x; i < kMoeMaxRows; i += kThreads) P.tops[(turn ^ 1u) * kMoeMaxRows + i] = 0u;
 
     if (P.tokens * P.experts <= kRouteAlone) {
         if (warp < kRouteWarps) moe_router_alone<T>(P, scratch, R.pick, R.shares);
@@ -429,8 +446,7 @@ __global__ void __launch_bounds__(Stream<T, MX, NT>::kThreads, 1)
         t.rows[0] = min(kTileRows, P.hidden - tile * kTileRows);
         return t;
     };
-    T* h = static_cast<T*>(P.h);
-    const int64_t h_plane = int64_t(P.tokens) * P.topk * P.h_pitch;
+    float* h = static_cast<float*>(P.h);
     typename Pipe::Place place;
 
     if (warp == kConsumers) {
@@ -482,8 +498,9 @@ __global__ void __launch_bounds__(Stream<T, MX, NT>::kThreads, 1)
                 tokens.count = R.start[a + 1] - start;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    tokens.x[n] = h + int64_t(start + min(n * 8 + (lane >> 2), tokens.count - 1)) * P.h_pitch;
-                    tokens.x[NT + n] = tokens.x[n] + h_plane;
+                    const int row = start + min(n * 8 + (lane >> 2), tokens.count - 1);
+                    tokens.x[n] = h + int64_t(row) * P.h_pitch;
+                    if constexpr (kHalf) tokens.top[n] = __ldcg(tops + row);
                 }
             };
             turn_to(d0, 0);
@@ -505,24 +522,33 @@ __global__ void __launch_bounds__(Stream<T, MX, NT>::kThreads, 1)
             int group, row;
             gate_item(i, group, row);
             const int start = R.start[group], count = R.start[group + 1] - start;
-            for (int c = thread; c < count * kTileRows; c += kEpilogueThreads) {
+            for (int c = thread; c - lane < count * kTileRows; c += kEpilogueThreads) {  // whole warps
                 const int n = c >> 4, r = c & 15;
-                const float g = Pipe::template sum<2>(l, place, 0, n, r), u = Pipe::template sum<2>(l, place, 1, n, r);
-                // rows up to the pitch of h are zero, so that a whole piece of h may be read
-                const float v = row + r < P.inter ? silu(g) * u : 0.f;
-                const T hi = Num<T>::from_float(v);
-                const int64_t at = int64_t(start + n) * P.h_pitch + row + r;
-                h[at] = hi;
-                h[h_plane + at] = Num<T>::from_float(v - Num<T>::to_float(hi));
+                float v = 0.f;
+                if (c < count * kTileRows) {
+                    const float g = Pipe::template sum<2>(l, place, 0, n, r), u = Pipe::template sum<2>(l, place, 1, n, r);
+                    // rows up to the pitch of h are zero, so that a whole piece of h may be read
+                    if (row + r < P.inter) v = silu(g) * u;
+                    h[int64_t(start + n) * P.h_pitch + row + r] = v;
+                }
+                if constexpr (kHalf) {  // 16 lanes hold 16 places of a row
+                    uint32_t top = __float_as_uint(v) & 0x7FFFFFFFu;
+#pragma unroll
+                    for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                    if (r == 0 && c < count * kTileRows) atomicMax(tops + start + n, top);
+                }
             }
             Pipe::release(l, place);
         }
         named_barrier_sync(3, kEpilogueThreads);
         if (thread == 0) {
             flag = place.ok && moe_grid_arrive_wait(P.sync);
+            if (kHalf && b == 0 && flag) P.sync[kSyncTurn] = turn ^ 1u;
             __threadfence();
         }
         named_barrier_sync(2, kThreads - 32);
+        if constexpr (kHalf)  // before the barrier that precedes the first sums
+            for (int i = thread; i < P.tokens * P.topk; i += kEpilogueThreads) R.unit[i] = row_unit(__ldcg(tops + i));
         T* y = static_cast<T*>(P.y);
         for (int d = d0; d < d1 && flag; ++d) {
             for (int c = thread; c < P.tokens * kTileRows; c += kEpilogueThreads) total[c] = 0.f;
@@ -538,7 +564,9 @@ __global__ void __launch_bounds__(Stream<T, MX, NT>::kThreads, 1)
                 for (int c = thread; c < count * kTileRows; c += kEpilogueThreads) {
                     const int n = c >> 4, r = c & 15;  // a token takes an expert once: no two threads meet
                     float& sum = total[R.token[start + n] * kTileRows + r];
-                    sum = fmaf(R.share[start + n], Pipe::template sum<1>(l, place, 0, n, r), sum);
+                    float v = Pipe::template sum<1>(l, place, 0, n, r);
+                    if constexpr (kHalf) v *= R.unit[start + n];
+                    sum = fmaf(R.share[start + n], v, sum);
                 }
                 Pipe::release(l, place);
             }

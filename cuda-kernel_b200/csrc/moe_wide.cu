@@ -3,8 +3,11 @@
 //
 //   gate   router and selection as in moe.cuh, then items (expert's group of tokens, 64 rows of Wg
 //          and of Wu): gate rows in lanes 0 to 63 of the accumulator, up rows in 64 to 127. h goes
-//          to the workspace as the rows the second kernel's copies bring: two values of the layer's
-//          type (rounded, and what the rounding left), or three e4m3 pieces with block scales.
+//          to the workspace as the second kernel reads it: fp16 layers in fp32, with the largest
+//          magnitude of each row, from which that kernel splits it (split_pairs: within 2^-22); bf16
+//          as two values (rounded, and what the rounding left: within 2^-16) that its copies bring;
+//          four-bit experts' as three e4m3 pieces with block scales (within 2^-14 of the block's
+//          largest value).
 //   down   a cluster owns 128 rows of y; its CTAs take equal shares of the experts' steps along
 //          the intermediate dimension, keep y's sums in shared memory and add them in rank order.
 //
@@ -47,7 +50,7 @@ struct WideMaps {
 template <typename T_, bool MX, bool SPLIT, int TOK>
 struct GateWork {
     using T = T_;
-    static constexpr bool kMx = MX, kLoad = SPLIT || !MX, kGather = MX && !SPLIT;
+    static constexpr bool kMx = MX, kLoad = SPLIT || !MX, kFloat = false, kGather = MX && !SPLIT;
     static constexpr int kPieces = MX ? (std::is_same<T, __half>::value ? 3 : 2) : 1;
     static constexpr int kTok = TOK, kAccs = 2, kPerSm = 1;
     static constexpr int kStages = MX ? 3 : 8, kRaw = 4, kTokenStages = MX ? (TOK == 16 ? 10 : 5) : 6;
@@ -116,6 +119,10 @@ struct GateWork {
                     if (i < P->inter) h[(row * 3 + p) * P->h_pitch + i] = static_cast<unsigned char>(b);
                     if (lane == 0) s[(row * 3 + p) * mx_blocks(P->inter) + i / kMxBlock] = static_cast<unsigned char>(scale - 5u * p);
                 }
+            } else if constexpr (std::is_same<T, __half>::value) {
+                const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v) & 0x7FFFFFFFu);
+                if (lane == 0) atomicMax(P->tops + kTopsWide * kMoeMaxRows + row, top);
+                if (i < P->inter) reinterpret_cast<float*>(h)[row * P->h_pitch + i] = v;
             } else if (i < P->inter) {
                 T* to = reinterpret_cast<T*>(h) + row * 2 * P->h_pitch + i;
                 const T hi = Num<T>::from_float(v);
@@ -129,11 +136,12 @@ struct GateWork {
 template <typename T_, bool MX, int TOK>
 struct DownWork {
     using T = T_;
-    static constexpr bool kMx = MX, kLoad = false, kGather = false;
+    static constexpr bool kFloat = !MX && std::is_same<T, __half>::value;
+    static constexpr bool kMx = MX, kLoad = kFloat, kGather = false;
     static constexpr int kPieces = h_pieces(MX);
     static constexpr int kTok = TOK, kAccs = 2, kPerSm = 1;
     static constexpr int kStages = MX ? 3 : 7, kRaw = 4, kTokenStages = MX ? (TOK == 16 ? 8 : 4) : 6;
-    static constexpr int kSpreadGroups = 2, kSplitters = MX ? kTokenStages : 4, kGroupWarps = 1;
+    static constexpr int kSpreadGroups = 2, kSplitters = MX || kFloat ? kTokenStages : 4, kGroupWarps = 1;
 
     const unsigned char* sa[2];
     const unsigned char *sb, *pieces;
@@ -160,9 +168,14 @@ struct DownWork {
         return true;
     }
     __device__ __forceinline__ int place(const WideItem&, int) const { return 0; }
+    __device__ __forceinline__ const float* token(const WideItem& it, int n) const {
+        return static_cast<const float*>(P->h) + int64_t(it.first + n) * P->h_pitch;
+    }
+    __device__ __forceinline__ float up(const WideItem& it, int n) const { return unit_inverse(R->unit[it.first + n]); }
     __device__ __forceinline__ void begin(const WideItem&) const {}
     // a thread owns a row of y; items come in the order of their experts
     __device__ __forceinline__ void value(const WideItem& it, int n, int row, float v) const {
+        if constexpr (kFloat) v *= R->unit[it.first + n];
         const uint32_t at = total + (R->token[it.first + n] * kWideM + row) * 4;
         sts32(at, __float_as_uint(fmaf(R->share[it.first + n], v, __uint_as_float(lds32(at)))));
     }
@@ -222,6 +235,10 @@ __global__ void __launch_bounds__(Wide<GateWork<T, MX, SPLIT, TOK>>::kThreads, 1
     __shared__ int flag;
     MoeRoute& R = *reinterpret_cast<MoeRoute*>(smem + S::kRoute);
     S::Pipe::init(sh);
+    if constexpr (!MX && std::is_same<T, __half>::value) {  // before the router's barrier
+        if (blockIdx.x == 0)
+            for (int i = threadIdx.x; i < P.tokens * P.topk; i += kWideThreads) P.tops[kTopsWide * kMoeMaxRows + i] = 0u;
+    }
     if constexpr (Work::kGather) split_tokens<T, Work::kPieces>(P);
     if (threadIdx.x < kRouteThreads) moe_router<T>(P, scratch, &flag);
     const bool routed = moe_grid_barrier(P.sync, &flag);
@@ -279,6 +296,11 @@ __global__ void __launch_bounds__(Wide<DownWork<T, MX, TOK>>::kThreads, 1)
     }
     __syncthreads();
     moe_lists(P, R);
+    if constexpr (Work::kFloat) {
+        for (int i = threadIdx.x; i < P.tokens * P.topk; i += kWideThreads)
+            R.unit[i] = row_unit(__ldcg(P.tops + kTopsWide * kMoeMaxRows + i));
+        __syncthreads();
+    }
     const int rank = int(blockIdx.x % splits);
     Work work;
     work.sa[0] = work.sa[1] = P.s[2];
@@ -340,7 +362,9 @@ int launch_moe_wide(const MoeParams& P, cudaStream_t stream) {
     if (int rc = make_wide_map(&maps.gate, P.w[0], gate_rows, P.hidden, MX)) return rc;
     if (int rc = make_wide_map(&maps.up, P.w[1], gate_rows, P.hidden, MX)) return rc;
     if (int rc = make_wide_map(&map_w, P.w[2], int64_t(P.experts) * P.hidden, P.inter, MX)) return rc;
-    if (int rc = make_typed_map(&map_h, MX ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, P.h, P.inter,
+    if (DownWork<T, MX, TOK>::kFloat)
+        map_h = map_w;  // its kernel loads h itself
+    else if (int rc = make_typed_map(&map_h, MX ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, P.h, P.inter,
                                 rows, int64_t(P.h_pitch) * (MX ? 1 : 2), MX ? 128 : 64, 16))
         return rc;
     // every CTA resident at once: the cooperative launch makes the runtime check it

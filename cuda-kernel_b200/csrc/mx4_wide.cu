@@ -32,7 +32,7 @@ namespace {
 template <typename T_, int TOK>
 struct ProjectWork {
     using T = T_;
-    static constexpr bool kMx = true, kLoad = true, kGather = false;
+    static constexpr bool kMx = true, kLoad = true, kFloat = false, kGather = false;
     static constexpr int kPieces = std::is_same<T, __half>::value ? 3 : 2;
     static constexpr int kTok = TOK, kAccs = 1;
     static constexpr int kPerSm = TOK == 16 ? 2 : 1;

@@ -29,6 +29,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "device.cuh"
 #include "mx4.cuh"
 #include "tensor_map.h"
@@ -72,6 +74,42 @@ struct Num<__nv_bfloat16> {
                           __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
     }
 };
+
+// A row of fp32 values goes through the tensor cores as two values of T: the nearest, and what the
+// rounding left, rounded. With fp16 the row is first divided by a unit, a power of two that brings
+// its largest value to [2^14, 2^15), so that fp32's range is kept and only values 2^-28 below the
+// largest meet fp16's subnormals (errors within 2^-39 of it); the sums are multiplied by the unit.
+// bf16 has fp32's range. `top`: the bits of the largest magnitude; NaN and infinity stay what they are.
+__device__ __forceinline__ float row_unit(uint32_t top) {
+    const uint32_t e = top >> 23;
+    return __uint_as_float((e > 254u ? 127u : max(e, 15u) - 14u) << 23);
+}
+__device__ __forceinline__ float unit_inverse(float unit) { return __uint_as_float((254u << 23) - __float_as_uint(unit)); }
+// Eight fp32 values times `up` (fp16) -> both parts.
+template <typename T>
+__device__ __forceinline__ void split_pairs(const uint4& a, const uint4& b, float up, uint4& hi, uint4& lo) {
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float x = __uint_as_float(w[2 * i]), y = __uint_as_float(w[2 * i + 1]);
+        if constexpr (kHalf) x *= up, y *= up;  // exact
+        const auto one = [](float p, float q) {
+            uint32_t bits;
+            if constexpr (kHalf)
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(bits) : "f"(q), "f"(p));
+            else
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(bits) : "f"(q), "f"(p));
+            return bits;
+        };
+        h[i] = one(x, y);
+        const float2 back = kHalf ? half2_bits_to_float2(h[i]) : make_float2(__uint_as_float(h[i] << 16), __uint_as_float(h[i] & 0xFFFF0000u));
+        l[i] = one(x - back.x, y - back.y);
+    }
+    hi = make_uint4(h[0], h[1], h[2], h[3]);
+    lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
 
 // Shared loads by 32-bit address, left to the compiler to schedule between barriers.
 __device__ __forceinline__ const void* smem_ptr(uint32_t a) {
@@ -431,17 +469,19 @@ struct Stream {
     }
 
     // The tokens of an item as a consumer lane reads them: its row of each group of eight; with
-    // SPLIT, the rows of a second addend after the first NT, multiplied by the same weights. A warp
-    // takes every kConsumers-th unit of a stage and loads its tokens kGroup sub-steps of 32 values
-    // ahead, into the next item too: enough that they come from L2 in time.
+    // SPLIT, rows of fp32 values (zero up to a multiple of eight, `top`: row_unit), which are
+    // multiplied as two values of T. A warp takes every kConsumers-th unit of a stage and loads its
+    // tokens kGroup sub-steps of 32 values ahead, into the next item too: enough that they come from
+    // L2 in time.
     template <int NM, bool SPLIT>
     struct Tokens {
         static constexpr int kRows = SPLIT ? 2 * NT : NT;
         static constexpr int kSteps = Shape<NM>::kUnits / kConsumers * kSub;  // sub-steps of a warp in a full stage
         static constexpr int kMost = kConsumers == 16 ? 4 / kRows : 8 / kRows;  // that the registers hold
         static constexpr int kGroup = kMost < 1 ? 1 : kMost > 4 ? (kSteps < 4 ? kSteps : 4) : kMost < kSteps ? kMost : kSteps;
-        const T* x[kRows];  // this lane's rows
-        int count;          // tokens; 0: no item
+        const std::conditional_t<SPLIT, float, T>* x[NT];  // this lane's rows
+        uint32_t top[NT];
+        int count;  // tokens; 0: no item
         uint4 ahead[kGroup][kRows];
 
         // k of this lane's piece in sub-step s of chunk c
@@ -454,8 +494,17 @@ struct Stream {
 #pragma unroll
             for (int i = 0; i < kGroup; ++i)
 #pragma unroll
-                for (int n = 0; n < kRows; ++n)
-                    if (n % NT * 8 < count) ahead[i][n] = load_piece<T, FAST>(x[n], k_of(c, s + i), cols);
+                for (int n = 0; n < NT; ++n) {
+                    if (n * 8 >= count) break;
+                    const int k = k_of(c, s + i);
+                    if constexpr (SPLIT) {
+                        const uint4* p = reinterpret_cast<const uint4*>(x[n] + k);
+                        ahead[i][n] = k < cols ? p[0] : make_uint4(0u, 0u, 0u, 0u);
+                        ahead[i][NT + n] = k < cols ? p[1] : make_uint4(0u, 0u, 0u, 0u);
+                    } else {
+                        ahead[i][n] = load_piece<T, FAST>(x[n], k, cols);
+                    }
+                }
         }
     };
 
@@ -477,6 +526,11 @@ struct Stream {
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) acc[m][n][c] = 0.f;
+        float up[NT];
+        if constexpr (SPLIT && std::is_same<T, __half>::value) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) up[n] = unit_inverse(row_unit(tokens.top[n]));
+        }
         const int row = tile_row(g);  // and row + 8
         // how far these rows are shifted in their stage
         uint32_t shift[NM][2];
@@ -499,9 +553,18 @@ struct Stream {
             for (int s = 0; s < kSteps; s += kGroup) {
                 uint4 now[kGroup][NP];
 #pragma unroll
-                for (int i = 0; i < kGroup; ++i)
+                for (int i = 0; i < kGroup; ++i) {
+                    if constexpr (SPLIT) {
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) now[i][n] = MX ? Num<T>::order(tokens.ahead[i][n]) : tokens.ahead[i][n];
+                        for (int n = 0; n < NT; ++n)
+                            if (n * 8 < count) split_pairs<T>(tokens.ahead[i][n], tokens.ahead[i][NT + n], up[n], now[i][n], now[i][NT + n]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) {
+                        const uint4& v = SPLIT ? now[i][n] : tokens.ahead[i][n];
+                        now[i][n] = MX ? Num<T>::order(v) : v;
+                    }
+                }
                 if (s + kGroup < kSteps) {
                     tokens.template load<FAST>(c, s + kGroup, x_cols);
                 } else if (c + 1 < chunks) {

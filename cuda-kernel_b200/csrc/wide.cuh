@@ -163,7 +163,8 @@ struct WideItem {
 
 // W describes the work:
 //   types      T; kMx; kPieces; kTok (tokens of an item, a multiple of 16); kLoad (tokens by the
-//              splitters; else rows `first * kPieces` on of a tensor map, or with kGather rows
+//              splitters; kFloat: rows of fp32 on 16 bytes, `cols` a multiple of eight, times
+//              up(it, n), as two 16-bit pieces; else rows `first * kPieces` on of a tensor map, or with kGather rows
 //              place(it, n) * kPieces on of `pieces`, `pitch` bytes apart, and for four-bit
 //              weights scales `sb`, `pitch_b` apart); kAccs; kStages and kTokenStages (of the
 //              rings); kRaw (stages of packed codes); kSpreadGroups; kSplitters (warps) in groups
@@ -192,6 +193,7 @@ struct Wide {
     static_assert(kUsed <= 512 && kColumns * W::kPerSm <= 512, "TMEM columns");
     static_assert(W::kLoad || kGroupWarps == 1, "a warp brings prepared tokens");
     static_assert(!W::kGather || kMx, "gathered rows are pieces");
+    static_assert(!W::kFloat || (W::kLoad && !kMx && W::kPieces == 2), "fp32 rows are split in two");
     // a group that waits for a stage of tokens is at most one round of the ring ahead of its readers
     static_assert(kGroups <= W::kTokenStages, "groups do not overtake the ring");
 
@@ -494,16 +496,21 @@ struct Wide {
         const int t = threadIdx.x - (kWideEpilogue + kSpreaders + group * kGroupWarps) * 32, j = t % kPer, n0 = t / kPer;
         uint32_t q0 = 0;
         WideItem it;
-        uint4 x[kTurns];
+        uint4 x[kTurns], second[W::kFloat ? kTurns : 1];
         for (int i = 0; work.item(i, it); ++i) {
             auto load = [&](int k) {
                 if (k >= it.s1) return;
 #pragma unroll
                 for (int u = 0; u < kTurns; ++u) {
                     if (u * kStride >= it.count) break;
-                    const T* row = work.token(it, min(n0 + u * kStride, it.count - 1));
+                    const auto* row = work.token(it, min(n0 + u * kStride, it.count - 1));
                     const int at = k * kValues + j * 8;
-                    x[u] = work.x_aligned ? load_piece<T, true>(row, at, work.cols) : load_piece<T, false>(row, at, work.cols);
+                    if constexpr (W::kFloat) {
+                        const uint4* p = reinterpret_cast<const uint4*>(row + at);
+                        x[u] = at < work.cols ? __ldcg(p) : make_uint4(0u, 0u, 0u, 0u);
+                        second[u] = at < work.cols ? __ldcg(p + 1) : make_uint4(0u, 0u, 0u, 0u);
+                    } else
+                        x[u] = work.x_aligned ? load_piece<T, true>(row, at, work.cols) : load_piece<T, false>(row, at, work.cols);
                 }
             };
             int k = first_of<kGroups>(group, q0, it.s0);
@@ -519,7 +526,14 @@ struct Wide {
 #pragma unroll
                         for (int u = u0; u < u0 + kBatch && u < kTurns; ++u) {
                             const int n = n0 + u * kStride;
-                            if (n < it.count) sts128(b + swizzled(n, j), x[u].x, x[u].y, x[u].z, x[u].w);
+                            if constexpr (W::kFloat) {
+                                if (n >= it.count) continue;
+                                uint4 hi, lo;
+                                split_pairs<T>(x[u], second[u], work.up(it, n), hi, lo);
+                                sts128(b + swizzled(2 * n, j), hi.x, hi.y, hi.z, hi.w);
+                                sts128(b + swizzled(2 * n + 1, j), lo.x, lo.y, lo.z, lo.w);
+                            } else if (n < it.count)
+                                sts128(b + swizzled(n, j), x[u].x, x[u].y, x[u].z, x[u].w);
                         }
                     } else {
                         uint2 piece[kBatch][W::kPieces];

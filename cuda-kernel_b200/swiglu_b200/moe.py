@@ -5,8 +5,8 @@
 
 Ties go to the lowest index and a NaN logit counts as the largest. ``renormalize``: the
 softmax runs over the selected logits, so that a token's weights sum to one; else over all
-logits. In fp16 the product of the activations must lie within that type's range, or y is not
-finite. Like ``swiglu_out`` the call adds no bias and no residual, writes buffers the caller
+logits. The product of the activations keeps fp32's range in either type (swb_moe states its
+precision). Like ``swiglu_out`` the call adds no bias and no residual, writes buffers the caller
 owns, launches on the current CUDA stream and allocates nothing.
 """
 from __future__ import annotations

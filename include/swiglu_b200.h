@@ -341,10 +341,11 @@ SWB_API int swb_mx4_matmul(int type, const void* x_codes, const void* x_scales, 
  * (x_pitch elements from token to token), router [experts, hidden], y [tokens, hidden] and
  * of gate, up [experts, inter, hidden] and down [experts, hidden, inter]; with SWB_MOE_MX4
  * these three are four-bit codes (16-byte aligned) and *_scales their scales, else
- * *_scales are ignored. The router's sums are held in 64 bits, the others in fp32; the
- * product of the activations goes on as two values of `type` (rounded, and what the rounding
- * left) or, with SWB_MOE_MX4 and more than eight tokens, as three 8-bit values; with SWB_F16 it
- * must lie within fp16's range, or y is not finite. A token that holds a NaN or an infinity
+ * *_scales are ignored. The router's sums are held in 64 bits, the others in fp32. The product h
+ * of the activations keeps fp32's range; it goes on as two values of `type` (SWB_F16: after a power
+ * of two for each token and expert, within 2^-22 of itself and 2^-38 of that row's largest;
+ * SWB_BF16: within 2^-16) or, with SWB_MOE_MX4 and more than eight tokens, as three 8-bit values
+ * (within 2^-14 of the largest of its block of 32). A token that holds a NaN or an infinity
  * makes its y NaN or infinite, and leaves the others as they are. ids [tokens, topk] int32 and
  * weights [tokens, topk] fp32 receive the selection; either may be NULL.
  * One cooperative kernel, for more than eight tokens a second one after it, which fill the GPU.
