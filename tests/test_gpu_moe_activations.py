@@ -125,6 +125,47 @@ def test_range_of_activations(kind, four_bit, tokens, regime):
     within(y, want, bound)
 
 
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("tokens", [1, 8, 9, 33])
+def test_remainder_of_activations(kind, four_bit, tokens):
+    """Rows of down that cancel the rounded h, so that y consists of what the rounding left.
+
+    h of places i and i + 32 have one gate row and up rows 2^-6 apart; a row of down takes their
+    difference. x is -1, 0 or 1 and the matrices hold codes of two blocks, so that every partial sum
+    of gate and up is a multiple of 2^-7 below 2^9 and exact in fp32 in any order. The two places then
+    share the computed silu: its error scales y (2^-20), the product of h rounds once (2^-24 |h|)."""
+    dtype = TYPES[kind]
+    r = np.random.RandomState(5)
+    hidden, m = 64, 32
+    codes = np.array([.5, 1, 1.5, 2, 3, 4, 6])
+    x = r.randint(-1, 2, (tokens, hidden)).astype(np.float64)
+    x[:, 0], x[:, 32] = 1, 1
+    gate, up, down = (np.zeros((2, 2 * m, hidden)) for _ in range(3))
+    down = np.zeros((2, hidden, 2 * m))
+    for e in range(2):
+        gate[e, :m, :4] = codes[r.randint(0, 7, (m, 4))]
+        gate[e, m:] = gate[e, :m]
+        up[e, :m, :32] = codes[r.randint(0, 7, (m, 32))] * r.choice([-1, 1], (m, 32))
+        up[e, :m, 0] = 6
+        up[e, m:] = up[e, :m]
+        up[e, m:, 32] = codes[r.randint(0, 7, m)] * 2.0 ** -6
+        for row in range(hidden):
+            down[e, row, row % m], down[e, row, row % m + m] = 1, -1
+    d, v = put(dtype, four_bit, x, r.randn(2, hidden), gate=gate, up=up, down=down)
+    assert all(np.array_equal(v[k], w) for k, w in (("gate", gate), ("up", up), ("down", down), ("x", x)))
+    y, ids = call(d, 1)
+    e = ids.cpu().numpy()[:, 0]
+    g, u = np.stack([gate[k] @ t for k, t in zip(e, x)]), np.stack([up[k] @ t for k, t in zip(e, x)])
+    h = g / (1 + np.exp(-g)) * u
+    want = np.stack([down[k] @ t for k, t in zip(e, h)])
+    # of the two places: the product's rounding, what is kept; of their sum in the tensor core: two products
+    # of each of up to three parts, a truncation of 17 2^-24 each, and the parts' additions
+    dh = 2.0 ** -24 * np.abs(h) + kept(h, dtype, four_bit) + 7 * 17 * 2.0 ** -24 * np.abs(h)
+    bound = np.stack([np.abs(down[k]) @ t for k, t in zip(e, dh)]) + 2.0 ** -20 * np.abs(want)
+    within(y, want, bound)
+
+
 def test_calls_of_other_magnitudes_share_a_workspace():
     """Large, small and mixed activations, few and more tokens, routed alone or together, in turn on one
     workspace: the same bits as with a workspace of their own, call after call and in a graph."""
