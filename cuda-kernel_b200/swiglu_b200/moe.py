@@ -66,7 +66,7 @@ def moe_out(x: torch.Tensor, router: torch.Tensor, gate: torch.Tensor, up: torch
             raise RuntimeError("router, weights and y must be contiguous, of x's type and on its device")
         if t.requires_grad:
             raise RuntimeError("inference only: disable gradients")
-    _check(not x.requires_grad, "inference only: disable gradients")
+    _check(not x.requires_grad and (weights is None or not weights.requires_grad), "inference only: disable gradients")
     _check(y.shape == x.shape, "y must have x's shape")
     _check(workspace.device == device and workspace.dtype == torch.uint8 and workspace.is_contiguous(),
            "workspace must come from moe_workspace on x's device")

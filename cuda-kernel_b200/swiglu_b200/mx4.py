@@ -106,6 +106,7 @@ def mx4_dequantize_out(codes: torch.Tensor, scales: torch.Tensor, out: torch.Ten
     """The values of ``codes`` and ``scales`` into ``out`` [..., cols] (swb_mx4_dequantize); fp16
     rounds what its range does not hold."""
     _check(out.is_cuda and out.dtype in _TYPES and out.dim() >= 1, "out must be a CUDA FP16, BF16 or FP32 tensor")
+    _check(not out.requires_grad, "inference only: disable gradients")
     rows, cols, pitch = _rows(out, "out")
     _check_packed(codes, scales, out.shape[:-1], cols, out.device)
     _call(out.device, _lib.lib().swb_mx4_dequantize, _TYPES[out.dtype], codes.data_ptr(), scales.data_ptr(),
@@ -125,6 +126,8 @@ def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, cols: int | None =
 def _product_arguments(out, like, tokens, rows, bias, residual):
     if out.shape != (tokens, rows) or not out.is_contiguous():
         raise RuntimeError("out must be contiguous [tokens, rows]")
+    if out.requires_grad:
+        raise RuntimeError("inference only: disable gradients")
     for t, shape in ((bias, (rows,)), (residual, (tokens, rows))):
         if t is not None:
             if t.dtype != like or t.device != out.device or not t.is_contiguous() or t.shape != shape:
