@@ -20,11 +20,17 @@ from .mx4 import _TYPES, _call, _check_packed
 MAX_TOKENS = _lib.SWB_MOE_MAX_TOKENS
 
 
+def _check_sizes(tokens: int, experts: int, topk: int, inter: int) -> None:
+    """Here too, since the library's arguments are 32 bits wide and ctypes cuts longer ones."""
+    _check(0 <= tokens <= MAX_TOKENS and 0 < experts <= _lib.SWB_MOE_MAX_EXPERTS
+           and 0 < topk <= min(experts, _lib.SWB_MOE_MAX_TOPK) and 0 < inter <= _lib.SWB_MOE_MAX_DIM, "invalid shape")
+
+
 def moe_workspace(tokens: int, experts: int, topk: int, inter: int, device=None) -> torch.Tensor:
     """A zeroed workspace for calls of up to these sizes, one per stream of calls (calls that may
     overlap on the GPU, captured ones included, need one each)."""
+    _check_sizes(tokens, experts, topk, inter)
     n = _lib.lib().swb_moe_workspace_bytes(tokens, experts, topk, inter)
-    _check(n > 0, "invalid shape")
     return torch.zeros(n, dtype=torch.uint8, device=device or "cuda")
 
 
@@ -49,6 +55,8 @@ def moe_out(x: torch.Tensor, router: torch.Tensor, gate: torch.Tensor, up: torch
     _check(router.dim() == 2 and router.size(1) == hidden, "router must be [experts, hidden]")
     _check(gate.dim() == 3, "gate must be [experts, inter, hidden]")
     experts, inter = router.size(0), gate.size(1)
+    _check_sizes(tokens, experts, topk, inter)
+    _check(0 < hidden <= _lib.SWB_MOE_MAX_DIM, "invalid shape")
     four_bit = gate_scales is not None
     _check(four_bit == (up_scales is not None) == (down_scales is not None),
            "scales belong to all three matrices or to none")

@@ -41,3 +41,15 @@ def test_no_tensor_may_require_gradients():
         a = [t(2, 64, grad=i == 0), t(4, 64, grad=i == 1), t(4, 32, 64, grad=i == 2), t(4, 32, 64, grad=i == 3),
              t(4, 64, 32, grad=i == 4), t(2, 64, grad=i == 5)]
         refused(S.moe_out, *a, u8(1 << 20), 2, weights=t(2, 2, dtype=torch.float32, grad=i == 6), match=m)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Not cut to their low bits: 2^32 + 2 places are not two."""
+    big = 1 << 32
+    for sizes in ((1 + big, 8, 2, 64), (1, 8 + big, 2, 64), (1, 8, 2 + big, 64), (1, 8, 2, 64 + big),
+                  (1 - big, 8, 2, 64), (1, 8, 2 - big, 64)):
+        refused(S.moe_workspace, *sizes, device="cpu", match="invalid shape")
+    a = [t(2, 64), t(4, 64), t(4, 32, 64), t(4, 32, 64), t(4, 64, 32), t(2, 64), u8(1 << 20)]
+    for topk in (2 + big, 2 - big, 0, 5, 17):
+        refused(S.moe_out, *a, topk, match="invalid shape")
+    refused(S.moe, *a[:5], 2 + big, match="invalid shape")
