@@ -15,8 +15,8 @@
 // stages and its epilogue overlap with nothing.
 //
 // Roles: copies (TMA: 64 values of the tokens a stage, 256 of W's packed rows), decoding
-// warps in groups, stage about, products, eight epilogue warps. Two accumulators,
-// so that a tile's epilogue runs beside the next tile's products.
+// warps in groups, stage about, products, eight epilogue warps. Where a CTA takes several tiles,
+// two accumulators, so that a tile's epilogue runs beside the next tile's products.
 #include <algorithm>
 #include <cstring>
 
@@ -50,17 +50,20 @@ struct DeepShape {
     static constexpr int kThreads = (kDeepEpilogue + kDecoders + 2) * 32;
     static constexpr int kStagesA = N == 192 ? 4 : 5, kStagesB = N == 192 ? 3 : 8, kRaw = N == 192 ? 2 : 4;
     static_assert(kGroups <= kStagesB, "groups do not overtake the ring");
+    // 64 rows are taken while every CTA gets one tile at most (dispatch_deep).
+    static constexpr bool kOneTile = N == 64;
+    static constexpr int kAccs = kOneTile ? 1 : 2;
     // Tiles whose row factors are kept. Decoders that begin tile t have filled the ring with stages before
     // it, of which the products have finished all but the last kStagesB, tile t - 1 - kStagesB at least
     // (one stage a tile); those began when the epilogue had read two tiles before.
-    static constexpr int kFactors = kStagesB + 3;
+    static constexpr int kFactors = kOneTile ? 1 : kStagesB + 3;
     static constexpr int kStageA = kDeepM * 128, kStageB = N * 128, kRawStage = N * 128;
     static constexpr uint32_t kAtB = kStagesA * kStageA, kAtRaw = kAtB + kStagesB * kStageB;
     static constexpr uint32_t kAtTurn = kAtRaw + kRaw * kRawStage;
     static constexpr uint32_t kAtFactors = kAtTurn + kDeepEpilogue * 32 * kDeepPitch * 4;
     static constexpr size_t kSmem = kAtFactors + (kFactors + 1) * N * 4 + 1024;  // factors, and the current tile's largest scales
-    static constexpr int kColumns = N == 192 ? 512 : 128;  // two accumulators
-    static_assert(kSmem + 1024 <= kSmemPerCtaMax && 2 * N <= kColumns, "fits");
+    static constexpr int kColumns = N == 192 ? 512 : 64;
+    static_assert(kSmem + 1024 <= kSmemPerCtaMax && kAccs * N <= kColumns, "fits");
 };
 
 // The factor of a block in fp16: 2^(scale - top + 13), NaN for 255.
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(DeepShape<N>::kThreads, 1)
     constexpr int kDeepDecoders = S::kDecoders;
     extern __shared__ unsigned char raw_smem[];
     __shared__ uint64_t a_full[S::kStagesA], a_empty[S::kStagesA], b_full[S::kStagesB], b_empty[S::kStagesB];
-    __shared__ uint64_t raw_full[S::kRaw], raw_empty[S::kRaw], acc_full[2], acc_empty[2];
+    __shared__ uint64_t raw_full[S::kRaw], raw_empty[S::kRaw], acc_full[S::kAccs], acc_empty[S::kAccs];
     __shared__ uint32_t s_tmem;
     const uint32_t base = (smem_u32(raw_smem) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -119,7 +122,7 @@ __global__ void __launch_bounds__(DeepShape<N>::kThreads, 1)
         for (int i = 0; i < S::kStagesA; ++i) mbar_init(smem_u32(a_full + i), 1), mbar_init(smem_u32(a_empty + i), 1);
         for (int i = 0; i < S::kStagesB; ++i) mbar_init(smem_u32(b_full + i), S::kGroupWarps), mbar_init(smem_u32(b_empty + i), 1);
         for (int i = 0; i < S::kRaw; ++i) mbar_init(smem_u32(raw_full + i), 1), mbar_init(smem_u32(raw_empty + i), 4 * S::kGroupWarps);
-        for (int i = 0; i < 2; ++i) mbar_init(smem_u32(acc_full + i), 1), mbar_init(smem_u32(acc_empty + i), kDeepEpilogue);
+        for (int i = 0; i < S::kAccs; ++i) mbar_init(smem_u32(acc_full + i), 1), mbar_init(smem_u32(acc_empty + i), kDeepEpilogue);
         mbar_fence_init();
     }
     if (warp == 0) tmem_alloc(smem_u32(&s_tmem), S::kColumns);
@@ -170,7 +173,7 @@ __global__ void __launch_bounds__(DeepShape<N>::kThreads, 1)
             uint32_t pa = 0, pb = 0, pacc = 0;
             bool ok = true, have_a = false, have_b = false;
             for (int64_t tile = blockIdx.x; tile < P.items && ok; tile += gridDim.x, ++done) {
-                ok = done < 2 || mbar_wait(smem_u32(acc_empty + acc), pacc ^ 1u);
+                ok = done < S::kAccs || mbar_wait(smem_u32(acc_empty + acc), pacc ^ 1u);
                 for (int k = 0; k < stages && ok; ++k) {
                     ok = (have_a || mbar_wait(smem_u32(a_full + a), pa)) && (have_b || mbar_wait(smem_u32(b_full + b), pb));
                     if (!ok) break;
@@ -188,7 +191,7 @@ __global__ void __launch_bounds__(DeepShape<N>::kThreads, 1)
                     mma_commit(smem_u32(b_empty + bs));
                     if (k == stages - 1) mma_commit(smem_u32(acc_full + acc));
                 }
-                if (++acc == 2) acc = 0, pacc ^= 1u;
+                if (++acc == S::kAccs) acc = 0, pacc ^= 1u;
             }
         }
     } else if (warp >= kDeepEpilogue) {
@@ -348,7 +351,7 @@ __global__ void __launch_bounds__(DeepShape<N>::kThreads, 1)
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(acc_empty + acc));
-            if (++acc == 2) acc = 0, pacc ^= 1u;
+            if (++acc == S::kAccs) acc = 0, pacc ^= 1u;
             if (++slot == S::kFactors) slot = 0;
         }
     }
@@ -390,8 +393,16 @@ int dispatch_deep(const ProjectParams& P, cudaStream_t stream) {
 
 }  // namespace
 
-// Up to 32 tokens their pieces cost less than decoding W (14336 x 4096: 32 tokens 39.4 us against 44.6, 24
-// tokens 32.0 against 43.7), from 33 on more (64 tokens: 76.6 against 44.7).
+// Pieces up to 32 tokens, decoding W from 33 on. Both ways, us, pieces first:
+//                        24 tokens      32             33             64             128
+//   14336 x 4096  fp16   33.0  45.7     40.2  46.4     66.5  46.4     77.8  46.5    150.4  47.2
+//                 bf16   30.3  43.0     37.3  44.0     49.7  43.7     55.1  44.1    107.3  44.2
+//   5632 x 2048   fp16   14.4  19.4     17.0  14.8     20.9  15.0     24.5  14.8     42.0  15.1
+//                 bf16   13.7  17.7     16.1  14.4     17.6  14.7     19.8  14.5     31.6  14.7
+//   4096 x 14336  fp16   29.1  80.9     35.0  81.2     58.2  81.2     67.6  81.6    129.7  81.5
+//                 bf16   27.3  79.9     33.2  80.3     44.0  80.2     48.4  80.4     88.4  80.3
+// The border suits the first two; long rows in few tiles (64 CTAs of 224 stages, K is not split) would
+// gain from pieces to about 64 tokens.
 bool project_deep_takes(const ProjectParams& P) { return P.tokens > 32 && P.x_aligned; }
 
 int project_deep(int type, const ProjectParams& P, cudaStream_t stream) {
