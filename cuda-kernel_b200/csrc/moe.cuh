@@ -22,11 +22,14 @@
 //           the layer's type (split_pairs): 2^-22 of it is lost with fp16, 2^-16 with bf16.
 //
 // An expert with more than 32 tokens is taken in groups of 32, each group of a tile right
-// after the other, so that the second finds the weights in L2.
+// after the other, so that the second finds the weights in L2 (64 tokens through two experts read 147
+// MB from DRAM, 32 tokens 139).
 //
 // 40 us for the two experts that one token selects of 5632 x 2048 (fp16, 138 MB: 3.4 TB/s of the
 // 6.5 that a copy reaches); the router, its lists and the grid barrier take about 7 us of it, the
-// first and last stages of the two streams most of the rest.
+// first and last stages of the two streams most of the rest. Four-bit experts, one token: 37 us for 37 MB
+// (5632 x 2048; issue slots 32 % busy, DRAM 9 %, most stalls at barriers and waits) and 104 us for 187 MB
+// (14336 x 4096).
 #pragma once
 
 #include <type_traits>

@@ -11,8 +11,8 @@
 //   down   a cluster owns 128 rows of y; its CTAs take equal shares of the experts' steps along
 //          the intermediate dimension, keep y's sums in shared memory and add them in rank order.
 //
-// 16 tokens, 8 of 64 experts of 1376 x 2048, bf16: 192 us for 955 MB (146 at the copy rate); 2 of 8
-// of 8192 x 4096: 262 us, 93 % of it. Four bits, 32 tokens, 2 of 8 of 14336 x 4096: 248 us for
+// 16 tokens, 8 of 64 experts of 1376 x 2048: bf16 190 us, fp16 193 for 955 MB (146 at the copy rate); 2 of 8
+// of 8192 x 4096, bf16: 256 us, 95 % of it. Four bits, 32 tokens, 2 of 8 of 14336 x 4096: 251 us for
 // 749 MB (114): spreading codes and bringing tokens take turns with the products at each stage.
 #include <algorithm>
 #include <cstring>

@@ -11,8 +11,8 @@
 //          largest; a smaller value is off by at most 6 2^-38 of that scale (fp16's subnormals
 //          end there), 2^-37 of the largest value of a row that was rounded from 16 bits.
 //
-// 512 tokens by 5632 x 2048: 21.8 us, 540 TFLOP/s; one tile an SM, so that decoding its first
-// stages and its epilogue overlap with nothing.
+// 512 tokens by 5632 x 2048: 24.4 us, 480 TFLOP/s (22 with W in L2); one tile an SM, so that decoding
+// its first stages and its epilogue overlap with nothing.
 //
 // Roles: copies (TMA: 64 values of the tokens a stage, 256 of W's packed rows), decoding
 // warps in groups, stage about, products, eight epilogue warps. Where a CTA takes several tiles,

@@ -17,7 +17,8 @@
 // Few tokens (W on the M side, N = 16 to 128 tokens): bound by the bytes of W. The
 // CTAs of a cluster split K, so that every SM streams, and add their parts through
 // each other's shared memory in a fixed order.
-// 4096 tokens by 14336 x 4096: 167 us with a residual, 2.9 PFLOP/s. 16 tokens: 11 us for 31 MB.
+// 4096 tokens by 14336 x 4096 with a residual: 169 us, 2.85 PFLOP/s, a few launches at a time; 195 us,
+// 2.5, launched without a pause (the power cap lowers the clocks). 16 tokens: 13 us for 31 MB, 11 with W in L2.
 #include <algorithm>
 #include <cstring>
 
@@ -471,8 +472,10 @@ int dispatch_matmul(const Side& x, const Side& w, const MatmulParams& P, cudaStr
     if (P.tokens <= 16) return launch_matmul<T, 16, false>(x, w, P, stream);
     if (P.tokens <= 32) return launch_matmul<T, 32, false>(x, w, P, stream);
     if (P.tokens <= 64) return launch_matmul<T, 64, false>(x, w, P, stream);
-    // 65 to 128 tokens: a tile of tokens by 192 rows where that gives half the SMs one (14336 x 4096, 128
-    // tokens: 16.2 us against 20.1, 100 tokens: 15.7 against 18.2; 64 tokens: 15.1 against 14.2)
+    // 65 to 128 tokens: a tile of tokens by 192 rows where that gives half the SMs one (W in L2, us, fp16;
+    // bf16 within 0.4: 14336 x 4096, 65 tokens 16.8 against 17.4, 128 17.6 against 21.5), else W on the M side
+    // (4096 x 14336, 65 tokens 15.3 against 37.5, 128 17.7 against 39.1; 5632 x 2048, 65 tokens 10.8 against
+    // 11.3, but 128 13.3 against 11.3). 64 tokens by 14336 x 4096: W's side 16.3 against 16.7.
     if (P.tokens <= 128 && (P.rows + 191) / 192 * 2 < sm_count()) return launch_matmul<T, 128, false>(x, w, P, stream);
     return launch_matmul<T, 192, true>(x, w, P, stream);
 }

@@ -4,7 +4,7 @@
 // leaves SMs without work the CTAs of a cluster split K and add their parts through each other's
 // shared memory in rank order. Up to 16 tokens two CTAs share an SM, so that one's first bytes and
 // exchange run beside the other's stream.
-// 14336 x 4096, one token: 16.4 us for 31 MB, 4.8 at the copy rate; about half is launch, first
+// 14336 x 4096, one token: 16.6 us for 31 MB, 4.8 at the copy rate; about half is launch, first
 // bytes and exchange, the rest 16 stages a CTA, each a chain of waits, spreading and a product.
 #include <algorithm>
 #include <cstring>

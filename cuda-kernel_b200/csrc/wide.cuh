@@ -7,7 +7,8 @@
 // the sum of `pieces` e4m3 values, each block of 32 with a scale of its own, five binades apart,
 // rounded from what the piece before left. Three pieces hold an fp16 value exactly within 13
 // binades of its block's largest, and to 2^-27 of the largest below; two hold a bf16 value to
-// 2^-22 of it. A piece is a column of its own; the epilogue
+// 2^-22 of it; an fp32 value, such as an expert's h, is held to 2^-14 of it by three. A piece is a
+// column of its own; the epilogue
 // adds a token's columns. Every product is exact and the sums are the tensor core's fp32.
 //
 // Roles of a CTA, through two rings of stages of 128 bytes of every row (one for the weights, one

@@ -345,7 +345,8 @@ SWB_API int swb_mx4_matmul(int type, const void* x_codes, const void* x_scales, 
  * of the activations keeps fp32's range; it goes on as two values of `type` (SWB_F16: after a power
  * of two for each token and expert, within 2^-22 of itself and 2^-38 of that row's largest;
  * SWB_BF16: within 2^-16) or, with SWB_MOE_MX4 and more than eight tokens, as three 8-bit values
- * (within 2^-14 of the largest of its block of 32). A token that holds a NaN or an infinity
+ * (within 2^-14 of the largest of its block of 32; x is then held as swb_mx4_project holds up to 32
+ * tokens). A token that holds a NaN or an infinity
  * makes its y NaN or infinite, and leaves the others as they are. ids [tokens, topk] int32 and
  * weights [tokens, topk] fp32 receive the selection; either may be NULL.
  * One cooperative kernel, for more than eight tokens a second one after it, which fill the GPU.
