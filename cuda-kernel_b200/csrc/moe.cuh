@@ -14,12 +14,12 @@
 //           and sums in 64 bits, so that the selection does not depend on the order of
 //           a sum. The CTA that completes a group of four tokens selects their experts.
 //   gate    items (expert, 16 rows of Wg and Wu) spread over the CTAs; h goes to the
-//           workspace in fp32 with an expert's tokens side by side, for fp16 layers also the largest
-//           magnitude of each row.
+//           workspace with an expert's tokens side by side: fp16 layers in fp32, with the largest
+//           magnitude of each row, bf16 as two values (rounded, and what the rounding left).
 //   down    a CTA owns 16 rows of y at a time and takes every expert's product for
 //           them in expert order, so y needs no atomics and repeats bit for bit. Its
 //           weights are on their way while the grid waits for h. h is multiplied as two values of
-//           the layer's type (split_pairs): 2^-22 of it is lost with fp16, 2^-16 with bf16.
+//           the layer's type (row_unit): 2^-22 of it is lost with fp16, 2^-16 with bf16.
 //
 // An expert with more than 32 tokens is taken in groups of 32, each group of a tile right
 // after the other, so that the second finds the weights in L2 (64 tokens through two experts read 147
@@ -68,7 +68,8 @@ struct MoeParams {
     double* logits;  // [tokens, experts]
     int* picks;      // [tokens, topk]
     float* shares;   // [tokens, topk]
-    void* h;         // [tokens * topk, h_pitch] fp32 (moe_wide.cu: or what its second kernel's copies bring)
+    void* h;         // [tokens * topk, h_pitch], four bytes a value: fp32, or two parts of eight values after
+                     // another (bf16); moe_wide.cu: or what its second kernel's copies bring
     void* pieces;    // tokens split into e4m3 values (moe_wide.cu)
     int64_t x_pitch;
     int tokens, hidden, inter, experts, topk, h_pitch;
@@ -532,7 +533,15 @@ __global__ void __launch_bounds__(Stream<T, MX, NT>::kThreads, 1)
                     const float g = Pipe::template sum<2>(l, place, 0, n, r), u = Pipe::template sum<2>(l, place, 1, n, r);
                     // rows up to the pitch of h are zero, so that a whole piece of h may be read
                     if (row + r < P.inter) v = silu(g) * u;
-                    h[int64_t(start + n) * P.h_pitch + row + r] = v;
+                    float* to = h + int64_t(start + n) * P.h_pitch + row;
+                    if constexpr (kHalf) {
+                        to[r] = v;
+                    } else {
+                        T* parts = reinterpret_cast<T*>(to + (r & 8)) + (r & 7);
+                        const T hi = Num<T>::from_float(v);
+                        parts[0] = hi;
+                        parts[8] = Num<T>::from_float(v - Num<T>::to_float(hi));
+                    }
                 }
                 if constexpr (kHalf) {  // 16 lanes hold 16 places of a row
                     uint32_t top = __float_as_uint(v) & 0x7FFFFFFFu;

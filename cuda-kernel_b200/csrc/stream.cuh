@@ -76,36 +76,26 @@ struct Num<__nv_bfloat16> {
 };
 
 // A row of fp32 values goes through the tensor cores as two values of T: the nearest, and what the
-// rounding left, rounded. With fp16 the row is first divided by a unit, a power of two that brings
-// its largest value to [2^14, 2^15), so that fp32's range is kept and only values 2^-28 below the
-// largest meet fp16's subnormals (errors within 2^-39 of it); the sums are multiplied by the unit.
-// bf16 has fp32's range. `top`: the bits of the largest magnitude; NaN and infinity stay what they are.
+// rounding left, rounded. bf16 has fp32's range, and both are made where the value is. With fp16 the
+// row is first divided by a unit, a power of two that brings its largest value to [2^14, 2^15), so
+// that fp32's range is kept and only values 2^-28 below the largest meet fp16's subnormals (errors
+// within 2^-39 of it); the sums are multiplied by the unit. `top`: the bits of the largest
+// magnitude; NaN and infinity stay what they are.
 __device__ __forceinline__ float row_unit(uint32_t top) {
     const uint32_t e = top >> 23;
     return __uint_as_float((e > 254u ? 127u : max(e, 15u) - 14u) << 23);
 }
 __device__ __forceinline__ float unit_inverse(float unit) { return __uint_as_float((254u << 23) - __float_as_uint(unit)); }
-// Eight fp32 values times `up` (fp16) -> both parts.
-template <typename T>
+// Eight fp32 values times `up` -> both fp16 parts.
 __device__ __forceinline__ void split_pairs(const uint4& a, const uint4& b, float up, uint4& hi, uint4& lo) {
-    constexpr bool kHalf = std::is_same<T, __half>::value;
     const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     uint32_t h[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        float x = __uint_as_float(w[2 * i]), y = __uint_as_float(w[2 * i + 1]);
-        if constexpr (kHalf) x *= up, y *= up;  // exact
-        const auto one = [](float p, float q) {
-            uint32_t bits;
-            if constexpr (kHalf)
-                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(bits) : "f"(q), "f"(p));
-            else
-                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(bits) : "f"(q), "f"(p));
-            return bits;
-        };
-        h[i] = one(x, y);
-        const float2 back = kHalf ? half2_bits_to_float2(h[i]) : make_float2(__uint_as_float(h[i] << 16), __uint_as_float(h[i] & 0xFFFF0000u));
-        l[i] = one(x - back.x, y - back.y);
+        const float x = __uint_as_float(w[2 * i]) * up, y = __uint_as_float(w[2 * i + 1]) * up;  // exact
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[i]) : "f"(y), "f"(x));
+        const float2 back = half2_bits_to_float2(h[i]);
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(l[i]) : "f"(y - back.y), "f"(x - back.x));
     }
     hi = make_uint4(h[0], h[1], h[2], h[3]);
     lo = make_uint4(l[0], l[1], l[2], l[3]);
@@ -469,10 +459,10 @@ struct Stream {
     }
 
     // The tokens of an item as a consumer lane reads them: its row of each group of eight; with
-    // SPLIT, rows of fp32 values (zero up to a multiple of eight, `top`: row_unit), which are
-    // multiplied as two values of T. A warp takes every kConsumers-th unit of a stage and loads its
-    // tokens kGroup sub-steps of 32 values ahead, into the next item too: enough that they come from
-    // L2 in time.
+    // SPLIT, rows of 32 bytes for every eight values, which are multiplied as two values of T: fp32
+    // with fp16 (`top`: row_unit), eight first parts and eight second parts with bf16; zero up to a
+    // multiple of eight. A warp takes every kConsumers-th unit of a stage and loads its tokens kGroup
+    // sub-steps of 32 values ahead, into the next item too: enough that they come from L2 in time.
     template <int NM, bool SPLIT>
     struct Tokens {
         static constexpr int kRows = SPLIT ? 2 * NT : NT;
@@ -554,14 +544,15 @@ struct Stream {
                 uint4 now[kGroup][NP];
 #pragma unroll
                 for (int i = 0; i < kGroup; ++i) {
-                    if constexpr (SPLIT) {
+                    constexpr bool kFloat = SPLIT && std::is_same<T, __half>::value;
+                    if constexpr (kFloat) {
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
-                            if (n * 8 < count) split_pairs<T>(tokens.ahead[i][n], tokens.ahead[i][NT + n], up[n], now[i][n], now[i][NT + n]);
+                            if (n * 8 < count) split_pairs(tokens.ahead[i][n], tokens.ahead[i][NT + n], up[n], now[i][n], now[i][NT + n]);
                     }
 #pragma unroll
                     for (int n = 0; n < NP; ++n) {
-                        const uint4& v = SPLIT ? now[i][n] : tokens.ahead[i][n];
+                        const uint4& v = kFloat ? now[i][n] : tokens.ahead[i][n];
                         now[i][n] = MX ? Num<T>::order(v) : v;
                     }
                 }

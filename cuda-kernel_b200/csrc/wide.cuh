@@ -530,7 +530,7 @@ struct Wide {
                             if constexpr (W::kFloat) {
                                 if (n >= it.count) continue;
                                 uint4 hi, lo;
-                                split_pairs<T>(x[u], second[u], work.up(it, n), hi, lo);
+                                split_pairs(x[u], second[u], work.up(it, n), hi, lo);
                                 sts128(b + swizzled(2 * n, j), hi.x, hi.y, hi.z, hi.w);
                                 sts128(b + swizzled(2 * n + 1, j), lo.x, lo.y, lo.z, lo.w);
                             } else if (n < it.count)
